@@ -45,6 +45,11 @@ class TrainGeom(C.Structure):
                [(n, _i) for n in ("group_wgrads", "group_bm", "group_bn", "wgrad_flush_mask")]
 
 
+class PackedSeqs(C.Structure):
+    """capdec_packed_seqs of include/capdec.h."""
+    _fields_ = [(n, _i) for n in ("n", "causal", "rows_q", "rows_k")] + [("tiles", _i * 4), ("table", _vp)]
+
+
 TRAIN_LAYER_PARAMS = ("w_in", "b_in", "w_out", "b_out", "ln1_w", "ln1_b", "wc_in", "bc_in", "wc_out", "bc_out", "ln2_w", "ln2_b",
                       "w1", "b1", "w2", "b2", "ln3_w", "ln3_b")
 TRAIN_LAYER_COPIES = ("w_in16", "w_out16", "wcq16", "wc_out16", "w1_16", "w2_16")
@@ -105,6 +110,11 @@ SIGNATURES = {
     "capdec_attn_fwd_bf16": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _f, _u64, _vp]),
     "capdec_attn_bwd_bf16": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _i,
                                   _i, _i, _i, _i, _i, _i, _f, _f, _u64, _vp]),
+    "capdec_packed_table_bytes": (_sz, [C.POINTER(_i), C.POINTER(_i), _i]),
+    "capdec_packed_plan": (_i, [C.POINTER(_i), C.POINTER(_i), _i, _i, _vp, _sz, C.POINTER(PackedSeqs)]),
+    "capdec_attn_packed_fwd": (_i, [C.POINTER(PackedSeqs), _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _sz, _i, _i, _i, _i, _f, _vp]),
+    "capdec_attn_packed_bwd": (_i, [C.POINTER(PackedSeqs), _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _sz,
+                                    _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _f, _vp]),
     "capdec_softmax_ce": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _f, _f, _vp]),
     "capdec_gemm_ce_tiles": (_i, [_i, _i, _i, _i]),
     "capdec_ce_finalize": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _f, _vp]),

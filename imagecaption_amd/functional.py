@@ -165,6 +165,33 @@ class LayerNormFn(torch.autograd.Function):
         return dx.view(shape), dg, db, None, None, None, None
 
 
+class AttnPackedFn(torch.autograd.Function):
+    """Attention over packed sequences of different lengths, grouped heads (ops.attn_packed_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, Hq, Hkv, seqs, scale):
+        need = any(ctx.needs_input_grad)
+        o, lse = ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs, save_lse=need, scale=scale)
+        if need:
+            ctx.save_for_backward(q, k, v, o, lse)
+            ctx.meta = (Hq, Hkv, seqs, scale)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse = ctx.saved_tensors
+        Hq, Hkv, seqs, scale = ctx.meta
+        # the gradient may come in any layout: autograd promises values, not strides
+        do = do if do.stride(-1) == 1 and do.stride(0) == do.shape[1] and do.data_ptr() % 16 == 0 else do.contiguous()
+        dq, dk, dv = ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, scale=scale)
+        return dq, dk, dv, None, None, None, None
+
+
+def attn_packed(q, k, v, Hq, Hkv, seqs, scale=None):
+    """Differentiable ops.attn_packed_fwd: q [rows, Hq * dh], k / v [rows, Hkv * dh], ``seqs`` an ops.PackedSeqs -> o."""
+    return AttnPackedFn.apply(q, k, v, Hq, Hkv, seqs, scale)
+
+
 class SoftmaxCEFn(torch.autograd.Function):
     """Label-smoothed CE, mean over all rows (ref train.py:41-50); dlogits computed in the forward pass."""
 

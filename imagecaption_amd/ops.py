@@ -15,7 +15,7 @@ from ._capi import ACT_GELU_BWD, ACT_NONE, F32, check, lib, ptr, stream
 
 __all__ = ["compute_dtype", "gemm", "linear_fwd", "linear_dgrad", "linear_wgrad", "layernorm_fwd", "layernorm_bwd", "embed_fwd",
            "embed_bwd", "attn_fwd", "attn_bwd", "softmax_ce", "ce_tiles", "ce_finalize", "ce_dlogits", "ce_dlogits_bf16", "cast_bf16", "reduce_sum", "sumsq", "adamw", "clip_scale", "pe_add",
-           "act_dropout_bwd"]
+           "act_dropout_bwd", "PackedSeqs", "attn_packed_fwd", "attn_packed_bwd"]
 
 
 # Arithmetic type of the matrix products.  F32: exact fp32 MFMA (reference precision, the default).
@@ -922,6 +922,117 @@ def attn_bwd(q, k, v, o, do, lse, B, H, Tq, Tk, causal, drop_p=0.0, seed=0, dq=N
                                     ptr(dk),
                                     dk.stride(0), ptr(dv), dv.stride(0), B, H, Tq, Tk, dh, int(causal),
                                     1.0 / math.sqrt(dh), float(drop_p), int(seed), stream()), "capdec_attn_bwd")
+    return dq, dk, dv
+
+
+# ---- attention over packed sequences -----------------------------------------------------------------------------------
+class PackedSeqs:
+    """Lengths of the sequences that lie back to back in the rows of packed matrices, and the tile table that the packed
+    attention kernels walk on the device: made once for a set of lengths, used by every layer and both directions.
+    ``lengths_k`` None: keys / values have the queries' lengths.  ``causal``: row i of nq sees the rows j <= i + nk - nq
+    of its sequence.  Makes a blocking copy to ``device``: not under graph capture."""
+
+    def __init__(self, lengths_q, lengths_k=None, causal=True, device="cuda"):
+        lq = [int(v) for v in lengths_q]
+        lk = lq if lengths_k is None else [int(v) for v in lengths_k]
+        if not lq or len(lq) != len(lk) or min(min(lq), min(lk)) < 0 or max(sum(lq), sum(lk)) >= 1 << 31:
+            raise _capi.CapdecError("PackedSeqs: one length >= 0 for every sequence, under 2^31 rows together, as many for the "
+                                    "keys as for the queries")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise _capi.CapdecError(f"PackedSeqs: device {device}; the capdec ops run on the GPU only (no CPU fallback)")
+        self.lengths_q, self.lengths_k, self.causal = tuple(lq), tuple(lk), bool(causal)
+        self.rows_q, self.rows_k = sum(lq), sum(lk)
+        n = len(lq)
+        cq, ck = (C.c_int * n)(*lq), (C.c_int * n)(*lk)
+        l = lib()
+        self.table = torch.empty(l.capdec_packed_table_bytes(cq, ck, n), dtype=torch.uint8, device=device)
+        self.c = _capi.PackedSeqs()
+        with torch.cuda.device(self.table.device):
+            check(l.capdec_packed_plan(cq, ck, n, int(self.causal), ptr(self.table), self.table.numel(), C.byref(self.c)),
+                  "capdec_packed_plan")
+
+
+def _on_current(name, *tensors):
+    """Every tensor on the current device: its stream is the one the kernels are launched on."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != cur:
+            raise _capi.CapdecError(f"{name}: a tensor is on {t.device}, the current device is cuda:{cur}")
+
+
+def _packed_mat(t, name, dtype, rows, width):
+    _req(t, name, dtype)
+    piece = 16 // t.element_size()
+    if t.dim() != 2 or t.shape[1] != width or t.shape[0] < rows or (t.shape[0] > 0 and (
+            t.stride(1) != 1 or t.stride(0) < width or t.stride(0) % piece or t.data_ptr() % 16)):
+        raise _capi.CapdecError(f"{name}: need a 16-byte aligned [>= {rows}, {width}] matrix with unit column stride and a row "
+                                f"stride that is a multiple of {piece}, got {tuple(t.shape)} / {t.stride()}")
+    return t
+
+
+def _packed_args(name, q, k, v, Hq, Hkv, seqs, scale):
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise _capi.CapdecError(f"{name}: q is {q.dtype}: fp32 or bf16 matrices")
+    if Hkv <= 0 or Hq <= 0 or Hq % Hkv or q.dim() != 2 or q.shape[1] % Hq or q.shape[1] // Hq not in (64, 128):
+        raise _capi.CapdecError(f"{name}: {tuple(q.shape)} with Hq={Hq}, Hkv={Hkv}: Hq a multiple of Hkv, heads of 64 or 128")
+    dh = q.shape[1] // Hq
+    _packed_mat(q, name + ".q", q.dtype, seqs.rows_q, Hq * dh)
+    _packed_mat(k, name + ".k", q.dtype, seqs.rows_k, Hkv * dh), _packed_mat(v, name + ".v", q.dtype, seqs.rows_k, Hkv * dh)
+    _on_current(name, q, k, v, seqs.table)
+    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise _capi.CapdecError(f"{name}: scale {scale} must be positive and finite")
+    return dh, F32 if q.dtype == torch.float32 else _capi.BF16S, scale
+
+
+def attn_packed_fwd(q, k, v, Hq, Hkv, seqs, out=None, save_lse=True, scale=None):
+    """Attention over packed sequences: q [>= rows_q, Hq * dh], k / v [>= rows_k, Hkv * dh] (row-strided views, all fp32 or
+    all bf16, dh 64 or 128), ``seqs`` a PackedSeqs.  Returns (o, lse [Hq, rows of q] or None).  Rows behind the last sequence
+    stay as they are in a given ``out`` and are zeros in a new one."""
+    dh, dtype, scale = _packed_args("attn_packed_fwd", q, k, v, Hq, Hkv, seqs, scale)
+    if out is None:
+        out = torch.empty((q.shape[0], Hq * dh), dtype=q.dtype, device=q.device)
+        if q.shape[0] > seqs.rows_q:
+            out[seqs.rows_q:].zero_()
+    else:
+        _packed_mat(out, "attn_packed_fwd.out", q.dtype, seqs.rows_q, Hq * dh)
+        _on_current("attn_packed_fwd", out)
+    lse = torch.empty((Hq, q.shape[0]), dtype=torch.float32, device=q.device) if save_lse else None
+    if save_lse and q.shape[0] > seqs.rows_q:
+        lse[:, seqs.rows_q:].zero_()
+    check(lib().capdec_attn_packed_fwd(C.byref(seqs.c), ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0), ptr(out),
+                                       out.stride(0), ptr(lse), q.shape[0], Hq, Hkv, dh, dtype, scale, stream()),
+          "capdec_attn_packed_fwd")
+    return out, lse
+
+
+def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=None, scale=None):
+    """(dq, dk, dv) of attn_packed_fwd; ``o`` / ``lse`` are its results, ``do`` the gradient of o.  Given dq / dk / dv are
+    written in place, rows behind the last sequence stay as they are there and are zeros in new ones."""
+    name = "attn_packed_bwd"
+    dh, dtype, scale = _packed_args(name, q, k, v, Hq, Hkv, seqs, scale)
+    _packed_mat(o, name + ".o", q.dtype, seqs.rows_q, Hq * dh), _packed_mat(do, name + ".do", q.dtype, seqs.rows_q, Hq * dh)
+    _req(lse, name + ".lse")
+    if lse.dim() != 2 or lse.shape[0] != Hq or lse.shape[1] < seqs.rows_q or not lse.is_contiguous():
+        raise _capi.CapdecError(f"{name}: lse {tuple(lse.shape)} must be the contiguous [Hq, rows] block that attn_packed_fwd returned")
+    out = []
+    for t, n, like, rows, width in ((dq, ".dq", q, seqs.rows_q, Hq * dh), (dk, ".dk", k, seqs.rows_k, Hkv * dh),
+                                    (dv, ".dv", v, seqs.rows_k, Hkv * dh)):
+        if t is None:
+            t = torch.empty((like.shape[0], width), dtype=q.dtype, device=q.device)
+            if like.shape[0] > rows:
+                t[rows:].zero_()
+        else:
+            _packed_mat(t, name + n, q.dtype, rows, width)
+        out.append(t)
+    _on_current(name, o, do, lse, *out)
+    delta = torch.empty_like(lse)
+    dq, dk, dv = out
+    check(lib().capdec_attn_packed_bwd(C.byref(seqs.c), ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0), ptr(o),
+                                       o.stride(0), ptr(do), do.stride(0), ptr(lse), ptr(delta), lse.shape[1], ptr(dq), dq.stride(0),
+                                       ptr(dk), dk.stride(0), ptr(dv), dv.stride(0), Hq, Hkv, dh, dtype, scale, stream()),
+          "capdec_attn_packed_bwd")
     return dq, dk, dv
 
 

@@ -343,6 +343,42 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
                          void* dk16, int lddk, void* dv16, int lddv, int B, int H, int Tq, int Tk, int dh, int causal,
                          float scale, float drop_p, uint64_t drop_seed, capdec_stream_t stream);
 
+/* ---- attention over packed sequences ----------------------------------------------------------------------------
+ * Sequences of different lengths lie back to back in the rows of one matrix (no padding): sequence i owns lens_q[i]
+ * rows of q / o and lens_k[i] rows of k / v.  Hq query heads share Hkv key / value heads (Hq a multiple of Hkv; query
+ * head h reads key / value head h / (Hq / Hkv)); element (row, head, j) lives at ptr[row * ld + head * dh + j].
+ *   o[i,h,:] = sum_j softmax_j(scale q[i,h,:].k[j,h',:]) v[j,h',:] over the rows j of i's own sequence; causal: row i of
+ *   nq sees the rows j <= i + nk - nq.  A row that sees nothing (lens_k = 0, or causal with nk < nq) gets o = 0 and
+ *   lse = -inf, and gradients of zero.  Rows behind the last sequence are not touched.
+ *   lse / delta: fp32 [Hq, stat_rows], entry head * stat_rows + row; lse (natural log-sum-exp of the scaled scores) may be
+ *   NULL in fwd; delta is scratch that bwd fills (rowsum(do * o)).
+ *   bwd: dq, dk, dv from do; dk / dv sum over the query heads of their group.  No atomics: bitwise reproducible.
+ * dtype CAPDEC_F32: every matrix fp32, exact fp32 products; CAPDEC_BF16S: every matrix bf16, fp32 accumulation, softmax and
+ * statistics, probabilities and score gradients rounded to bf16 for the products that take them (the only roundings
+ * besides the results').  dh in {64, 128}; 16-byte aligned matrices, row strides multiples of 16 bytes.  Non-finite values:
+ * the products are plain ones (0 x inf = NaN), so an infinity or NaN in v reaches the rows of ITS sequence that share a
+ * tile with it even where they are masked; it never reaches another sequence.
+ * The plan: capdec_packed_plan checks the lengths (host arrays; lens_k = NULL: the same as lens_q), writes the tile table to
+ * table_dev (capdec_packed_table_bytes bytes of device memory, 16-byte aligned; a blocking copy: once for a set of lengths,
+ * not under capture) and fills *seqs, which every later call with these lengths takes -- all layers, both directions.
+ * The padded form of the same attention is capdec_attn_fwd / _bwd (torch/nn/functional.py:6386-6390, 6613-6631); the
+ * reference pads every caption to one length (ref dataset.py:213-228). */
+typedef struct capdec_packed_seqs {
+    int n, causal, rows_q, rows_k;
+    int tiles[4]; /* query tiles of 128 / 32 rows, key tiles of 128 / 32 rows */
+    const void* table;
+} capdec_packed_seqs;
+size_t capdec_packed_table_bytes(const int* lens_q, const int* lens_k, int n); /* 0: bad lengths */
+int capdec_packed_plan(const int* lens_q, const int* lens_k, int n, int causal, void* table_dev, size_t table_bytes,
+                       capdec_packed_seqs* seqs);
+int capdec_attn_packed_fwd(const capdec_packed_seqs* seqs, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
+                           void* o, int ldo, void* lse, size_t stat_rows, int Hq, int Hkv, int dh, int dtype, float scale,
+                           capdec_stream_t stream);
+int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
+                           const void* o, int ldo, const void* dout, int lddo, const void* lse, void* delta, size_t stat_rows,
+                           void* dq, int lddq, void* dk, int lddk, void* dv, int lddv, int Hq, int Hkv, int dh, int dtype,
+                           float scale, capdec_stream_t stream);
+
 /* ---- label-smoothed softmax cross-entropy, forward + backward in one pass -------------------------
  * Per row m of logits [M,V] (row stride ldl) with target y = targets[m] (int64):
  *   loss_rows[m] = lse(z) - (1-eps)*z_y - (eps/V)*sum_v z_v

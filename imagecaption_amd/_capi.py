@@ -11,10 +11,10 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CAPDEC_LIBRARY") or os.path.join(_HERE, "libcapdec.so")  # override: kernel experiments
 
-F32, BF16, F32X3, BF16S = 0, 1, 2, 3
+F32, BF16, F32X3, BF16S, E4M3 = 0, 1, 2, 3, 4
 ACT_NONE, ACT_GELU, ACT_GELU_BWD = 0, 1, 2
 
-_vp, _i, _f, _u64, _sz = C.c_void_p, C.c_int, C.c_float, C.c_uint64, C.c_size_t
+_vp, _i, _f, _u64, _sz, _i64 = C.c_void_p, C.c_int, C.c_float, C.c_uint64, C.c_size_t, C.c_int64
 
 
 class Epilogue(C.Structure):
@@ -48,6 +48,11 @@ class TrainGeom(C.Structure):
 class PackedSeqs(C.Structure):
     """capdec_packed_seqs of include/capdec.h."""
     _fields_ = [(n, _i) for n in ("n", "causal", "rows_q", "rows_k")] + [("tiles", _i * 4), ("table", _vp)]
+
+
+class KVCache(C.Structure):
+    """capdec_kv_cache of include/capdec.h."""
+    _fields_ = [(n, _vp) for n in ("k", "v", "k_scale", "v_scale")] + [(n, _i) for n in ("pages", "heads", "page", "dh", "dtype")]
 
 
 TRAIN_LAYER_PARAMS = ("w_in", "b_in", "w_out", "b_out", "ln1_w", "ln1_b", "wc_in", "bc_in", "wc_out", "bc_out", "ln2_w", "ln2_b",
@@ -115,6 +120,12 @@ SIGNATURES = {
     "capdec_attn_packed_fwd": (_i, [C.POINTER(PackedSeqs), _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _sz, _i, _i, _i, _i, _f, _vp]),
     "capdec_attn_packed_bwd": (_i, [C.POINTER(PackedSeqs), _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _sz,
                                     _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _f, _vp]),
+    "capdec_kv_write": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _i, _i, _vp, _i, _vp]),
+    "capdec_kv_read": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _i, _vp, _i, _i, _vp]),
+    "capdec_attn_paged_workspace_bytes": (_sz, [C.POINTER(KVCache), _i, _i, _i, _i, _i]),
+    "capdec_attn_paged": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _vp, _vp, _sz, _vp]),
+    "capdec_kv_bad_pages": (_i, [C.POINTER(C.c_uint), _i]),
+    "capdec_draft_verify": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i64, _vp, _vp, _vp]),
     "capdec_softmax_ce": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _f, _f, _vp]),
     "capdec_gemm_ce_tiles": (_i, [_i, _i, _i, _i]),
     "capdec_ce_finalize": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _f, _vp]),

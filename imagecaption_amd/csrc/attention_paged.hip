@@ -1,0 +1,632 @@
+// Attention of new tokens over a paged cache.  See include/capdec.h (capdec_attn_paged).
+//
+// The rows of a (sequence, key / value head) are its new tokens times the query heads of the group: they all read the same
+// keys, so they share a tile.  Two kernels, both over (sequence, key / value head, split of the keys, tile of rows):
+//   paged_keys_kernel  few rows (decode steps, drafted tokens): bound by the cache's bytes.  A tile of 32 or 64 rows; each of
+//                      the four waves streams every fourth run of 32 keys through an LDS image of its own (global ->
+//                      registers one run ahead -> LDS, no barrier in the loop) and the waves join at the end.
+//   paged_rows_kernel  many rows (chunks of a prompt): bound by the matrix products.  A tile of 128 rows, 32 a wave; 64
+//                      keys at a time are shared by the waves through LDS.
+// e4m3 codes become bf16 (exactly) on their way into LDS; a key's scale multiplies its scores, a value's scale its weights.
+// Splits leave (maximum, sum, unnormalised context) in fp32 and a second launch joins them; a sequence short enough for one
+// split writes its result at once.
+#include <algorithm>
+
+#include "attention_tile.h"
+#include "paged.h"
+
+namespace capdec {
+
+static __device__ unsigned int g_bad_pages;
+
+constexpr int SPLIT_KEYS = 8192;             // most keys of a split: its page ids fit LDS
+constexpr int SPLIT_IDS = SPLIT_KEYS / 8 + 2;
+constexpr int SPLIT_MIN = 256;               // fewest keys worth a split of their own
+
+struct PagedParams {
+    const void* k; const void* v; const float* ks; const float* vs;
+    const __bf16* q; __bf16* o; float* lse;
+    const int* cu; const int* lens; const int* table;
+    float* part_o; float2* part_ml; int* part_n;
+    int ldq, ldo, ld_table, cols, n, rows, Hq, Hkv, group, page_log2, pages;
+    int splits, tiles;
+    float scale;
+};
+
+// what a workgroup works on
+struct PagedItem {
+    int seq, hk, split, tile;
+    int a, nq, len, kbegin, kend, nsplit;  // rows a .. a + nq - 1; keys kbegin .. kend - 1 of len
+    bool ok;
+};
+
+// keys of one split of a sequence of `len` keys: as many splits as there are, of at least SPLIT_MIN keys, in whole runs of 128
+__device__ __forceinline__ int split_size(int len, int splits) {
+    int c = (len + splits - 1) / splits;
+    c = max(c, SPLIT_MIN);
+    return (c + 127) & ~127;
+}
+
+__device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
+    // the row tiles of one (sequence, head, split) read the same keys: they sit on one XCD (blockIdx % 8)
+    PagedItem w;
+    const int blk = blockIdx.x, idx = blk >> 3;
+    w.tile = idx % p.tiles;
+    const int u = (idx / p.tiles) * 8 + (blk & 7);
+    w.ok = u < p.n * p.Hkv * p.splits;
+    w.split = u % p.splits;
+    const int sh = u / p.splits;
+    w.hk = sh % p.Hkv;
+    w.seq = w.ok ? sh / p.Hkv : 0;
+    if (p.cu) {
+        w.a = min(max(p.cu[w.seq], 0), p.rows);
+        w.nq = min(max(p.cu[w.seq + 1], w.a), p.rows) - w.a;
+    } else {
+        w.a = w.seq;
+        w.nq = 1;
+    }
+    const int cap = p.cols << p.page_log2;
+    const int len = p.lens[w.seq];
+    w.len = min(max(len, 0), cap);
+    if (len > cap && w.split == 0 && w.tile == 0 && w.hk == 0 && threadIdx.x == 0 && w.ok) atomicAdd(&g_bad_pages, 1u);
+    const int size = split_size(w.len, p.splits);
+    w.nsplit = max(1, (w.len + size - 1) / size);
+    w.kbegin = w.split * size;
+    w.kend = min(w.len, w.kbegin + size);
+    w.ok = w.ok && w.split < w.nsplit;
+    return w;
+}
+
+// the split's page ids into LDS; ids outside the cache become -1 and are counted
+__device__ __forceinline__ void load_ids(int* ids, const PagedParams& p, const PagedItem& w, int tid, int nt) {
+    const int first = w.kbegin >> p.page_log2, n = w.kend > w.kbegin ? ((w.kend - 1) >> p.page_log2) - first + 1 : 0;
+    const int* row = p.table + (size_t)w.seq * p.ld_table + first;
+    for (int i = tid; i < n; i += nt) {
+        int id = row[i];
+        if (id < 0 || id >= p.pages) {
+            id = -1;
+            if (w.hk == 0 && w.tile == 0) atomicAdd(&g_bad_pages, 1u);
+        }
+        ids[i] = id;
+    }
+}
+
+// ROWS keys (or values) of one head on their way pages -> registers -> LDS image, shared out over NT threads in 16-byte
+// pieces; positions past the split's end or on a bad page become zeros
+template <bool E4M3, int DH, int NT, int ROWS>
+struct PageStage {
+    using L = AttTile<__bf16, DH>;
+    static constexpr int RB = E4M3 ? DH : 2 * DH, PP = RB / 16, N = (ROWS * PP + NT - 1) / NT;
+    static_assert(ROWS * PP % NT == 0, "every thread moves the same number of pieces");
+    uint4 r[N];
+    __device__ __forceinline__ void load(const void* base, const int* ids, int first_page, int head, int heads, int page_log2, int key0,
+                                         int kend, int tid) {
+        const int mask = (1 << page_log2) - 1;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int key = key0 + (j * NT + tid) / PP, piece = (j * NT + tid) % PP;
+            r[j] = uint4{0, 0, 0, 0};
+            if (key < kend) {
+                const int id = ids[(key >> page_log2) - first_page];
+                if (id >= 0)
+                    r[j] = *reinterpret_cast<const uint4*>((const unsigned char*)base +
+                                                           ((((size_t)id * heads + head) << page_log2) + (key & mask)) * RB + piece * 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* img, int tid) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int row = (j * NT + tid) / PP, piece = (j * NT + tid) % PP;
+            unsigned char* at = img + row * L::ROWB;
+            if constexpr (E4M3) {
+                *reinterpret_cast<bf16x8p*>(at + (((2 * piece) ^ L::swz(row)) << 4)) = e4m3_to_bf16(r[j].x, r[j].y);
+                *reinterpret_cast<bf16x8p*>(at + (((2 * piece + 1) ^ L::swz(row)) << 4)) = e4m3_to_bf16(r[j].z, r[j].w);
+            } else {
+                *reinterpret_cast<uint4*>(at + ((piece ^ L::swz(row)) << 4)) = r[j];
+            }
+        }
+    }
+};
+
+// key `key`'s scale of one head; zero past the split's end or on a bad page.  *there: the position exists
+__device__ __forceinline__ void key_scales(const PagedParams& p, const int* ids, int first_page, int head, int key, int kend, bool e4m3,
+                                           float& sk, float& sv, bool& there) {
+    sk = sv = 0.f;
+    there = false;
+    if (key < kend) {
+        const int id = ids[(key >> p.page_log2) - first_page];
+        there = id >= 0;
+        if (there && e4m3) {
+            const size_t at = (((size_t)id * p.Hkv + head) << p.page_log2) + (key & ((1 << p.page_log2) - 1));
+            sk = p.ks[at];
+            sv = p.vs[at];
+        }
+    }
+}
+
+// Orders a wave's LDS writes before other lanes' reads (and reads before the next writes) for the compiler; the hardware
+// executes one wave's LDS operations in order, so nothing is waited for.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// R blocks of 32 rows; every wave walks its own runs of 32 keys
+template <bool E4M3, int DH, int R>
+__global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedParams p) {
+    using L = AttTile<__bf16, DH>;
+    constexpr int IMG = 32 * L::ROWB;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[8 * IMG];
+    __shared__ int ids[SPLIT_IDS];
+    __shared__ __attribute__((aligned(16))) float sc[4][2][32];
+    __shared__ float ml[4][2][32];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const PagedItem w = paged_place(p);
+    if (!w.ok) return;
+    const int nrows = w.nq * p.group;
+    load_ids(ids, p, w, tid, 256);
+    __syncthreads();
+    const int first_page = w.kbegin >> p.page_log2;
+    const typename L::lanes ln = L::make_lanes(lane);
+    const float c = p.scale * LOG2E;
+    unsigned char* Ks = smem + wave * 2 * IMG;
+    unsigned char* Vs = Ks + IMG;
+
+    for (int tile = w.tile; tile * 32 * R < nrows; tile += p.tiles) {
+        int see[R], lo_see = 0x7fffffff;
+        typename L::frag qf[R][L::NF];
+#pragma unroll
+        for (int b = 0; b < R; ++b) {
+            const int r = tile * 32 * R + b * 32 + l31, token = r / p.group, g = r % p.group;
+            see[b] = w.len - w.nq + token + 1;
+            lo_see = min(lo_see, w.len - w.nq + (tile * 32 * R + b * 32) / p.group + 1);
+            L::load_row(qf[b], p.q + (size_t)(w.a + token) * p.ldq + (w.hk * p.group + g) * DH, r < nrows, half);
+        }
+        f32x16 acc[R][L::NDT];
+        Running run[R];
+#pragma unroll
+        for (int b = 0; b < R; ++b) {
+            run[b].init();
+#pragma unroll
+            for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[b][dt]);
+        }
+        PageStage<E4M3, DH, 64, 32> ks, vs;
+        float sk, sv;
+        bool there;
+        int k0 = w.kbegin + wave * 32;
+        if (k0 < w.kend) {
+            ks.load(p.k, ids, first_page, w.hk, p.Hkv, p.page_log2, k0, w.kend, lane);
+            vs.load(p.v, ids, first_page, w.hk, p.Hkv, p.page_log2, k0, w.kend, lane);
+            key_scales(p, ids, first_page, w.hk, k0 + l31, w.kend, E4M3, sk, sv, there);
+        }
+        for (; k0 < w.kend; k0 += 128) {
+            // one wave's LDS operations execute in order: the previous run's reads are done before these writes land
+            ks.store(Ks, lane);
+            vs.store(Vs, lane);
+            if (E4M3 && half == 0) {
+                sc[wave][0][l31] = sk;
+                sc[wave][1][l31] = sv;
+            }
+            const uint32_t exists = (uint32_t)__ballot(there);
+            if (k0 + 128 < w.kend) {
+                ks.load(p.k, ids, first_page, w.hk, p.Hkv, p.page_log2, k0 + 128, w.kend, lane);
+                vs.load(p.v, ids, first_page, w.hk, p.Hkv, p.page_log2, k0 + 128, w.kend, lane);
+                key_scales(p, ids, first_page, w.hk, k0 + 128 + l31, w.kend, E4M3, sk, sv, there);
+            }
+            wave_fence();
+            const bool plain = exists == 0xffffffffu && k0 + 32 <= lo_see;
+#pragma unroll
+            for (int b = 0; b < R; ++b) {
+                f32x16 s;
+                zero16(s);
+                L::mma_rows(s, Ks, ln, qf[b]);  // S^T[key][row]
+                if constexpr (E4M3) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4t f = *reinterpret_cast<const f32x4t*>(&sc[wave][0][8 * i + 4 * half]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[4 * i + j] *= f[j];
+                    }
+                }
+                if (!plain) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int kr = row_of(r, half);
+                        s[r] = ((exists >> kr) & 1) && k0 + kr < see[b] ? s[r] : -INFINITY;
+                    }
+                }
+                float top = s[0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+                bool raised;
+                const float a = run[b].raise(top, c, &raised);
+                if (raised) {
+#pragma unroll
+                    for (int dt = 0; dt < L::NDT; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[b][dt][r] *= a;
+                }
+                const float base = run[b].base();
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f32x4t f = {1.f, 1.f, 1.f, 1.f};
+                    if constexpr (E4M3) f = *reinterpret_cast<const f32x4t*>(&sc[wave][1][8 * i + 4 * half]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float e = exp2_fast(__fmaf_rn(s[4 * i + j], c, -base));
+                        run[b].l += e;
+                        x[4 * i + j] = E4M3 ? e * f[j] : e;
+                    }
+                }
+                typename L::weights pw;
+                L::pack(pw, x);
+                L::mma_cols(acc[b], Vs, ln, pw);
+            }
+            wave_fence();
+        }
+        // join the four waves: statistics first, then the contexts through their (now free) images, in wave order
+        constexpr int PIECES = DH / 4;  // 16-byte pieces of an fp32 row
+#pragma unroll
+        for (int b = 0; b < R; ++b) {
+            const float l = run[b].l + __shfl_xor(run[b].l, 32, 64);
+            if (half == 0) {
+                ml[wave][0][l31] = run[b].m2;
+                ml[wave][1][l31] = l;
+            }
+            __syncthreads();
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, ml[i][0][l31]);
+            const float mine = run[b].m2 == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_fast(run[b].m2 - m);
+            float* ctx = reinterpret_cast<float*>(smem + wave * 2 * IMG);
+#pragma unroll
+            for (int dt = 0; dt < L::NDT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int piece = dt * 8 + 2 * i + half;
+                    const f32x4t v = {acc[b][dt][4 * i] * mine, acc[b][dt][4 * i + 1] * mine, acc[b][dt][4 * i + 2] * mine,
+                                      acc[b][dt][4 * i + 3] * mine};
+                    *reinterpret_cast<f32x4t*>(ctx + l31 * DH + ((piece ^ (l31 & 15)) << 2)) = v;
+                }
+            __syncthreads();
+            const int rl = tid >> 3, r = tile * 32 * R + b * 32 + rl;  // eight threads a row
+            if (r < nrows) {
+                float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mm = fmaxf(mm, ml[i][0][rl]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float mi = ml[i][0][rl], li = ml[i][1][rl];
+                    ll += mi == -INFINITY ? li : li * exp2_fast(mi - mm);
+                }
+                const int token = r / p.group, head = w.hk * p.group + r % p.group, grow = w.a + token;
+                const bool any = ll != 0.f;
+                const size_t at = (size_t)grow * p.Hq + head;
+                const float inv = w.nsplit == 1 ? (any ? 1.f / ll : 0.f) : 1.f;
+                float* po = p.part_o + ((size_t)w.split * p.rows * p.Hq + at) * DH;
+#pragma unroll
+                for (int j = 0; j < PIECES / 8; ++j) {
+                    const int piece = j * 8 + (tid & 7);
+                    f32x4t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        v += *reinterpret_cast<const f32x4t*>(reinterpret_cast<const float*>(smem + i * 2 * IMG) + rl * DH + ((piece ^ (rl & 15)) << 2));
+                    if (w.nsplit == 1) {
+                        const bf16x4t out = {(__bf16)(v[0] * inv), (__bf16)(v[1] * inv), (__bf16)(v[2] * inv), (__bf16)(v[3] * inv)};
+                        *reinterpret_cast<bf16x4t*>(p.o + (size_t)grow * p.ldo + head * DH + piece * 4) = out;
+                    } else {
+                        *reinterpret_cast<f32x4t*>(po + piece * 4) = v;
+                    }
+                }
+                if ((tid & 7) == 0) {
+                    if (w.nsplit == 1) {
+                        if (p.lse) p.lse[(size_t)head * p.rows + grow] = any ? ((mm == -INFINITY ? 0.f : mm) + __log2f(ll)) * LN2 : -INFINITY;
+                    } else {
+                        p.part_ml[(size_t)w.split * p.rows * p.Hq + at] = float2{mm, ll};
+                    }
+                    if (w.split == 0 && p.part_n) p.part_n[at] = w.nsplit;
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// 128 rows, 32 a wave; 64 keys at a time shared by the waves
+template <bool E4M3, int DH>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
+    using L = AttTile<__bf16, DH>;
+    constexpr int KB = 2, BN = 32 * KB, IMG = BN * L::ROWB;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
+    __shared__ int ids[SPLIT_IDS];
+    __shared__ __attribute__((aligned(16))) float sc[2][2][BN];
+    __shared__ uint32_t exist[2][KB];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const PagedItem w = paged_place(p);
+    if (!w.ok) return;
+    const int nrows = w.nq * p.group;
+    load_ids(ids, p, w, tid, 256);
+    const int first_page = w.kbegin >> p.page_log2;
+    const typename L::lanes ln = L::make_lanes(lane);
+    const float c = p.scale * LOG2E;
+    for (int tile = w.tile; tile * 128 < nrows; tile += p.tiles) {
+        const int r0 = tile * 128 + wave * 32, r = r0 + l31, token = r / p.group, head = w.hk * p.group + r % p.group;
+        const int see = w.len - w.nq + token + 1;
+        const int all_see = w.len - w.nq + r0 / p.group + 1;
+        const int wave_end = r0 < nrows ? min(w.kend, w.len - w.nq + min(r0 + 31, nrows - 1) / p.group + 1) : 0;
+        const int end = min(w.kend, w.len - w.nq + min(tile * 128 + 127, nrows - 1) / p.group + 1);
+        const int nt = end > w.kbegin ? (end - w.kbegin + BN - 1) / BN : 0;
+        typename L::frag qf[L::NF];
+        L::load_row(qf, p.q + (size_t)(w.a + token) * p.ldq + head * DH, r < nrows, half);
+        f32x16 acc[L::NDT];
+#pragma unroll
+        for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
+        Running run;
+        run.init();
+        PageStage<E4M3, DH, 256, BN> ks, vs;
+        float sk, sv;
+        bool there = false;
+        auto fetch = [&](int t) {
+            const int k0 = w.kbegin + t * BN;
+            ks.load(p.k, ids, first_page, w.hk, p.Hkv, p.page_log2, k0, w.kend, tid);
+            vs.load(p.v, ids, first_page, w.hk, p.Hkv, p.page_log2, k0, w.kend, tid);
+            if (tid < BN) key_scales(p, ids, first_page, w.hk, k0 + tid, w.kend, E4M3, sk, sv, there);
+        };
+        auto put = [&](int t) {
+            unsigned char* img = smem + (t & 1) * 2 * IMG;
+            ks.store(img, tid);
+            vs.store(img + IMG, tid);
+            if (tid < BN) {  // wave 0
+                if (E4M3) {
+                    sc[t & 1][0][tid] = sk;
+                    sc[t & 1][1][tid] = sv;
+                }
+                const uint64_t all = __ballot(there);
+                if (tid < KB) exist[t & 1][tid] = (uint32_t)(all >> (32 * tid));
+            }
+        };
+        __syncthreads();  // page ids; the images of the previous tile are free
+        if (nt > 0) {
+            fetch(0);
+            put(0);
+        }
+        __syncthreads();
+        for (int t = 0; t < nt; ++t) {
+            const unsigned char* Ks = smem + (t & 1) * 2 * IMG;
+            const unsigned char* Vs = Ks + IMG;
+            const bool more = t + 1 < nt;
+            if (more) fetch(t + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            const int k0 = w.kbegin + t * BN;
+            if (k0 < wave_end) {
+                f32x16 s[KB];
+                uint32_t ex[KB];
+                bool plain = k0 + BN <= all_see;
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    ex[b] = exist[t & 1][b];
+                    plain = plain && ex[b] == 0xffffffffu;
+                    zero16(s[b]);
+                    L::mma_rows(s[b], Ks + b * 32 * L::ROWB, ln, qf);
+                    if constexpr (E4M3) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const f32x4t f = *reinterpret_cast<const f32x4t*>(&sc[t & 1][0][32 * b + 8 * i + 4 * half]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) s[b][4 * i + j] *= f[j];
+                        }
+                    }
+                }
+                if (!plain) {
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int kr = row_of(i, half);
+                            s[b][i] = ((ex[b] >> kr) & 1) && k0 + 32 * b + kr < see ? s[b][i] : -INFINITY;
+                        }
+                }
+                float top = s[0][0];
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+                bool raised;
+                const float a = run.raise(top, c, &raised);
+                if (raised) {
+#pragma unroll
+                    for (int dt = 0; dt < L::NDT; ++dt)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[dt][i] *= a;
+                }
+                const float base = run.base();
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    float x[16];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        f32x4t f = {1.f, 1.f, 1.f, 1.f};
+                        if constexpr (E4M3) f = *reinterpret_cast<const f32x4t*>(&sc[t & 1][1][32 * b + 8 * i + 4 * half]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float e = exp2_fast(__fmaf_rn(s[b][4 * i + j], c, -base));
+                            run.l += e;
+                            x[4 * i + j] = E4M3 ? e * f[j] : e;
+                        }
+                    }
+                    typename L::weights pw;
+                    L::pack(pw, x);
+                    L::mma_cols(acc, Vs + b * 32 * L::ROWB, ln, pw);
+                }
+            }
+            if (more) {
+                put(t + 1);
+                __syncthreads();
+            }
+        }
+        const float l = run.l + __shfl_xor(run.l, 32, 64);
+        if (r < nrows) {
+            const int grow = w.a + token;
+            const bool any = l != 0.f;
+            const size_t at = (size_t)grow * p.Hq + head;
+            if (w.nsplit == 1) {
+                L::store_row(p.o + (size_t)grow * p.ldo + head * DH, acc, any ? 1.f / l : 0.f, half);
+                if (p.lse && half == 0) p.lse[(size_t)head * p.rows + grow] = any ? (run.base() + __log2f(l)) * LN2 : -INFINITY;
+            } else {
+                const size_t sat = (size_t)w.split * p.rows * p.Hq + at;
+                AttTile<float, DH>::store_row(p.part_o + sat * DH, acc, 1.f, half);
+                if (half == 0) p.part_ml[sat] = float2{run.m2, l};
+            }
+            if (half == 0 && w.split == 0 && p.part_n) p.part_n[at] = w.nsplit;
+        }
+    }
+}
+
+// one wave for each (row, head): the splits' contexts joined in split order
+template <int DH>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
+    const int lane = threadIdx.x & 63;
+    const size_t at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const size_t all = (size_t)p.rows * p.Hq;
+    if (at >= all) return;
+    const int grow = (int)(at / p.Hq), head = (int)(at % p.Hq);
+    if (p.cu ? (grow < p.cu[0] || grow >= p.cu[p.n]) : grow >= p.n) return;
+    const int n = min(p.part_n[at], p.splits);
+    if (n <= 1) return;
+    float m = -INFINITY;
+    for (int s = lane; s < n; s += 64) m = fmaxf(m, p.part_ml[s * all + at].x);
+    m = wave_max(m);
+    float l = 0.f;
+    constexpr int E = DH / 64;
+    float acc[E] = {};
+    for (int s = 0; s < n; ++s) {
+        const float2 v = p.part_ml[s * all + at];
+        const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : 1.f) : exp2_fast(v.x - m);
+        l += v.y * f;
+        const float* src = p.part_o + (s * all + at) * DH + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = __fmaf_rn(src[e], f, acc[e]);
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    __bf16* dst = p.o + (size_t)grow * p.ldo + head * DH + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[e] = (__bf16)(acc[e] * inv);
+    if (p.lse && lane == 0) p.lse[(size_t)head * p.rows + grow] = l != 0.f ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
+}
+
+int paged_bad_count(unsigned int* count, bool reset) {
+    if (hipMemcpyFromSymbol(count, HIP_SYMBOL(g_bad_pages), sizeof(unsigned int)) != hipSuccess) return CAPDEC_ERR_LAUNCH;
+    if (reset && *count) {
+        const unsigned int zero = 0;
+        if (hipMemcpyToSymbol(HIP_SYMBOL(g_bad_pages), &zero, sizeof(zero)) != hipSuccess) return CAPDEC_ERR_LAUNCH;
+    }
+    return 0;
+}
+
+struct PagedShape {
+    bool rows_kernel;
+    int block, tiles, splits;  // rows of a tile, tiles of the longest chunk, splits of the longest sequence
+};
+
+static PagedShape paged_shape(const capdec_kv_cache* c, int n, int max_q, int Hq, int table_cols) {
+    PagedShape s;
+    const int64_t rows = (int64_t)max_q * (Hq / c->heads);
+    s.rows_kernel = rows > 64;
+    s.block = s.rows_kernel ? 128 : (rows > 32 ? 64 : 32);
+    s.tiles = (int)((rows + s.block - 1) / s.block);
+    const int64_t keys = (int64_t)table_cols * c->page, units = (int64_t)n * c->heads * s.tiles;
+    int64_t splits = (1024 + units - 1) / units;
+    splits = std::min(splits, (keys + SPLIT_MIN - 1) / SPLIT_MIN);
+    // a split's keys are rounded up to whole runs of 128 and its page ids have to fit LDS
+    splits = std::max(splits, (keys + SPLIT_KEYS - 129) / (SPLIT_KEYS - 128));
+    s.splits = (int)std::max<int64_t>(splits, 1);
+    return s;
+}
+
+static int paged_check(const char* what, const capdec_kv_cache* c, int n, int rows, int max_q, int Hq, int table_cols) {
+    if (int rc = kv_cache_check(what, c)) return rc;
+    CAPDEC_REQUIRE(n > 0 && rows >= 0 && max_q > 0 && table_cols > 0, "%s: bad shape n=%d rows=%d max_q=%d table_cols=%d", what, n, rows, max_q, table_cols);
+    CAPDEC_REQUIRE(Hq > 0 && Hq % c->heads == 0 && (int64_t)Hq * c->dh < (1 << 24), "%s: Hq=%d must be a multiple of the cache's %d heads", what, Hq, c->heads);
+    CAPDEC_REQUIRE((int64_t)table_cols * c->page < (1ll << 31) - SPLIT_KEYS, "%s: a page table of %d columns passes 2^31 positions", what, table_cols);
+    CAPDEC_REQUIRE((int64_t)rows * (Hq / c->heads) < (1ll << 30) && (int64_t)max_q * (Hq / c->heads) < (1ll << 30), "%s: too many rows", what);
+    const PagedShape s = paged_shape(c, n, max_q, Hq, table_cols);
+    CAPDEC_REQUIRE(((int64_t)n * c->heads * s.splits + 7) / 8 * 8 * s.tiles < (1ll << 31) && (int64_t)rows * Hq / 4 + 1 < (1ll << 31),
+                   "%s: too much work for one launch", what);
+    return 0;
+}
+
+// [part_o][part_ml][part_n], each rounded up to 256 bytes
+static size_t paged_bytes(int splits, int rows, int Hq, int dh, size_t* ml, size_t* cnt) {
+    const size_t items = (size_t)rows * Hq;
+    *ml = (splits * items * dh * 4 + 255) & ~(size_t)255;
+    *cnt = *ml + ((splits * items * 8 + 255) & ~(size_t)255);
+    return *cnt + items * 4;
+}
+
+}  // namespace capdec
+
+using namespace capdec;
+
+extern "C" size_t capdec_attn_paged_workspace_bytes(const capdec_kv_cache* cache, int n, int rows, int max_q, int Hq, int table_cols) {
+    if (paged_check("capdec_attn_paged_workspace_bytes", cache, n, rows, max_q, Hq, table_cols)) return 0;
+    const PagedShape s = paged_shape(cache, n, max_q, Hq, table_cols);
+    size_t a, b;
+    return s.splits == 1 ? 0 : paged_bytes(s.splits, rows, Hq, cache->dh, &a, &b);
+}
+
+extern "C" int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, int ldq, const int* cu_q, const int* kv_lens,
+                                 const int* page_table, int ld_table, int table_cols, int n, int rows, int max_q, int Hq, float scale,
+                                 void* o, int ldo, void* lse, void* workspace, size_t workspace_bytes, capdec_stream_t stream) {
+    if (int rc = paged_check("capdec_attn_paged", cache, n, rows, max_q, Hq, table_cols)) return rc;
+    CAPDEC_REQUIRE(kv_lens && page_table && ld_table >= table_cols, "capdec_attn_paged: lengths / page table missing, or ld_table=%d below %d columns",
+                   ld_table, table_cols);
+    CAPDEC_REQUIRE(cu_q || rows >= n, "capdec_attn_paged: %d rows for %d sequences of one token", rows, n);
+    CAPDEC_REQUIRE(scale > 0.f && scale < INFINITY, "capdec_attn_paged: scale must be positive and finite");
+    if (rows == 0) return 0;
+    CAPDEC_REQUIRE(q && o && aligned16(q) && aligned16(o) && ldq % 8 == 0 && ldo % 8 == 0 && ldq >= Hq * cache->dh && ldo >= Hq * cache->dh,
+                   "capdec_attn_paged: q / o must be non-null, 16-byte aligned bf16 matrices with row strides that are multiples of 8 and cover "
+                   "the heads");
+    const PagedShape s = paged_shape(cache, n, max_q, Hq, table_cols);
+    PagedParams p;
+    memset(&p, 0, sizeof(p));
+    if (s.splits > 1) {
+        size_t ml, cnt;
+        const size_t need = paged_bytes(s.splits, rows, Hq, cache->dh, &ml, &cnt);
+        CAPDEC_REQUIRE(workspace && aligned16(workspace), "capdec_attn_paged: workspace missing or not 16-byte aligned");
+        if (workspace_bytes < need) {
+            set_error("capdec_attn_paged: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+            return CAPDEC_ERR_WORKSPACE;
+        }
+        p.part_o = (float*)workspace;
+        p.part_ml = (float2*)((char*)workspace + ml);
+        p.part_n = (int*)((char*)workspace + cnt);
+    }
+    p.k = cache->k; p.v = cache->v; p.ks = (const float*)cache->k_scale; p.vs = (const float*)cache->v_scale;
+    p.q = (const __bf16*)q; p.o = (__bf16*)o; p.lse = (float*)lse;
+    p.cu = cu_q; p.lens = kv_lens; p.table = page_table;
+    p.ldq = ldq; p.ldo = ldo; p.ld_table = ld_table; p.cols = table_cols; p.n = n; p.rows = rows;
+    p.Hq = Hq; p.Hkv = cache->heads; p.group = Hq / cache->heads; p.page_log2 = log2_of(cache->page); p.pages = cache->pages;
+    p.splits = s.splits; p.tiles = s.tiles; p.scale = scale;
+    const unsigned blocks = (unsigned)(((int64_t)n * cache->heads * s.splits + 7) / 8 * 8 * s.tiles);
+    const bool e = cache->dtype == CAPDEC_E4M3, wide = cache->dh == 128;
+    hipStream_t st = (hipStream_t)stream;
+#define CAPDEC_PAGED(E, D)                                                                                       \
+    do {                                                                                                         \
+        if (s.rows_kernel) hipLaunchKernelGGL((paged_rows_kernel<E, D>), dim3(blocks), dim3(256), 0, st, p);     \
+        else if (s.block == 64) hipLaunchKernelGGL((paged_keys_kernel<E, D, 2>), dim3(blocks), dim3(256), 0, st, p); \
+        else hipLaunchKernelGGL((paged_keys_kernel<E, D, 1>), dim3(blocks), dim3(256), 0, st, p);                \
+    } while (0)
+    if (e && wide) CAPDEC_PAGED(true, 128);
+    else if (e) CAPDEC_PAGED(true, 64);
+    else if (wide) CAPDEC_PAGED(false, 128);
+    else CAPDEC_PAGED(false, 64);
+#undef CAPDEC_PAGED
+    if (s.splits > 1) {
+        const dim3 grid((unsigned)(((size_t)rows * Hq + 3) / 4));
+        if (wide) hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, st, p);
+    }
+    return check_launch("capdec_attn_paged");
+}

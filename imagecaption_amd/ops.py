@@ -15,7 +15,8 @@ from ._capi import ACT_GELU_BWD, ACT_NONE, F32, check, lib, ptr, stream
 
 __all__ = ["compute_dtype", "gemm", "linear_fwd", "linear_dgrad", "linear_wgrad", "layernorm_fwd", "layernorm_bwd", "embed_fwd",
            "embed_bwd", "attn_fwd", "attn_bwd", "softmax_ce", "ce_tiles", "ce_finalize", "ce_dlogits", "ce_dlogits_bf16", "cast_bf16", "reduce_sum", "sumsq", "adamw", "clip_scale", "pe_add",
-           "act_dropout_bwd", "PackedSeqs", "attn_packed_fwd", "attn_packed_bwd"]
+           "act_dropout_bwd", "PackedSeqs", "attn_packed_fwd", "attn_packed_bwd",
+           "PagedKVCache", "kv_cache_write", "kv_cache_read", "check_pages", "attn_paged", "draft_verify"]
 
 
 # Arithmetic type of the matrix products.  F32: exact fp32 MFMA (reference precision, the default).
@@ -1034,6 +1035,179 @@ def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=Non
                                        ptr(dk), dk.stride(0), ptr(dv), dv.stride(0), Hq, Hkv, dh, dtype, scale, stream()),
           "capdec_attn_packed_bwd")
     return dq, dk, dv
+
+
+# ---- paged key / value cache -------------------------------------------------------------------------------------------
+class PagedKVCache:
+    """Pages of keys and values: k / v [pages, heads, page, dh], bf16, or e4m3 codes (torch.float8_e4m3fn) with fp32 scales
+    k_scale / v_scale [pages, heads, page].  Position j of a sequence whose pages are listed in ``table`` lives in slot
+    ``table[j // page] * page + j % page`` (``slots``).  The tensors are the caller's; ``PagedKVCache.new`` makes them."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        e4m3 = k.dtype == torch.float8_e4m3fn
+        if not e4m3 and k.dtype != torch.bfloat16:
+            raise _capi.CapdecError(f"PagedKVCache: k is {k.dtype}: bf16 or float8_e4m3fn pages")
+        _req(k, "PagedKVCache.k", k.dtype), _req(v, "PagedKVCache.v", k.dtype)
+        if k.dim() != 4 or v.shape != k.shape or not (k.is_contiguous() and v.is_contiguous()):
+            raise _capi.CapdecError(f"PagedKVCache: k {tuple(k.shape)} / v {tuple(v.shape)} must be contiguous [pages, heads, page, dh]")
+        if e4m3 != (k_scale is not None) or e4m3 != (v_scale is not None):
+            raise _capi.CapdecError("PagedKVCache: e4m3 pages have scales, bf16 pages have none")
+        for t in (k_scale, v_scale):
+            if t is not None and (tuple(_req(t, "PagedKVCache.scale").shape) != tuple(k.shape[:3]) or not t.is_contiguous()):
+                raise _capi.CapdecError(f"PagedKVCache: scales must be contiguous {tuple(k.shape[:3])}, got {tuple(t.shape)}")
+        pages, heads, page, dh = k.shape
+        if dh not in (64, 128) or page not in (8, 16, 32, 64, 128, 256) or pages * page >= 1 << 31 or not 0 < heads <= 65535 or pages == 0:
+            raise _capi.CapdecError(f"PagedKVCache: {tuple(k.shape)}: heads of 64 or 128, pages of 8 .. 256 positions (a power of two)")
+        _on_one("PagedKVCache", k, v, k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.heads, self.page, self.dh = pages, heads, page, dh
+        self.c = _capi.KVCache(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, heads, page, dh, _capi.E4M3 if e4m3 else _capi.BF16S)
+
+    @classmethod
+    def new(cls, pages, heads, page, dh, dtype=torch.bfloat16, device="cuda"):
+        """An empty cache (contents undefined until written)."""
+        k, v = (torch.empty((pages, heads, page, dh), dtype=dtype, device=device) for _ in range(2))
+        if dtype != torch.float8_e4m3fn:
+            return cls(k, v)
+        return cls(k, v, *(torch.empty((pages, heads, page), dtype=torch.float32, device=device) for _ in range(2)))
+
+    def slots(self, table, positions):
+        """int32 slots of ``positions`` (int tensor) in the sequence whose pages are ``table`` (a row of the page table)."""
+        positions = positions.long()
+        return (table[positions // self.page].long() * self.page + positions % self.page).to(torch.int32)
+
+
+def _on_one(name, *tensors):
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise _capi.CapdecError(f"{name}: tensors on different devices ({', '.join(sorted(map(str, devices)))})")
+
+
+def _ints(t, name, n):
+    """A dense int32 vector of n entries."""
+    _req(t, name, torch.int32)
+    if t.dim() != 1 or t.numel() != n or (n > 1 and t.stride(0) != 1):
+        raise _capi.CapdecError(f"{name}: need a dense int32 vector of {n}, got {tuple(t.shape)} / {t.stride()}")
+    return t
+
+
+def _cache_rows(name, cache, k, v, slots):
+    if k.dtype not in (torch.float32, torch.bfloat16):
+        raise _capi.CapdecError(f"{name}: rows are {k.dtype}: fp32 or bf16")
+    rows, width = slots.numel(), cache.heads * cache.dh
+    _ints(slots, name + ".slots", rows)
+    _packed_mat(k, name + ".k", k.dtype, rows, width), _packed_mat(v, name + ".v", k.dtype, rows, width)
+    _on_current(name, k, v, slots, cache.k)
+    return rows, F32 if k.dtype == torch.float32 else _capi.BF16S
+
+
+def kv_cache_write(cache, k, v, slots):
+    """Row r of k / v ([>= rows, heads * dh], fp32 or bf16, row-strided views) into slot ``slots[r]`` (int32 [rows]; negative:
+    skipped) of a PagedKVCache, rounded to e4m3 with a scale of its own for each head where the cache holds e4m3.  The slots of
+    one call must differ."""
+    rows, dtype = _cache_rows("kv_cache_write", cache, k, v, slots)
+    check(lib().capdec_kv_write(C.byref(cache.c), ptr(k), k.stride(0), ptr(v), v.stride(0), dtype, ptr(slots), rows, stream()),
+          "capdec_kv_write")
+
+
+def kv_cache_read(cache, slots, k=None, v=None, dtype=torch.bfloat16):
+    """(k, v): the rows of ``slots`` (int32 [rows]; negative: zeros) as [rows, heads * dh] matrices of ``dtype`` (or into given
+    ones)."""
+    new = lambda: torch.empty((slots.numel(), cache.heads * cache.dh), dtype=dtype, device=cache.k.device)
+    k = new() if k is None else k
+    v = new() if v is None else v
+    rows, dt = _cache_rows("kv_cache_read", cache, k, v, slots)
+    check(lib().capdec_kv_read(C.byref(cache.c), ptr(slots), rows, ptr(k), k.stride(0), ptr(v), v.stride(0), dt, stream()),
+          "capdec_kv_read")
+    return k, v
+
+
+def check_pages():
+    """Raise IndexError if kernels on the current device have met slots or pages outside their cache, or lengths past their
+    page table, since the last check: such entries are never followed, only counted.  Synchronises."""
+    n = C.c_uint(0)
+    check(lib().capdec_kv_bad_pages(C.byref(n), 1), "capdec_kv_bad_pages")
+    if n.value:
+        raise IndexError(f"{n.value} slot(s), page(s) or length(s) outside the paged cache were given since the last check")
+
+
+def attn_paged(q, cache, page_table, kv_lens, Hq, cu_q=None, max_q=1, out=None, scale=None, return_lse=False):
+    """Attention of each sequence's newest tokens over its cached positions (write the new ones first): q [rows, Hq * dh] bf16
+    holds the new tokens of the n sequences back to back, sequence s those of rows cu_q[s] .. cu_q[s + 1] - 1 (int32 [n + 1];
+    None: one each), at most ``max_q``; kv_lens int32 [n]: positions of each sequence with the new ones; page_table int32
+    [n, columns].  Causal: new token i of nq sees the positions up to kv_lens - nq + i.  Returns o (rows of no sequence stay as
+    they are in a given ``out`` and are zeros in a new one), or (o, lse [Hq, rows])."""
+    name = "attn_paged"
+    n = kv_lens.numel()
+    _packed_mat(q, name + ".q", torch.bfloat16, 0 if cu_q is not None else n, Hq * cache.dh)
+    _ints(kv_lens, name + ".kv_lens", n)
+    if cu_q is not None:
+        _ints(cu_q, name + ".cu_q", n + 1)
+    _req(page_table, name + ".page_table", torch.int32)
+    if page_table.dim() != 2 or page_table.shape[0] != n or page_table.shape[1] == 0 or page_table.stride(1) != 1 \
+            or (n > 1 and page_table.stride(0) < page_table.shape[1]) or n == 0:
+        raise _capi.CapdecError(f"{name}: page_table {tuple(page_table.shape)} / {page_table.stride()} must be int32 [{n}, columns] "
+                                "with unit column stride")
+    if Hq <= 0 or Hq % cache.heads or max_q <= 0:
+        raise _capi.CapdecError(f"{name}: Hq={Hq} must be a multiple of the cache's {cache.heads} heads, max_q={max_q} positive")
+    scale = 1.0 / math.sqrt(cache.dh) if scale is None else float(scale)
+    rows, cols = q.shape[0], page_table.shape[1]
+    if out is None:
+        # (which rows belong to no sequence is known on the device only)
+        out = (torch.empty if cu_q is None and rows == n else torch.zeros)((rows, Hq * cache.dh), dtype=q.dtype, device=q.device)
+    else:
+        _packed_mat(out, name + ".out", torch.bfloat16, rows, Hq * cache.dh)
+    _on_current(name, q, out, kv_lens, cu_q, page_table, cache.k)
+    lse = torch.zeros((Hq, rows), dtype=torch.float32, device=q.device) if return_lse else None
+    l = lib()
+    need = l.capdec_attn_paged_workspace_bytes(C.byref(cache.c), n, rows, int(max_q), Hq, cols)
+    # a block of its own for every call: the allocator keeps it from calls on other streams and from other captured graphs
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    check(l.capdec_attn_paged(C.byref(cache.c), ptr(q), q.stride(0), ptr(cu_q), ptr(kv_lens), ptr(page_table),
+                              page_table.stride(0) if n > 1 else cols, cols, n, rows, int(max_q), Hq, scale, ptr(out), out.stride(0),
+                              ptr(lse), ptr(ws), need, stream()), "capdec_attn_paged")
+    return (out, lse) if return_lse else out
+
+
+def draft_verify(target, draft, tokens, u_accept, u_sample, num_draft=None, pad=0):
+    """Drafted tokens against the target's probabilities (capdec_draft_verify): target [n, drafts + 1, V], draft [n, drafts, V]
+    (None: a drafter sure of its tokens), fp32 probabilities with unit stride along the vocabulary; tokens int64 [n, drafts];
+    u_accept [n, drafts] / u_sample [n] uniforms in [0, 1); num_draft int32 [n] (None: all).  Returns (out int64
+    [n, drafts + 1]: accepted tokens, the drawn one, then ``pad``; accepted int32 [n])."""
+    name = "draft_verify"
+    _req(target, name + ".target")
+    if target.dim() != 3 or target.shape[1] == 0 or target.shape[2] == 0 or (target.numel() and target.stride(2) != 1):
+        raise _capi.CapdecError(f"{name}: target {tuple(target.shape)} / {target.stride()} must be [n, drafts + 1, V] with unit stride "
+                                "along the vocabulary")
+    n, d, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    if d > 64:
+        raise _capi.CapdecError(f"{name}: {d} drafted tokens; at most 64")
+    if draft is not None:
+        _req(draft, name + ".draft")
+        if tuple(draft.shape) != (n, d, V) or (draft.numel() and draft.stride(2) != 1):
+            raise _capi.CapdecError(f"{name}: draft {tuple(draft.shape)} / {draft.stride()} must be {(n, d, V)} with unit stride along "
+                                    "the vocabulary")
+    for t, what, dt in ((tokens, ".tokens", torch.int64), (u_accept, ".u_accept", torch.float32)):
+        _req(t, name + what, dt)
+        if tuple(t.shape) != (n, d) or (d > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < d):
+            raise _capi.CapdecError(f"{name}{what}: need {(n, d)} with unit column stride, got {tuple(t.shape)} / {t.stride()}")
+    _req(u_sample, name + ".u_sample")
+    if tuple(u_sample.shape) != (n,) or (n > 1 and u_sample.stride(0) != 1):
+        raise _capi.CapdecError(f"{name}.u_sample: need a dense vector of {n}, got {tuple(u_sample.shape)}")
+    if num_draft is not None:
+        _ints(num_draft, name + ".num_draft", n)
+    for t, rows in ((target, d + 1), (draft, d)):
+        if t is not None and t.numel() and ((rows > 1 and t.stride(1) < V) or (n > 1 and t.stride(0) < 0)):
+            raise _capi.CapdecError(f"{name}: rows of probabilities overlap: strides {t.stride()}")
+    _on_current(name, target, draft, tokens, u_accept, u_sample, num_draft)
+    out = torch.empty((n, d + 1), dtype=torch.int64, device=target.device)
+    accepted = torch.empty(n, dtype=torch.int32, device=target.device)
+    step = lambda t, rows: max(t.stride(1), V) if rows > 1 else V
+    check(lib().capdec_draft_verify(ptr(target), target.stride(0), step(target, d + 1), ptr(draft), draft.stride(0) if draft is not None else 0,
+                                    step(draft, d) if draft is not None else 0, ptr(tokens), max(tokens.stride(0), d), ptr(num_draft),
+                                    ptr(u_accept), max(u_accept.stride(0), d), ptr(u_sample), n, d, V, int(pad), ptr(out), ptr(accepted),
+                                    stream()), "capdec_draft_verify")
+    return out, accepted
 
 
 def softmax_ce(logits, targets, eps=0.1, grad_scale=None, want_grad=True, in_place=False):

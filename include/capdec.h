@@ -40,6 +40,8 @@ enum { CAPDEC_OK = 0, CAPDEC_ERR_ARG = -1, CAPDEC_ERR_LAUNCH = -2, CAPDEC_ERR_UN
  *                the row rounded up to 8; bf16 MFMA, fp32 accumulate, fp32 epilogue and result
  *                (csrc/gemm_bf16s.hip).  ce_lse is not available (use capdec_ce_dlogits_bf16). */
 enum { CAPDEC_F32 = 0, CAPDEC_BF16 = 1, CAPDEC_F32X3 = 2, CAPDEC_BF16S = 3 };
+/* element type of a paged cache besides CAPDEC_BF16S: OCP e4m3 codes with a scale for every row (capdec_kv_cache) */
+enum { CAPDEC_E4M3 = 4 };
 enum { CAPDEC_ACT_NONE = 0, CAPDEC_ACT_GELU = 1, CAPDEC_ACT_GELU_BWD = 2 };
 
 int capdec_abi_version(void);
@@ -378,6 +380,66 @@ int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ld
                            const void* o, int ldo, const void* dout, int lddo, const void* lse, void* delta, size_t stat_rows,
                            void* dq, int lddq, void* dk, int lddk, void* dv, int lddv, int Hq, int Hkv, int dh, int dtype,
                            float scale, capdec_stream_t stream);
+
+/* ---- paged key / value cache: write, read back, attention of new tokens over it ----------------------------------
+ * A cache is a set of pages; a page holds `page` positions of one sequence for every key / value head: k / v are dense
+ * [pages, heads, page, dh] matrices, so one head's rows of a page are contiguous.  A sequence's pages are listed, in order,
+ * in its row of a page table; position j lives in page table[j / page] at place j % page, i.e. in SLOT
+ * table[j / page] * page + j % page.  page is a power of two from 8 to 256, dh 64 or 128, pages * page < 2^31.
+ *   CAPDEC_BF16S  bf16 rows;
+ *   CAPDEC_E4M3   rounded as they are written: scale = max(amax |x|, 2^-100) / 448 (fp32, one for every row of a head, in
+ *                 k_scale / v_scale [pages, heads, page]), code = e4m3(x / scale), value code * scale.  A row that holds an
+ *                 infinity or a NaN reads back as NaN throughout.
+ * capdec_kv_write: row r of k / v ([rows, heads * dh], fp32 or bf16 by `dtype`) goes to slots[r]; a negative slot is skipped.
+ *   The slots of one call must differ: of two rows sent to one slot, which one each element comes from is not defined.
+ * capdec_kv_read: the rows back as fp32 or bf16 (rounded once); a negative slot reads as zeros.
+ * capdec_attn_paged: for each of n sequences, attention of its newest nq tokens over all its kv_lens[s] positions (the new
+ *   ones among them: write them first), causal: new token i of nq sees the positions up to kv_lens[s] - nq + i.  q / o are
+ *   bf16 matrices with the new tokens of all sequences back to back: sequence s owns the rows cu_q[s] .. cu_q[s + 1] - 1 (cu_q
+ *   NULL: one token each, row s).  max_q is the largest nq (a hint: more rows are still computed, more slowly).  Query head h
+ *   reads key / value head h / (Hq / heads).  Products in bf16 with fp32 accumulation, softmax in fp32; weights are rounded
+ *   to bf16 for the context product (after the value's scale is multiplied in), the result once.  A token that sees nothing
+ *   gets o = 0, lse = -inf; lse (fp32 [Hq, rows]) may be NULL.  Rows behind the last sequence stay as they are.
+ *   Everything that varies from step to step (cu_q, kv_lens, page_table) is read on the device, so a captured call can be
+ *   replayed with new contents.  The keys are split over workgroups and joined in a second launch when there are few rows;
+ *   the workspace (capdec_attn_paged_workspace_bytes, 16-byte aligned) needs no clearing and must not be shared by calls
+ *   that may overlap in time.  Fixed summation orders: bitwise reproducible for given arguments.
+ * Slots and pages outside the cache, and lengths past the page table, are never followed: a bad slot is skipped / reads as
+ * zeros, a position on a bad page counts as unseen, a length is cut to the table.  capdec_kv_bad_pages counts them (wave-wise,
+ * at least one for every bad entry met) on the current device since the last reset; it synchronises the device.
+ * The dense counterpart is capdec_decode_attn; the reference re-runs the whole prefix instead (ref train.py:312-332). */
+typedef struct capdec_kv_cache {
+    void *k, *v;
+    void *k_scale, *v_scale; /* CAPDEC_E4M3 only */
+    int pages, heads, page, dh, dtype;
+} capdec_kv_cache;
+int capdec_kv_write(const capdec_kv_cache* cache, const void* k, int ldk, const void* v, int ldv, int dtype, const int* slots,
+                    int rows, capdec_stream_t stream);
+int capdec_kv_read(const capdec_kv_cache* cache, const int* slots, int rows, void* k, int ldk, void* v, int ldv, int dtype,
+                   capdec_stream_t stream);
+size_t capdec_attn_paged_workspace_bytes(const capdec_kv_cache* cache, int n, int rows, int max_q, int Hq, int table_cols);
+int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, int ldq, const int* cu_q, const int* kv_lens,
+                      const int* page_table, int ld_table, int table_cols, int n, int rows, int max_q, int Hq, float scale, void* o,
+                      int ldo, void* lse, void* workspace, size_t workspace_bytes, capdec_stream_t stream);
+int capdec_kv_bad_pages(unsigned int* count, int reset);
+
+/* ---- verification of drafted tokens -------------------------------------------------------------------------------
+ * For each of n sequences: num_draft[b] <= drafts tokens x_0, x_1, .. (tokens [n, drafts] int64, row stride ldt) were drawn from
+ * the drafter's probabilities q_i (draft [n, drafts, V], strides in elements; NULL: a drafter that is sure of its tokens,
+ * q_i = 1 at x_i); p_i (target [n, drafts + 1, V]) are the target model's probabilities at the same places and after the last
+ * one.  Token i is accepted while u_accept[b, i] * q_i(x_i) < p_i(x_i); at the first refusal i the replacement is drawn from
+ * max(p_i - q_i, 0), after num_draft acceptances one more token from p_num_draft, by inverse CDF from u_sample[b]: the first v
+ * whose running sum exceeds u_sample * total (the last v of positive weight if rounding leaves none).  Uniforms in [0, 1).
+ * If max(p - q, 0) vanishes everywhere the draw is from p; if p does too, the token is 0.  Products, differences and sums in
+ * 64 bits; NaN and negative weights count as 0; a drafted token outside [0, V) is refused.
+ * out [n, drafts + 1] int64 (dense): accepted tokens, the drawn one, then pad; accepted[b] (int32) = how many were accepted.
+ * num_draft may be NULL (all `drafts`); entries are cut to [0, drafts].  drafts <= 64; drafts = 0 only draws (tokens, draft,
+ * u_accept may then be NULL).  The distribution of the output is the target's, as in sampling token by token
+ * (capdec_sample_select; ref train.py:335-383). */
+int capdec_draft_verify(const void* target, int64_t target_seq, int64_t target_row, const void* draft, int64_t draft_seq,
+                        int64_t draft_row, const int64_t* tokens, int ldt, const int* num_draft, const void* u_accept, int ldu,
+                        const void* u_sample, int n, int drafts, int V, int64_t pad, int64_t* out, int* accepted,
+                        capdec_stream_t stream);
 
 /* ---- label-smoothed softmax cross-entropy, forward + backward in one pass -------------------------
  * Per row m of logits [M,V] (row stride ldl) with target y = targets[m] (int64):

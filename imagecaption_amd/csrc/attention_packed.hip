@@ -30,6 +30,7 @@ struct PackedParams {
     const void* q; const void* k; const void* v; const void* o; const void* dout;
     void* out; void* dq; void* dk; void* dv;
     float* lse; float* delta;
+    void* stats;  // bf16 matrices: 16 bytes for each (head, row), see packed16_bwd_dkv_kernel
     const PackedItem* items;
     int ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
     int Hq, Hkv, group, causal;
@@ -51,12 +52,36 @@ __device__ __forceinline__ void packed_place(int heads, int& head, int& item) {
     }
 }
 
-template <typename T, int DH, int NW, int KB>
-__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(PackedParams p) {
+// accumulators of a wave through LDS to another wave with the same lane layout
+template <int NDT>
+__device__ __forceinline__ void put_sums(unsigned char* box, const f32x16* acc, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4 * NDT; ++i) {
+        const f32x16& a = acc[i >> 2];
+        const int e = 4 * (i & 3);
+        reinterpret_cast<f32x4t*>(box)[i * 64 + lane] = f32x4t{a[e], a[e + 1], a[e + 2], a[e + 3]};
+    }
+}
+// acc = acc fa + box fb
+template <int NDT>
+__device__ __forceinline__ void add_sums(const unsigned char* box, f32x16* acc, int lane, float fa, float fb) {
+#pragma unroll
+    for (int i = 0; i < 4 * NDT; ++i) {
+        const f32x4t v = reinterpret_cast<const f32x4t*>(box)[i * 64 + lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i >> 2][4 * (i & 3) + j] = acc[i >> 2][4 * (i & 3) + j] * fa + v[j] * fb;
+    }
+}
+
+// RB blocks of 32 rows; the KS waves of a block take every KS-th run of 32 KB keys of a tile and join at the end
+template <typename T, int DH, int RB, int KS, int KB>
+__global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd_kernel(PackedParams p) {
     using L = AttTile<T, DH>;
-    constexpr int BN = 32 * KB, IMG = BN * L::ROWB;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
-    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    constexpr int NT = RB * KS * 64, BN = 32 * KB * KS, IMG = BN * L::ROWB, BOX = (DH / 4 * 16 + 8) * 64;
+    constexpr int JOIN = RB * (KS - 1) * BOX;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG > JOIN ? 4 * IMG : JOIN];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const int rb = wave % RB, ksp = wave / RB;
     int head, it;
     packed_place(p.Hq, head, it);
     const PackedItem w = p.items[it];
@@ -64,9 +89,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(Pa
     const T* qg = (const T*)p.q + (size_t)w.q0 * p.ldq + head * DH;
     const T* kg = (const T*)p.k + (size_t)w.k0 * p.ldk + hk * DH;
     const T* vg = (const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH;
-    const int r0 = w.t0 + (tid >> 6) * 32;        // this wave's first row
+    const int r0 = w.t0 + rb * 32;                // this wave's first row
     const int row = r0 + l31, off = w.nk - w.nq;  // causal: row sees keys j <= row + off
-    const int kmax = p.causal ? min(w.nk, min(w.t0 + NW * 32, w.nq) + off) : w.nk;  // of the workgroup's last row
+    const int kmax = p.causal ? min(w.nk, min(w.t0 + RB * 32, w.nq) + off) : w.nk;  // of the workgroup's last row
     const int nt = kmax > 0 ? (kmax + BN - 1) / BN : 0;
     // keys the wave's rows can see at all, and keys that all of them see (no mask below)
     const int wave_end = r0 >= w.nq ? 0 : (p.causal ? min(w.nk, min(r0 + 32, w.nq) + off) : w.nk);
@@ -74,7 +99,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(Pa
 
     typename L::frag qf[L::NF];
     L::load_row(qf, qg + (size_t)row * p.ldq, row < w.nq, half);
-    Staged<T, DH, NW * 64, BN> ks, vs;
+    Staged<T, DH, NT, BN> ks, vs;
     if (nt > 0) {
         ks.load(kg, p.ldk, 0, w.nk, tid);
         vs.load(vg, p.ldv, 0, w.nk, tid);
@@ -90,7 +115,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(Pa
     run.init();
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
-        const unsigned char* Ks = smem + (t & 1) * 2 * IMG;
+        const unsigned char* Ks = smem + (t & 1) * 2 * IMG + ksp * 32 * KB * L::ROWB;
         const unsigned char* Vs = Ks + IMG;
         const bool more = t + 1 < nt;
         if (more) {
@@ -98,7 +123,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(Pa
             vs.load(vg, p.ldv, (t + 1) * BN, w.nk, tid);
         }
         __builtin_amdgcn_sched_barrier(0);
-        const int k0 = t * BN;
+        const int k0 = t * BN + ksp * 32 * KB;
         if (k0 < wave_end) {
             f32x16 s[KB];
 #pragma unroll
@@ -106,7 +131,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(Pa
                 zero16(s[b]);
                 L::mma_rows(s[b], Ks + b * 32 * L::ROWB, ln, qf);  // S^T[key][query]
             }
-            if (k0 + BN > all_see) {
+            if (k0 + 32 * KB > all_see) {
                 const int see = p.causal ? min(w.nk, row + 1 + off) : w.nk;
 #pragma unroll
                 for (int b = 0; b < KB; ++b)
@@ -147,31 +172,54 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void packed_fwd_kernel(Pa
             __syncthreads();
         }
     }
-    const float l = run.l + __shfl_xor(run.l, 32, 64);
+    float l = run.l + __shfl_xor(run.l, 32, 64);
+    if constexpr (KS > 1) {  // the later waves of a block hand their part to the first, which joins them in order
+        __syncthreads();
+        if (ksp > 0) {
+            unsigned char* box = smem + (rb * (KS - 1) + ksp - 1) * BOX;
+            put_sums<L::NDT>(box, acc, lane);
+            reinterpret_cast<float2*>(box + DH / 4 * 16 * 64)[lane] = float2{run.m2, l};
+        }
+        __syncthreads();
+        if (ksp > 0) return;
+#pragma unroll
+        for (int o = 0; o < KS - 1; ++o) {
+            const unsigned char* box = smem + (rb * (KS - 1) + o) * BOX;
+            const float2 ml = reinterpret_cast<const float2*>(box + DH / 4 * 16 * 64)[lane];
+            const float m = fmaxf(run.m2, ml.x);
+            const float fa = run.m2 == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_fast(run.m2 - m);
+            const float fb = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - m);
+            l = l * fa + ml.y * fb;
+            run.m2 = m;
+            add_sums<L::NDT>(box, acc, lane, fa, fb);
+        }
+    }
     if (row < w.nq) {
-        const bool any = run.m2 != -INFINITY || l != 0.f;  // (a NaN row is not an empty one)
+        const bool any = l != 0.f;  // (NaN too: such a row is not an empty one)
         L::store_row((T*)p.out + (size_t)(w.q0 + row) * p.ldo + head * DH, acc, any ? 1.f / l : 0.f, half);
         if (p.lse && half == 0)
             p.lse[(size_t)head * p.stat_rows + w.q0 + row] = any ? (run.base() + __log2f(l)) * LN2 : -INFINITY;
     }
 }
 
-// dq and delta = rowsum(do * o); the wave owns 32 query rows
-template <typename T, int DH, int NW, int KB>
-__global__ __launch_bounds__(NW * 64, NW == 4 && sizeof(T) == 2 ? 2 : 1) void packed_bwd_dq_kernel(PackedParams p) {
+// dq and delta = rowsum(do * o); blocks and waves as in the forward
+template <typename T, int DH, int RB, int KS, int KB>
+__global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH == 64) ? 2 : 1) void packed_bwd_dq_kernel(PackedParams p) {
     using L = AttTile<T, DH>;
-    constexpr int BN = 32 * KB, IMG = BN * L::ROWB;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
-    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    constexpr int NT = RB * KS * 64, BN = 32 * KB * KS, IMG = BN * L::ROWB, BOX = DH / 4 * 16 * 64;
+    constexpr int JOIN = RB * (KS - 1) * BOX;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG > JOIN ? 4 * IMG : JOIN];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const int rb = wave % RB, ksp = wave / RB;
     int head, it;
     packed_place(p.Hq, head, it);
     const PackedItem w = p.items[it];
     const int hk = head / p.group;
     const T* kg = (const T*)p.k + (size_t)w.k0 * p.ldk + hk * DH;
     const T* vg = (const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH;
-    const int r0 = w.t0 + (tid >> 6) * 32;
+    const int r0 = w.t0 + rb * 32;
     const int row = r0 + l31, off = w.nk - w.nq;
-    const int kmax = p.causal ? min(w.nk, min(w.t0 + NW * 32, w.nq) + off) : w.nk;
+    const int kmax = p.causal ? min(w.nk, min(w.t0 + RB * 32, w.nq) + off) : w.nk;
     const int nt = kmax > 0 ? (kmax + BN - 1) / BN : 0;
     const int wave_end = r0 >= w.nq ? 0 : (p.causal ? min(w.nk, min(r0 + 32, w.nq) + off) : w.nk);
     const int all_see = p.causal ? min(w.nk, r0 + 1 + off) : w.nk;
@@ -191,8 +239,19 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && sizeof(T) == 2 ? 2 : 1) void pa
     // p = exp2(s c - lse2); a row that sees nothing has lse = -inf: its weights are zeros
     float lse2 = mine ? p.lse[(size_t)head * p.stat_rows + grow] * LOG2E : INFINITY;
     if (lse2 == -INFINITY) lse2 = INFINITY;
-    if (mine && half == 0) p.delta[(size_t)head * p.stat_rows + grow] = dsum;
-    Staged<T, DH, NW * 64, BN> ks, vs;
+    if (mine && half == 0 && ksp == 0) {
+        const size_t at = (size_t)head * p.stat_rows + grow;
+        if (sizeof(T) == 2 && p.stats) {
+            // -lse / scale and -delta, three bf16 terms each; a row that sees nothing gets weights of zero
+            const float l = lse2 == INFINITY ? -1e30f : -lse2 / (p.scale * LOG2E), d = -dsum;
+            const __bf16 l0 = (__bf16)l, l1 = (__bf16)(l - (float)l0), l2 = (__bf16)(l - (float)l0 - (float)l1);
+            const __bf16 d0 = (__bf16)d, d1 = (__bf16)(d - (float)d0), d2 = (__bf16)(d - (float)d0 - (float)d1);
+            reinterpret_cast<bf16x8t*>(p.stats)[at] = bf16x8t{l0, l1, l2, (__bf16)0.f, d0, d1, d2, (__bf16)0.f};
+        } else {
+            p.delta[at] = dsum;
+        }
+    }
+    Staged<T, DH, NT, BN> ks, vs;
     if (nt > 0) {
         ks.load(kg, p.ldk, 0, w.nk, tid);
         vs.load(vg, p.ldv, 0, w.nk, tid);
@@ -206,7 +265,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && sizeof(T) == 2 ? 2 : 1) void pa
     for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
-        const unsigned char* Ks = smem + (t & 1) * 2 * IMG;
+        const unsigned char* Ks = smem + (t & 1) * 2 * IMG + ksp * 32 * KB * L::ROWB;
         const unsigned char* Vs = Ks + IMG;
         const bool more = t + 1 < nt;
         if (more) {
@@ -216,7 +275,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && sizeof(T) == 2 ? 2 : 1) void pa
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-            const int k0 = t * BN + 32 * b;
+            const int k0 = t * BN + (ksp * KB + b) * 32;
             if (k0 < wave_end) {
                 f32x16 s, dp;
                 zero16(s);
@@ -243,57 +302,67 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && sizeof(T) == 2 ? 2 : 1) void pa
             __syncthreads();
         }
     }
+    if constexpr (KS > 1) {
+        __syncthreads();
+        if (ksp > 0) put_sums<L::NDT>(smem + (rb * (KS - 1) + ksp - 1) * BOX, acc, lane);
+        __syncthreads();
+        if (ksp > 0) return;
+#pragma unroll
+        for (int o = 0; o < KS - 1; ++o) add_sums<L::NDT>(smem + (rb * (KS - 1) + o) * BOX, acc, lane, 1.f, 1.f);
+    }
     if (mine) L::store_row((T*)p.dq + grow * p.lddq + head * DH, acc, p.scale, half);
 }
 
-// dk, dv: the wave owns 32 key rows of one key / value head and walks the query tiles of every query head of the group.
-// Runs after packed_bwd_dq_kernel (reads delta).
-template <typename T, int DH, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 4 && sizeof(T) == 2 && DH == 64 ? 2 : 1) void packed_bwd_dkv_kernel(PackedParams p) {
+// dk, dv: KB blocks of 32 key rows of one key / value head, every block walked by QS waves that take every QS-th query tile
+// of every query head of the group and add up at the end.  Runs after packed_bwd_dq_kernel (reads delta).
+template <typename T, int DH, int KB, int QS>
+__global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && sizeof(T) == 2 ? 2 : 1) void packed_bwd_dkv_kernel(PackedParams p) {
     using L = AttTile<T, DH>;
-    constexpr int BN = 32, IMG = BN * L::ROWB;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
-    __shared__ float stat[2][2][BN];  // [buffer][lse2 | delta][query]
-    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    constexpr int NT = KB * QS * 64, BN = 32 * QS, IMG = BN * L::ROWB, KIMG = 32 * KB * L::ROWB;
+    constexpr bool V_LDS = sizeof(T) == 2 && DH == 128 && NT > 64;
+    constexpr int BOX = DH / 4 * 16 * 64, JOIN = KB * (QS - 1) * BOX, WALK = 2 * IMG + (V_LDS ? KIMG : 0);
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[WALK > JOIN ? WALK : JOIN];
+    __shared__ float stat[2][BN];  // [lse2 | delta][query]
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const int kb = wave % KB, qs = wave / KB;
     int hk, it;
     packed_place(p.Hkv, hk, it);
     const PackedItem w = p.items[it];
-    const int r0 = w.t0 + (tid >> 6) * 32;
+    const int r0 = w.t0 + kb * 32;
     const int key = r0 + l31, off = w.nk - w.nq;
     const bool mine = key < w.nk;
     // causal: query i sees key j iff i >= j - off; the first tile that meets one of the workgroup's keys
     const int first = p.causal ? max(0, w.t0 - off) / BN : 0;
     const int per = max(0, (w.nq + BN - 1) / BN - first), nt = per * p.group;
 
-    typename L::frag kf[L::NF], vf[L::NF];
+    typename L::frag kf[L::NF], vf[V_LDS ? 1 : L::NF];
     L::load_row(kf, (const T*)p.k + (size_t)(w.k0 + key) * p.ldk + hk * DH, mine, half);
-    L::load_row(vf, (const T*)p.v + (size_t)(w.k0 + key) * p.ldv + hk * DH, mine, half);
-    Staged<T, DH, NW * 64, BN> qs, ds;
-    float st = 0.f;  // threads 0..31: a row's lse2, 32..63: its delta
+    unsigned char* Vs = smem + 2 * IMG;
+    if constexpr (V_LDS) {
+        Staged<T, DH, NT, 32 * KB> vs;
+        vs.load((const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, w.t0, w.nk, tid);
+        vs.store(Vs, tid);
+    } else {
+        L::load_row(vf, (const T*)p.v + (size_t)(w.k0 + key) * p.ldv + hk * DH, mine, half);
+    }
+    Staged<T, DH, NT, BN> qst, dst;
+    float st = 0.f;  // threads 0 .. BN - 1: a row's lse2, the next BN: its delta
     auto fetch = [&](int t) {
         const int head = hk * p.group + t / per, q0 = (first + t % per) * BN;
-        qs.load((const T*)p.q + (size_t)w.q0 * p.ldq + head * DH, p.ldq, q0, w.nq, tid);
-        ds.load((const T*)p.dout + (size_t)w.q0 * p.lddo + head * DH, p.lddo, q0, w.nq, tid);
-        if (tid < 64) {
-            const int i = q0 + (tid & 31);
-            const float none = tid < 32 ? INFINITY : 0.f;
-            const float* src = tid < 32 ? p.lse : p.delta;
+        qst.load((const T*)p.q + (size_t)w.q0 * p.ldq + head * DH, p.ldq, q0, w.nq, tid);
+        dst.load((const T*)p.dout + (size_t)w.q0 * p.lddo + head * DH, p.lddo, q0, w.nq, tid);
+        if (tid < 2 * BN) {
+            const int i = q0 + tid % BN;
+            const float none = tid < BN ? INFINITY : 0.f;
+            const float* src = tid < BN ? p.lse : p.delta;
             st = i < w.nq ? src[(size_t)head * p.stat_rows + w.q0 + i] : none;
-            if (tid < 32) {
+            if (tid < BN) {
                 st *= LOG2E;
                 if (st == -INFINITY) st = INFINITY;
             }
         }
     };
-    auto put = [&](int b) {
-        qs.store(smem + b * 2 * IMG, tid);
-        ds.store(smem + b * 2 * IMG + IMG, tid);
-        if (tid < 64) stat[b][tid >> 5][tid & 31] = st;
-    };
-    if (nt > 0) {
-        fetch(0);
-        put(0);
-    }
+    if (nt > 0) fetch(0);
     const typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
     f32x16 dk[L::NDT], dv[L::NDT];
@@ -302,30 +371,33 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && sizeof(T) == 2 && DH == 64 ? 2 
         zero16(dk[dt]);
         zero16(dv[dt]);
     }
-    __syncthreads();
     for (int t = 0; t < nt; ++t) {
-        const unsigned char* Qs = smem + (t & 1) * 2 * IMG;
-        const unsigned char* Ds = Qs + IMG;
-        const bool more = t + 1 < nt;
-        if (more) fetch(t + 1);
+        qst.store(smem, tid);
+        dst.store(smem + IMG, tid);
+        if (tid < 2 * BN) stat[tid / BN][tid % BN] = st;
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1);
         __builtin_amdgcn_sched_barrier(0);
-        const int q0 = (first + t % per) * BN;
-        if (r0 < w.nk && (!p.causal || r0 <= q0 + BN - 1 + off)) {
+        const int q0 = (first + t % per) * BN + 32 * qs;
+        const unsigned char* Qs = smem + 32 * qs * L::ROWB;
+        const unsigned char* Ds = Qs + IMG;
+        if (r0 < w.nk && q0 < w.nq && (!p.causal || r0 <= q0 + 31 + off)) {
             f32x16 s, dp;
             zero16(s);
-            zero16(dp);
-            L::mma_rows(s, Qs, ln, kf);   // S[query][key]
-            L::mma_rows(dp, Ds, ln, vf);  // dP[query][key]
+            L::mma_rows(s, Qs, ln, kf);  // S[query][key]
             // queries past the end have lse2 = +inf (weight zero); keys past the end are nobody's
             if (p.causal && q0 + off < r0 + 31) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = key <= q0 + row_of(r, half) + off ? s[r] : -INFINITY;
             }
+            zero16(dp);  // dP[query][key]
+            if constexpr (V_LDS) L::mma_images(dp, Ds, Vs + kb * 32 * L::ROWB, ln);
+            else L::mma_rows(dp, Ds, ln, vf);
             float x[16], y[16];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4t ls = *reinterpret_cast<const f32x4t*>(&stat[t & 1][0][8 * i + 4 * half]);
-                const f32x4t de = *reinterpret_cast<const f32x4t*>(&stat[t & 1][1][8 * i + 4 * half]);
+                const f32x4t ls = *reinterpret_cast<const f32x4t*>(&stat[0][32 * qs + 8 * i + 4 * half]);
+                const f32x4t de = *reinterpret_cast<const f32x4t*>(&stat[1][32 * qs + 8 * i + 4 * half]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     x[4 * i + j] = exp2_fast(__fmaf_rn(s[4 * i + j], c, -ls[j]));
@@ -338,19 +410,141 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && sizeof(T) == 2 && DH == 64 ? 2 
             L::mma_cols(dv, Ds, ln, pw);  // dV^T[dim][key] += dO^T P
             L::mma_cols(dk, Qs, ln, dw);  // dK^T[dim][key] += Q^T dS
         }
-        if (more) {
-            put((t + 1) & 1);
+        __syncthreads();
+    }
+    if constexpr (QS > 1) {  // the later waves of a block hand their sums to the first, in order
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            f32x16* acc = side ? dk : dv;
+            if (qs > 0) put_sums<L::NDT>(smem + (kb * (QS - 1) + qs - 1) * BOX, acc, lane);
+            __syncthreads();
+            if (qs == 0) {
+#pragma unroll
+                for (int o = 0; o < QS - 1; ++o) add_sums<L::NDT>(smem + (kb * (QS - 1) + o) * BOX, acc, lane, 1.f, 1.f);
+            }
             __syncthreads();
         }
     }
-    if (mine) {
+    if (qs == 0 && mine) {
         L::store_row((T*)p.dk + (size_t)(w.k0 + key) * p.lddk + hk * DH, dk, p.scale, half);
         L::store_row((T*)p.dv + (size_t)(w.k0 + key) * p.lddv + hk * DH, dv, 1.f, half);
     }
 }
 
-// rows per workgroup: four waves of 32, or one
-constexpr int TALL = 128, SHORT = 32;
+// The same for bf16 with four waves, KB QS = 4.  Q and dO tiles travel global -> LDS by DMA,
+// one tile ahead: the rows come from beyond the L2 (every query head of the group is walked), and registers for them would
+// cost the second wave of a SIMD.  V fragments are read from LDS for the same reason.  Per-query statistics enter the
+// products as one more k-step: -lse / scale and -delta split into three bf16 terms each (24 bits, exact to fp32) times ones,
+// so a lane loads 8 bytes for its own query and no value has to be handed around in accumulator-row order.
+template <int DH, int KB, int QS>
+__global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd_dkv_kernel(PackedParams p) {
+    using L = DmaTile<DH>;
+    constexpr int BN = 32 * QS, IMG = BN * L::ROWB, KIMG = 32 * KB * L::ROWB;
+    constexpr int BOX = DH / 4 * 16 * 64, WALK = 4 * IMG + KIMG;
+    static_assert(KB * QS == 4 && KB * (QS - 1) * BOX <= WALK, "the sums of a block fit the images");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[WALK];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const int kb = wave % KB, qs = wave / KB;
+    int hk, it;
+    packed_place(p.Hkv, hk, it);
+    const PackedItem w = p.items[it];
+    const int r0 = w.t0 + kb * 32;
+    const int key = r0 + l31, off = w.nk - w.nq;
+    const bool mine = key < w.nk;
+    // causal: query i sees key j iff i >= j - off; the first tile that meets one of the workgroup's keys
+    const int first = p.causal ? max(0, w.t0 - off) / BN : 0;
+    const int per = max(0, (w.nq + BN - 1) / BN - first), nt = per * p.group;
+    unsigned char* Vs = smem + 4 * IMG;
+    const s16x4t* stats = reinterpret_cast<const s16x4t*>(p.stats);
+    s16x4t st;
+    int fh = hk * p.group, fq = first;  // the next tile to fetch: head, tile
+    auto fetch = [&](int b) {
+        const int q0 = fq * BN;
+        st = stats[2 * ((size_t)fh * p.stat_rows + w.q0 + min(q0 + 32 * qs + l31, w.nq - 1)) + half];
+        L::template fetch<BN, 4>(smem + b * 2 * IMG, (const __bf16*)p.q + (size_t)w.q0 * p.ldq + fh * DH, p.ldq, q0, w.nq, wave, lane);
+        L::template fetch<BN, 4>(smem + b * 2 * IMG + IMG, (const __bf16*)p.dout + (size_t)w.q0 * p.lddo + fh * DH, p.lddo, q0, w.nq, wave, lane);
+        if (++fq == first + per) {
+            fq = first;
+            ++fh;
+        }
+    };
+    typename L::frag kf[L::NF];
+    L::load_row(kf, (const __bf16*)p.k + (size_t)(w.k0 + key) * p.ldk + hk * DH, mine, half);
+    if (nt > 0) {
+        L::template fetch<32 * KB, 4>(Vs, (const __bf16*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, w.t0, w.nk, wave, lane);
+        fetch(0);
+    }
+    typename L::lanes ln = L::make_lanes(lane);
+    const float c = p.scale * LOG2E;
+    // half-wave 0 holds the terms of -lse / scale (k = 0..3), half-wave 1 those of -delta (k = 4..7)
+    constexpr short ONE = 0x3f80;
+    const short f0 = half ? 0 : ONE, f1 = half ? ONE : 0;
+    const s16x4t pick_l = {f0, f0, f0, f0}, pick_d = {f1, f1, f1, f1};
+    f32x16 dk[L::NDT], dv[L::NDT];
+#pragma unroll
+    for (int dt = 0; dt < L::NDT; ++dt) {
+        zero16(dk[dt]);
+        zero16(dv[dt]);
+    }
+    int qt = first;
+    for (int t = 0; t < nt; ++t) {
+        dma_sync();
+        s16x4t now = st;
+        asm volatile("" : "+v"(now));  // taken here, where it has landed: a wait further down would include the next tile's transfers
+        if (t + 1 < nt) fetch((t + 1) & 1);
+        const int q0 = qt * BN + 32 * qs;
+        if (++qt == first + per) qt = first;
+        opaque(ln.row);
+        const unsigned char* Qs = smem + (t & 1) * 2 * IMG + 32 * qs * L::ROWB;
+        const unsigned char* Ds = Qs + IMG;
+        if (r0 < w.nk && q0 < w.nq && (!p.causal || r0 <= q0 + 31 + off)) {
+            f32x16 s, dp;
+            zero16(s);
+            s = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(now, pick_l, s, 0, 0, 0);
+            L::mma_rows(s, Qs, ln, kf);  // S[query][key] - lse / scale
+            // rows past the last query are copies of it; keys past the end are nobody's
+            if ((p.causal && q0 + off < r0 + 31) || q0 + 32 > w.nq) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = q0 + row_of(r, half);
+                    s[r] = i < w.nq && (!p.causal || key <= i + off) ? s[r] : -INFINITY;
+                }
+            }
+            zero16(dp);
+            dp = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(now, pick_d, dp, 0, 0, 0);
+            L::mma_images(dp, Ds, Vs + kb * 32 * L::ROWB, ln);  // dP[query][key] - delta
+            float x[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = exp2_fast(s[r] * c);
+            typename L::weights pw, dw;
+            L::pack(pw, x);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] *= dp[r];
+            L::pack(dw, x);
+            L::mma_cols(dv, Ds, ln, pw);  // dV^T[dim][key] += dO^T P
+            L::mma_cols(dk, Qs, ln, dw);  // dK^T[dim][key] += Q^T dS
+        }
+    }
+    // the later waves of a block hand their sums to the first, in order
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        f32x16* acc = side ? dk : dv;
+        __syncthreads();
+        if (qs > 0) put_sums<L::NDT>(smem + (kb * (QS - 1) + qs - 1) * BOX, acc, lane);
+        __syncthreads();
+        if (qs == 0) {
+#pragma unroll
+            for (int o = 0; o < QS - 1; ++o) add_sums<L::NDT>(smem + (kb * (QS - 1) + o) * BOX, acc, lane, 1.f, 1.f);
+        }
+    }
+    if (qs == 0 && mine) {
+        L::store_row((__bf16*)p.dk + (size_t)(w.k0 + key) * p.lddk + hk * DH, dk, p.scale, half);
+        L::store_row((__bf16*)p.dv + (size_t)(w.k0 + key) * p.lddv + hk * DH, dv, 1.f, half);
+    }
+}
+
+// rows of a workgroup's tile, as the plan's table lists them for queries and then for keys
+constexpr int TILE_ROWS[3] = {128, 64, 32};
 
 static int64_t tiles_of(const int* lens, int n, int rows) {
     int64_t t = 0;
@@ -374,7 +568,8 @@ using namespace capdec;
 extern "C" size_t capdec_packed_table_bytes(const int* lens_q, const int* lens_k, int n) {
     if (!lens_q || n <= 0 || !lengths_ok(lens_q, n) || (lens_k && !lengths_ok(lens_k, n))) return 0;
     const int* lk = lens_k ? lens_k : lens_q;
-    const int64_t items = tiles_of(lens_q, n, TALL) + tiles_of(lens_q, n, SHORT) + tiles_of(lk, n, TALL) + tiles_of(lk, n, SHORT);
+    int64_t items = 0;
+    for (int rows : TILE_ROWS) items += tiles_of(lens_q, n, rows) + tiles_of(lk, n, rows);
     return (size_t)(items > 0 ? items : 1) * sizeof(PackedItem);
 }
 
@@ -392,10 +587,10 @@ extern "C" int capdec_packed_plan(const int* lens_q, const int* lens_k, int n, i
     try {
         std::vector<PackedItem> all;
         all.reserve(need / sizeof(PackedItem));
-        int count[4] = {0, 0, 0, 0};
-        for (int part = 0; part < 4; ++part) {  // query tiles of 128 and 32 rows, key tiles of 128 and 32 rows
-            const bool keys = part >= 2;
-            const int rows = part & 1 ? SHORT : TALL;
+        int count[6] = {0, 0, 0, 0, 0, 0};
+        for (int part = 0; part < 6; ++part) {  // query tiles, then key tiles
+            const bool keys = part >= 3;
+            const int rows = TILE_ROWS[part % 3];
             const size_t begin = all.size();
             int q0 = 0, k0 = 0;
             for (int i = 0; i < n; ++i) {
@@ -422,7 +617,7 @@ extern "C" int capdec_packed_plan(const int* lens_q, const int* lens_k, int n, i
             seqs->rows_q += lens_q[i];
             seqs->rows_k += lk[i];
         }
-        for (int part = 0; part < 4; ++part) seqs->tiles[part] = count[part];
+        for (int part = 0; part < 6; ++part) seqs->tiles[part] = count[part];
         seqs->table = table_dev;
     } catch (const std::exception& e) {
         set_error("capdec_packed_plan: %s", e.what());
@@ -444,47 +639,58 @@ static int packed_check(const char* what, const capdec_packed_seqs* s, int Hq, i
     CAPDEC_REQUIRE(dtype == CAPDEC_F32 || dtype == CAPDEC_BF16S, "%s: dtype %d: fp32 (CAPDEC_F32) or bf16 (CAPDEC_BF16S) matrices", what, dtype);
     CAPDEC_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", what);
     CAPDEC_REQUIRE((int64_t)Hq * dh < (1 << 24), "%s: Hq=%d heads of %d: too wide", what, Hq, dh);
-    const int64_t most = std::max(std::max((int64_t)s->tiles[0], (int64_t)s->tiles[1]), std::max((int64_t)s->tiles[2], (int64_t)s->tiles[3]));
+    const int64_t most = std::max(s->tiles[2], s->tiles[5]);
     CAPDEC_REQUIRE(most * Hq < (1ll << 31), "%s: too many tiles for one launch", what);
     return 0;
 }
 
-// Four waves share the tiles they walk; one wave wastes fewer rows on short sequences.
-static bool tall(int tiles_tall, int tiles_short) { return 2 * (int64_t)tiles_short >= 5 * (int64_t)tiles_tall; }
+// items of one part of the table
+static const PackedItem* items_of(const capdec_packed_seqs* s, int part) {
+    const PackedItem* t = (const PackedItem*)s->table;
+    for (int i = 0; i < part; ++i) t += s->tiles[i];
+    return t;
+}
+
+#define CAPDEC_PACKED(kernel, part, heads, threads)                                                                    \
+    do {                                                                                                               \
+        p.items = items_of(s, part);                                                                                   \
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(s->tiles[part] * (heads))), dim3(threads), 0, st, p);               \
+    } while (0)
+
+// One wave a tile where most sequences fit 32 rows: a taller tile would be half empty, and its waves would wait for each
+// other (256 captions of up to 20 tokens, bf16: forward 5.8 us against 9.9, dq 6.9 / 11.7, dk and dv 7.7 / 15.7; sequences
+// of 33 to 64 the other way, backward 46 / 34).
+static bool short_rows(const int* tiles) { return 2 * (int64_t)tiles[2] < 3 * (int64_t)tiles[1]; }
+
+// 128 rows a workgroup where that makes two for each of the 256 CUs (6 prompts, 16 heads of 128: 196 us against 265 with
+// 64 rows); 64 rows and two waves a block where it does not (one prompt of 2000: 46 / 55).  fp32: always the latter: 32
+// keys of fp32 already fill the LDS of a 64-key tile, and at 128 dims 128 rows spill (32 paragraphs 26 / 39, 8 texts 152 / 300).
+template <typename T>
+static bool tall_rows(const int* tiles, int heads) { return sizeof(T) == 2 && (int64_t)tiles[0] * heads >= 512; }
 
 template <typename T, int DH>
 static void launch_fwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t st) {
-    const PackedItem* table = (const PackedItem*)s->table;
-    if (tall(s->tiles[0], s->tiles[1])) {
-        p.items = table;
-        hipLaunchKernelGGL((packed_fwd_kernel<T, DH, 4, sizeof(T) == 2 ? 2 : 1>), dim3(s->tiles[0] * p.Hq), dim3(256), 0, st, p);
-    } else {
-        p.items = table + s->tiles[0];
-        hipLaunchKernelGGL((packed_fwd_kernel<T, DH, 1, 1>), dim3(s->tiles[1] * p.Hq), dim3(64), 0, st, p);
-    }
+    if (short_rows(s->tiles)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
+    else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
+    else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 4, 1, 2>), 0, p.Hq, 256);
 }
 
 template <typename T, int DH>
 static void launch_bwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t st) {
-    const PackedItem* table = (const PackedItem*)s->table;
+    const bool one = short_rows(s->tiles + 3);
+    if (sizeof(T) == 2 && !one) p.stats = p.delta;
     if (s->tiles[0] > 0) {
-        if (tall(s->tiles[0], s->tiles[1])) {
-            p.items = table;
-            hipLaunchKernelGGL((packed_bwd_dq_kernel<T, DH, 4, sizeof(T) == 2 ? 2 : 1>), dim3(s->tiles[0] * p.Hq), dim3(256), 0, st, p);
-        } else {
-            p.items = table + s->tiles[0];
-            hipLaunchKernelGGL((packed_bwd_dq_kernel<T, DH, 1, 1>), dim3(s->tiles[1] * p.Hq), dim3(64), 0, st, p);
-        }
+        if (short_rows(s->tiles)) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
+        else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
+        else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 4, 1, 2>), 0, p.Hq, 256);
     }
-    if (s->tiles[2] > 0) {
-        const PackedItem* keys = table + s->tiles[0] + s->tiles[1];
-        if (tall(s->tiles[2], s->tiles[3])) {
-            p.items = keys;
-            hipLaunchKernelGGL((packed_bwd_dkv_kernel<T, DH, 4>), dim3(s->tiles[2] * p.Hkv), dim3(256), 0, st, p);
-        } else {
-            p.items = keys + s->tiles[2];
-            hipLaunchKernelGGL((packed_bwd_dkv_kernel<T, DH, 1>), dim3(s->tiles[3] * p.Hkv), dim3(64), 0, st, p);
-        }
+    if (s->tiles[3] > 0) {
+        if (one) CAPDEC_PACKED((packed_bwd_dkv_kernel<T, DH, 1, 1>), 5, p.Hkv, 64);
+        else if constexpr (sizeof(T) == 4) CAPDEC_PACKED((packed_bwd_dkv_kernel<T, DH, 2, 2>), 4, p.Hkv, 256);
+        // 64 keys and two waves a block; 32 keys and four where 64 would leave CUs without a workgroup (one text of 2000 tokens,
+        // 16 heads over 2: backward 261 us against 399; 32 paragraphs of 8 heads of 128 the other way, 73 / 48)
+        else if ((int64_t)s->tiles[4] * p.Hkv < 256) CAPDEC_PACKED((packed16_bwd_dkv_kernel<DH, 1, 4>), 5, p.Hkv, 256);
+        else CAPDEC_PACKED((packed16_bwd_dkv_kernel<DH, 2, 2>), 4, p.Hkv, 256);
     }
 }
 

@@ -16,6 +16,7 @@ namespace capdec {
 
 typedef __bf16 bf16x8t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4t __attribute__((ext_vector_type(4)));
+typedef short s16x4t __attribute__((ext_vector_type(4)));
 typedef float f32x4t __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
@@ -79,6 +80,15 @@ struct AttTile<__bf16, DH> {
         for (int ks = 0; ks < NF; ++ks) {
             const bf16x8t a = *reinterpret_cast<const bf16x8t*>(img + (l.row ^ (ks << 5)));
             acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[ks], acc, 0, 0, 0);
+        }
+    }
+    // the same with both operands in LDS
+    __device__ static __forceinline__ void mma_images(f32x16& acc, const unsigned char* img, const unsigned char* own, const lanes& l) {
+#pragma unroll
+        for (int ks = 0; ks < NF; ++ks) {
+            const bf16x8t a = *reinterpret_cast<const bf16x8t*>(img + (l.row ^ (ks << 5)));
+            const bf16x8t b = *reinterpret_cast<const bf16x8t*>(own + (l.row ^ (ks << 5)));
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
         }
     }
     __device__ static __forceinline__ void pack(weights& w, const float* x) {
@@ -173,6 +183,92 @@ struct AttTile<float, DH> {
             }
     }
 };
+
+// a value the compiler has to take as it is here: nothing made from it is kept from an earlier turn of a loop
+__device__ __forceinline__ void opaque(int& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void opaque(unsigned& x) { asm volatile("" : "+v"(x)); }
+
+// ---- tiles that travel global -> LDS without registers (bf16) -------------------------------------------------------
+// The transposing reads below are inline assembly because the compiler waits for every DMA in flight before the builtin
+// form (it cannot tell that the DMA fills another image); each block waits for its own reads.
+template <int DH>
+struct DmaTile : AttTile<__bf16, DH> {
+    using B = AttTile<__bf16, DH>;
+    static constexpr int ROWS_PER = 64 / B::PPR;  // rows of one 1 KiB transfer
+    // rows row0 .. row0 + ROWS - 1 of a matrix (head slice at g) -> image, shared out over NW waves; rows past the last one
+    // (n - 1) are copies of it.  ROWS * ROWB / 1024 / NW transfers a wave.  Uniform base plus a 32-bit lane offset, made anew
+    // every time: kept across a loop, the addresses would take the registers that the accumulators need.
+    template <int ROWS, int NW>
+    __device__ static __forceinline__ void fetch(unsigned char* img, const __bf16* g, int ld, int row0, int n, int wave, int lane) {
+        constexpr int N = ROWS / ROWS_PER / NW;
+        static_assert(ROWS % (ROWS_PER * NW) == 0, "every wave moves the same number of transfers");
+        const char* base = (const char*)(g + (size_t)row0 * ld);
+        const unsigned pitch = (unsigned)ld * 2u;
+        const int last = n - 1 - row0;
+        unsigned at = lane;
+        opaque(at);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = (wave * N + j) * ROWS_PER + (int)(at / B::PPR);
+            const unsigned piece = (at % B::PPR) ^ (unsigned)B::swz(r);
+            const unsigned off = (unsigned)min(r, last) * pitch + piece * 16u;
+            __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)(base + off),
+                                             (void __attribute__((address_space(3)))*)(img + (wave * N + j) * 1024), 16, 0, 0);
+        }
+    }
+    __device__ static __forceinline__ unsigned lds_addr(const unsigned char* p) {
+        return (unsigned)(size_t)(const __attribute__((address_space(3))) unsigned char*)p;
+    }
+    template <int OFF>
+    __device__ static __forceinline__ void read_cols(bf16x4t* lo, bf16x4t* hi, const unsigned* a0, const unsigned* a1) {
+        if constexpr (B::NDT == 4)
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
+                "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
+                "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+                "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
+                : "v"(a0[0]), "v"(a1[0]), "v"(a0[1]), "v"(a1[1]), "v"(a0[2]), "v"(a1[2]), "v"(a0[3]), "v"(a1[3]), "n"(OFF)
+                : "memory");
+        else
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
+                "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+                : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
+                : "v"(a0[0]), "v"(a1[0]), "v"(a0[1]), "v"(a1[1]), "n"(OFF)
+                : "memory");
+    }
+    // AttTile::mma_cols with its reads as above
+    __device__ static __forceinline__ void mma_cols(f32x16* out, const unsigned char* img, const typename B::lanes& l,
+                                                    const typename B::weights& w) {
+        const unsigned base = lds_addr(img);
+        int c0 = l.col[0], c1 = l.col[1];
+        opaque(c0);
+        opaque(c1);
+        unsigned a0[B::NDT], a1[B::NDT];
+#pragma unroll
+        for (int dt = 0; dt < B::NDT; ++dt) {
+            a0[dt] = base + (unsigned)(c0 ^ (dt << 6));
+            a1[dt] = base + (unsigned)(c1 ^ (dt << 6));
+        }
+        bf16x4t lo[B::NDT], hi[B::NDT];
+        read_cols<0>(lo, hi, a0, a1);
+#pragma unroll
+        for (int dt = 0; dt < B::NDT; ++dt)
+            out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join(lo[dt], hi[dt]), w.f[0], out[dt], 0, 0, 0);
+        read_cols<16 * B::ROWB>(lo, hi, a0, a1);
+#pragma unroll
+        for (int dt = 0; dt < B::NDT; ++dt)
+            out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join(lo[dt], hi[dt]), w.f[1], out[dt], 0, 0, 0);
+    }
+    __device__ static __forceinline__ bf16x8t join(bf16x4t a, bf16x4t b) { return bf16x8t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+};
+// every transfer of this wave has landed, and every wave of the workgroup has come this far
+__device__ __forceinline__ void dma_sync() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 // ROWS consecutive rows of a matrix on their way global -> registers -> LDS image, shared out over NT threads in
 // 16-byte pieces.  Rows at or past `n` become zeros: a weight of zero times whatever lies behind the last row (the next

@@ -1028,7 +1028,8 @@ def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=Non
             _packed_mat(t, name + n, q.dtype, rows, width)
         out.append(t)
     _on_current(name, o, do, lse, *out)
-    delta = torch.empty_like(lse)
+    # scratch: rowsum(do * o), with bf16 matrices 16 bytes for each (head, row)
+    delta = torch.empty(lse.numel() * (1 if q.dtype == torch.float32 else 4), dtype=torch.float32, device=q.device)
     dq, dk, dv = out
     check(lib().capdec_attn_packed_bwd(C.byref(seqs.c), ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0), ptr(o),
                                        o.stride(0), ptr(do), do.stride(0), ptr(lse), ptr(delta), lse.shape[1], ptr(dq), dq.stride(0),

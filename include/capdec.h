@@ -367,7 +367,7 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
  * reference pads every caption to one length (ref dataset.py:213-228). */
 typedef struct capdec_packed_seqs {
     int n, causal, rows_q, rows_k;
-    int tiles[4]; /* query tiles of 128 / 32 rows, key tiles of 128 / 32 rows */
+    int tiles[6]; /* query tiles of 128 / 64 / 32 rows, key tiles of 128 / 64 / 32 rows */
     const void* table;
 } capdec_packed_seqs;
 size_t capdec_packed_table_bytes(const int* lens_q, const int* lens_k, int n); /* 0: bad lengths */

@@ -260,12 +260,12 @@ def test_plans_and_arguments_are_refused_without_a_gpu():
     lib = _capi.lib()
     ints = lambda *v: (C.c_int * len(v))(*v)
     assert lib.capdec_packed_table_bytes(ints(3, -1), None, 2) == 0
-    assert lib.capdec_packed_table_bytes(ints(128, 0, 129), None, 3) == 32 * 2 * (1 + 2 + 4 + 5)
+    assert lib.capdec_packed_table_bytes(ints(128, 0, 129), None, 3) == 32 * 2 * (1 + 2 + 2 + 3 + 4 + 5)
     s = _capi.PackedSeqs()
     assert lib.capdec_packed_plan(ints(3), None, 1, 1, 16, 1, C.byref(s)) == -4  # the table does not fit
     assert lib.capdec_packed_plan(ints(3), ints(-1), 1, 1, 16, 1024, C.byref(s)) == -1
     s.rows_q = s.rows_k = 3
-    s.tiles[:] = [1, 1, 1, 1]
+    s.tiles[:] = [1] * 6
     s.table = 16
     good = dict(q=16, ldq=128, k=16, ldk=64, v=16, ldv=64, o=16, ldo=128, Hq=2, Hkv=1, dh=64, dtype=0, scale=0.1, rows=3)
     for change in (dict(Hq=3, Hkv=2), dict(Hkv=0), dict(dh=32), dict(dtype=1), dict(scale=0.0), dict(scale=-1.0),

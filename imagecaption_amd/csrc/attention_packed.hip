@@ -113,6 +113,7 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd
     for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
     Running run;
     run.init();
+    landed(qf);
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
         const unsigned char* Ks = smem + (t & 1) * 2 * IMG + ksp * 32 * KB * L::ROWB;
@@ -263,6 +264,8 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
     f32x16 acc[L::NDT];
 #pragma unroll
     for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
+    landed(qf);
+    landed(df);
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
         const unsigned char* Ks = smem + (t & 1) * 2 * IMG + ksp * 32 * KB * L::ROWB;
@@ -371,6 +374,8 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && sizeof(T) == 2 ? 2 : 
         zero16(dk[dt]);
         zero16(dv[dt]);
     }
+    landed(kf);
+    if constexpr (!V_LDS) landed(vf);
     for (int t = 0; t < nt; ++t) {
         qst.store(smem, tid);
         dst.store(smem + IMG, tid);
@@ -486,6 +491,7 @@ __global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd
         zero16(dk[dt]);
         zero16(dv[dt]);
     }
+    landed(kf);
     int qt = first;
     for (int t = 0; t < nt; ++t) {
         dma_sync();
@@ -629,7 +635,8 @@ extern "C" int capdec_packed_plan(const int* lens_q, const int* lens_k, int n, i
 namespace capdec {
 
 static bool packed_mat(const void* p, int ld, int width, int es, int rows) {
-    return rows == 0 || (p && aligned16(p) && ld >= width && ld % (16 / es) == 0);
+    // (a tile's rows are addressed by 32-bit offsets: 128 rows of at most 2^25 bytes)
+    return rows == 0 || (p && aligned16(p) && ld >= width && ld % (16 / es) == 0 && (int64_t)ld * es <= (1 << 25));
 }
 
 static int packed_check(const char* what, const capdec_packed_seqs* s, int Hq, int Hkv, int dh, int dtype, float scale) {
@@ -704,7 +711,7 @@ extern "C" int capdec_attn_packed_fwd(const capdec_packed_seqs* seqs, const void
     CAPDEC_REQUIRE(packed_mat(q, ldq, Hq * dh, es, seqs->rows_q) && packed_mat(k, ldk, Hkv * dh, es, seqs->rows_k) &&
                        packed_mat(v, ldv, Hkv * dh, es, seqs->rows_k) && packed_mat(o, ldo, Hq * dh, es, seqs->rows_q),
                    "capdec_attn_packed_fwd: matrices must be non-null, 16-byte aligned, with row strides that are multiples of 16 "
-                   "bytes and cover the heads");
+                   "bytes, cover the heads and do not pass 2^25 bytes");
     CAPDEC_REQUIRE(!lse || stat_rows >= (size_t)seqs->rows_q, "capdec_attn_packed_fwd: stat_rows=%zu below the %d query rows", stat_rows, seqs->rows_q);
     if (seqs->rows_q == 0) return 0;
     PackedParams p;
@@ -734,7 +741,7 @@ extern "C" int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void
                        packed_mat(dout, lddo, Hq * dh, es, seqs->rows_q) && packed_mat(dq, lddq, Hq * dh, es, seqs->rows_q) &&
                        packed_mat(dk, lddk, Hkv * dh, es, seqs->rows_k) && packed_mat(dv, lddv, Hkv * dh, es, seqs->rows_k),
                    "capdec_attn_packed_bwd: matrices must be non-null, 16-byte aligned, with row strides that are multiples of 16 "
-                   "bytes and cover the heads");
+                   "bytes, cover the heads and do not pass 2^25 bytes");
     CAPDEC_REQUIRE(seqs->rows_q == 0 || (lse && delta && stat_rows >= (size_t)seqs->rows_q),
                    "capdec_attn_packed_bwd: lse / delta missing, or stat_rows=%zu below the %d query rows", stat_rows, seqs->rows_q);
     PackedParams p;

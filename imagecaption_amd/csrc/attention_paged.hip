@@ -77,44 +77,64 @@ __device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
     return w;
 }
 
-// the split's page ids into LDS; ids outside the cache become -1 and are counted
-__device__ __forceinline__ void load_ids(int* ids, const PagedParams& p, const PagedItem& w, int tid, int nt) {
+// the split's pages into LDS, as byte offsets of this head's first row there; pages outside the cache become -1
+// and are counted; *bad tells that there are some
+__device__ __forceinline__ void load_pages(int64_t* pages, int* bad, const PagedParams& p, const PagedItem& w, int row_bytes, int tid, int nt) {
+    if (tid == 0) *bad = 0;
+    __syncthreads();
     const int first = w.kbegin >> p.page_log2, n = w.kend > w.kbegin ? ((w.kend - 1) >> p.page_log2) - first + 1 : 0;
     const int* row = p.table + (size_t)w.seq * p.ld_table + first;
     for (int i = tid; i < n; i += nt) {
-        int id = row[i];
-        if (id < 0 || id >= p.pages) {
-            id = -1;
+        const int id = row[i];
+        int64_t at = -1;
+        if (id >= 0 && id < p.pages) at = (((int64_t)id * p.Hkv + w.hk) << p.page_log2) * row_bytes;
+        else {
+            *bad = 1;
             if (w.hk == 0 && w.tile == 0) atomicAdd(&g_bad_pages, 1u);
         }
-        ids[i] = id;
+        pages[i] = at;
     }
 }
 
-// ROWS keys (or values) of one head on their way pages -> registers -> LDS image, shared out over NT threads in 16-byte
+// ROWS keys and values of one head on their way pages -> registers -> LDS images, shared out over NT threads in 16-byte
 // pieces; positions past the split's end or on a bad page become zeros
 template <bool E4M3, int DH, int NT, int ROWS>
 struct PageStage {
     using L = AttTile<__bf16, DH>;
-    static constexpr int RB = E4M3 ? DH : 2 * DH, PP = RB / 16, N = (ROWS * PP + NT - 1) / NT;
+    static constexpr int RB = E4M3 ? DH : 2 * DH, PP = RB / 16, N = ROWS * PP / NT;
     static_assert(ROWS * PP % NT == 0, "every thread moves the same number of pieces");
-    uint4 r[N];
-    __device__ __forceinline__ void load(const void* base, const int* ids, int first_page, int head, int heads, int page_log2, int key0,
-                                         int kend, int tid) {
-        const int mask = (1 << page_log2) - 1;
+    uint4 k[N], v[N];
+    // whole: every position of the run exists (wave-uniform): all page offsets are read, then all rows are requested
+    __device__ __forceinline__ void load(const PagedParams& p, const int64_t* pages, int first_page, int key0, int kend, bool whole, int tid) {
+        const int mask = (1 << p.page_log2) - 1;
+        size_t at[N];
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int key = key0 + (j * NT + tid) / PP, piece = (j * NT + tid) % PP;
+                at[j] = (size_t)pages[(key >> p.page_log2) - first_page] + (unsigned)((key & mask) * RB + piece * 16);
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) k[j] = *reinterpret_cast<const uint4*>((const unsigned char*)p.k + at[j]);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = *reinterpret_cast<const uint4*>((const unsigned char*)p.v + at[j]);
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int key = key0 + (j * NT + tid) / PP, piece = (j * NT + tid) % PP;
-            r[j] = uint4{0, 0, 0, 0};
+            k[j] = v[j] = uint4{0, 0, 0, 0};
             if (key < kend) {
-                const int id = ids[(key >> page_log2) - first_page];
-                if (id >= 0)
-                    r[j] = *reinterpret_cast<const uint4*>((const unsigned char*)base +
-                                                           ((((size_t)id * heads + head) << page_log2) + (key & mask)) * RB + piece * 16);
+                const int64_t page = pages[(key >> p.page_log2) - first_page];
+                if (page >= 0) {
+                    at[0] = (size_t)page + (unsigned)((key & mask) * RB + piece * 16);
+                    k[j] = *reinterpret_cast<const uint4*>((const unsigned char*)p.k + at[0]);
+                    v[j] = *reinterpret_cast<const uint4*>((const unsigned char*)p.v + at[0]);
+                }
             }
         }
     }
-    __device__ __forceinline__ void store(unsigned char* img, int tid) const {
+    __device__ static __forceinline__ void put(unsigned char* img, const uint4* r, int tid) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int row = (j * NT + tid) / PP, piece = (j * NT + tid) % PP;
@@ -127,18 +147,23 @@ struct PageStage {
             }
         }
     }
+    __device__ __forceinline__ void store(unsigned char* kimg, unsigned char* vimg, int tid) const {
+        put(kimg, k, tid);
+        put(vimg, v, tid);
+    }
 };
 
-// key `key`'s scale of one head; zero past the split's end or on a bad page.  *there: the position exists
-__device__ __forceinline__ void key_scales(const PagedParams& p, const int* ids, int first_page, int head, int key, int kend, bool e4m3,
-                                           float& sk, float& sv, bool& there) {
+// scales of one key and its value; zero past the split's end or on a bad page.  there: the position exists
+template <bool E4M3, int DH>
+__device__ __forceinline__ void key_scales(const PagedParams& p, const int64_t* pages, int first_page, int key, int kend, float& sk, float& sv,
+                                           bool& there) {
     sk = sv = 0.f;
     there = false;
     if (key < kend) {
-        const int id = ids[(key >> p.page_log2) - first_page];
-        there = id >= 0;
-        if (there && e4m3) {
-            const size_t at = (((size_t)id * p.Hkv + head) << p.page_log2) + (key & ((1 << p.page_log2) - 1));
+        const int64_t page = pages[(key >> p.page_log2) - first_page];
+        there = page >= 0;
+        if (E4M3 && there) {
+            const size_t at = (size_t)page / DH + (key & ((1 << p.page_log2) - 1));
             sk = p.ks[at];
             sv = p.vs[at];
         }
@@ -158,15 +183,17 @@ __global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedPa
     using L = AttTile<__bf16, DH>;
     constexpr int IMG = 32 * L::ROWB;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[8 * IMG];
-    __shared__ int ids[SPLIT_IDS];
+    __shared__ int64_t pages[SPLIT_IDS];
+    __shared__ int s_bad;
     __shared__ __attribute__((aligned(16))) float sc[4][2][32];
     __shared__ float ml[4][2][32];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const PagedItem w = paged_place(p);
     if (!w.ok) return;
     const int nrows = w.nq * p.group;
-    load_ids(ids, p, w, tid, 256);
+    load_pages(pages, &s_bad, p, w, E4M3 ? DH : 2 * DH, tid, 256);
     __syncthreads();
+    const bool good = s_bad == 0;
     const int first_page = w.kbegin >> p.page_log2;
     const typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
@@ -191,28 +218,27 @@ __global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedPa
 #pragma unroll
             for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[b][dt]);
         }
-        PageStage<E4M3, DH, 64, 32> ks, vs;
+        PageStage<E4M3, DH, 64, 32> st;
         float sk, sv;
         bool there;
         int k0 = w.kbegin + wave * 32;
         if (k0 < w.kend) {
-            ks.load(p.k, ids, first_page, w.hk, p.Hkv, p.page_log2, k0, w.kend, lane);
-            vs.load(p.v, ids, first_page, w.hk, p.Hkv, p.page_log2, k0, w.kend, lane);
-            key_scales(p, ids, first_page, w.hk, k0 + l31, w.kend, E4M3, sk, sv, there);
+            st.load(p, pages, first_page, k0, w.kend, good && k0 + 32 <= w.kend, lane);
+            key_scales<E4M3, DH>(p, pages, first_page, k0 + l31, w.kend, sk, sv, there);
         }
+#pragma unroll
+        for (int b = 0; b < R; ++b) landed(qf[b]);
         for (; k0 < w.kend; k0 += 128) {
             // one wave's LDS operations execute in order: the previous run's reads are done before these writes land
-            ks.store(Ks, lane);
-            vs.store(Vs, lane);
+            st.store(Ks, Vs, lane);
             if (E4M3 && half == 0) {
                 sc[wave][0][l31] = sk;
                 sc[wave][1][l31] = sv;
             }
             const uint32_t exists = (uint32_t)__ballot(there);
             if (k0 + 128 < w.kend) {
-                ks.load(p.k, ids, first_page, w.hk, p.Hkv, p.page_log2, k0 + 128, w.kend, lane);
-                vs.load(p.v, ids, first_page, w.hk, p.Hkv, p.page_log2, k0 + 128, w.kend, lane);
-                key_scales(p, ids, first_page, w.hk, k0 + 128 + l31, w.kend, E4M3, sk, sv, there);
+                st.load(p, pages, first_page, k0 + 128, w.kend, good && k0 + 160 <= w.kend, lane);
+                key_scales<E4M3, DH>(p, pages, first_page, k0 + 128 + l31, w.kend, sk, sv, there);
             }
             wave_fence();
             const bool plain = exists == 0xffffffffu && k0 + 32 <= lo_see;
@@ -340,14 +366,17 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     using L = AttTile<__bf16, DH>;
     constexpr int KB = 2, BN = 32 * KB, IMG = BN * L::ROWB;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
-    __shared__ int ids[SPLIT_IDS];
+    __shared__ int64_t pages[SPLIT_IDS];
+    __shared__ int s_bad;
     __shared__ __attribute__((aligned(16))) float sc[2][2][BN];
     __shared__ uint32_t exist[2][KB];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const PagedItem w = paged_place(p);
     if (!w.ok) return;
     const int nrows = w.nq * p.group;
-    load_ids(ids, p, w, tid, 256);
+    load_pages(pages, &s_bad, p, w, E4M3 ? DH : 2 * DH, tid, 256);
+    __syncthreads();
+    const bool good = s_bad == 0;
     const int first_page = w.kbegin >> p.page_log2;
     const typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
@@ -365,19 +394,17 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
         for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
         Running run;
         run.init();
-        PageStage<E4M3, DH, 256, BN> ks, vs;
+        PageStage<E4M3, DH, 256, BN> st;
         float sk, sv;
         bool there = false;
         auto fetch = [&](int t) {
             const int k0 = w.kbegin + t * BN;
-            ks.load(p.k, ids, first_page, w.hk, p.Hkv, p.page_log2, k0, w.kend, tid);
-            vs.load(p.v, ids, first_page, w.hk, p.Hkv, p.page_log2, k0, w.kend, tid);
-            if (tid < BN) key_scales(p, ids, first_page, w.hk, k0 + tid, w.kend, E4M3, sk, sv, there);
+            st.load(p, pages, first_page, k0, w.kend, good && k0 + BN <= w.kend, tid);
+            if (tid < BN) key_scales<E4M3, DH>(p, pages, first_page, k0 + tid, w.kend, sk, sv, there);
         };
         auto put = [&](int t) {
             unsigned char* img = smem + (t & 1) * 2 * IMG;
-            ks.store(img, tid);
-            vs.store(img + IMG, tid);
+            st.store(img, img + IMG, tid);
             if (tid < BN) {  // wave 0
                 if (E4M3) {
                     sc[t & 1][0][tid] = sk;
@@ -392,6 +419,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
             fetch(0);
             put(0);
         }
+        landed(qf);
         __syncthreads();
         for (int t = 0; t < nt; ++t) {
             const unsigned char* Ks = smem + (t & 1) * 2 * IMG;
@@ -484,13 +512,12 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     }
 }
 
-// one wave for each (row, head): the splits' contexts joined in split order
+// a workgroup for each (row, head): its four waves take every fourth split's context and join in wave order
 template <int DH>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
-    const int lane = threadIdx.x & 63;
-    const size_t at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const size_t all = (size_t)p.rows * p.Hq;
-    if (at >= all) return;
+    __shared__ float box[4][DH + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t at = blockIdx.x, all = (size_t)p.rows * p.Hq;
     const int grow = (int)(at / p.Hq), head = (int)(at % p.Hq);
     if (p.cu ? (grow < p.cu[0] || grow >= p.cu[p.n]) : grow >= p.n) return;
     const int n = min(p.part_n[at], p.splits);
@@ -501,7 +528,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
     float l = 0.f;
     constexpr int E = DH / 64;
     float acc[E] = {};
-    for (int s = 0; s < n; ++s) {
+#pragma unroll 4
+    for (int s = wave; s < n; s += 4) {
         const float2 v = p.part_ml[s * all + at];
         const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : 1.f) : exp2_fast(v.x - m);
         l += v.y * f;
@@ -509,11 +537,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = __fmaf_rn(src[e], f, acc[e]);
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    __bf16* dst = p.o + (size_t)grow * p.ldo + head * DH + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = (__bf16)(acc[e] * inv);
-    if (p.lse && lane == 0) p.lse[(size_t)head * p.rows + grow] = l != 0.f ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
+    for (int e = 0; e < E; ++e) box[wave][lane * E + e] = acc[e];
+    if (lane == 0) box[wave][DH] = l;
+    __syncthreads();
+    if (tid >= DH) return;
+    l = ((box[0][DH] + box[1][DH]) + box[2][DH]) + box[3][DH];
+    const float o = ((box[0][tid] + box[1][tid]) + box[2][tid]) + box[3][tid];
+    p.o[(size_t)grow * p.ldo + head * DH + tid] = (__bf16)(l != 0.f ? o / l : 0.f);
+    if (p.lse && tid == 0) p.lse[(size_t)head * p.rows + grow] = l != 0.f ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
 }
 
 int paged_bad_count(unsigned int* count, bool reset) {
@@ -537,7 +569,8 @@ static PagedShape paged_shape(const capdec_kv_cache* c, int n, int max_q, int Hq
     s.block = s.rows_kernel ? 128 : (rows > 32 ? 64 : 32);
     s.tiles = (int)((rows + s.block - 1) / s.block);
     const int64_t keys = (int64_t)table_cols * c->page, units = (int64_t)n * c->heads * s.tiles;
-    int64_t splits = (1024 + units - 1) / units;
+    const int64_t want = getenv("PW") ? atoi(getenv("PW")) : 1024;
+    int64_t splits = (want + units - 1) / units;
     splits = std::min(splits, (keys + SPLIT_MIN - 1) / SPLIT_MIN);
     // a split's keys are rounded up to whole runs of 128 and its page ids have to fit LDS
     splits = std::max(splits, (keys + SPLIT_KEYS - 129) / (SPLIT_KEYS - 128));
@@ -552,7 +585,7 @@ static int paged_check(const char* what, const capdec_kv_cache* c, int n, int ro
     CAPDEC_REQUIRE((int64_t)table_cols * c->page < (1ll << 31) - SPLIT_KEYS, "%s: a page table of %d columns passes 2^31 positions", what, table_cols);
     CAPDEC_REQUIRE((int64_t)rows * (Hq / c->heads) < (1ll << 30) && (int64_t)max_q * (Hq / c->heads) < (1ll << 30), "%s: too many rows", what);
     const PagedShape s = paged_shape(c, n, max_q, Hq, table_cols);
-    CAPDEC_REQUIRE(((int64_t)n * c->heads * s.splits + 7) / 8 * 8 * s.tiles < (1ll << 31) && (int64_t)rows * Hq / 4 + 1 < (1ll << 31),
+    CAPDEC_REQUIRE(((int64_t)n * c->heads * s.splits + 7) / 8 * 8 * s.tiles < (1ll << 31) && (int64_t)rows * Hq < (1ll << 31),
                    "%s: too much work for one launch", what);
     return 0;
 }
@@ -624,7 +657,7 @@ extern "C" int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, in
     else CAPDEC_PAGED(false, 64);
 #undef CAPDEC_PAGED
     if (s.splits > 1) {
-        const dim3 grid((unsigned)(((size_t)rows * Hq + 3) / 4));
+        const dim3 grid((unsigned)((size_t)rows * Hq));
         if (wide) hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, st, p);
         else hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, st, p);
     }

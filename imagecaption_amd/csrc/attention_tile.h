@@ -188,6 +188,14 @@ struct AttTile<float, DH> {
 __device__ __forceinline__ void opaque(int& x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ void opaque(unsigned& x) { asm volatile("" : "+v"(x)); }
 
+// row fragments loaded before a loop are taken there: left to the compiler, the wait for them would stand inside the loop
+// and drain the loop's own requests every turn
+template <typename F, int N>
+__device__ __forceinline__ void landed(F (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
 // ---- tiles that travel global -> LDS without registers (bf16) -------------------------------------------------------
 // The transposing reads below are inline assembly because the compiler waits for every DMA in flight before the builtin
 // form (it cannot tell that the DMA fills another image); each block waits for its own reads.
@@ -280,11 +288,22 @@ struct Staged {
     static_assert(ROWS * L::PPR % NT == 0, "every thread moves the same number of pieces");
     uint4 r[N];
     __device__ __forceinline__ void load(const T* g, int ld, int row0, int n, int tid) {
+        // uniform base plus a 32-bit lane offset; no branch between the requests of a tile that lies inside the matrix
+        const char* base = (const char*)(g + (size_t)row0 * ld);
+        const unsigned pitch = (unsigned)ld * (unsigned)L::ES;
+        if (row0 + ROWS <= n) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int row = row0 + (j * NT + tid) / L::PPR, piece = (j * NT + tid) % L::PPR;
-            r[j] = uint4{0, 0, 0, 0};
-            if (row < n) r[j] = *reinterpret_cast<const uint4*>(g + (size_t)row * ld + piece * L::EPP);
+            for (int j = 0; j < N; ++j) {
+                const unsigned row = (j * NT + tid) / L::PPR, piece = (j * NT + tid) % L::PPR;
+                r[j] = *reinterpret_cast<const uint4*>(base + (row * pitch + piece * 16u));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const unsigned row = (j * NT + tid) / L::PPR, piece = (j * NT + tid) % L::PPR;
+                r[j] = uint4{0, 0, 0, 0};
+                if (row0 + (int)row < n) r[j] = *reinterpret_cast<const uint4*>(base + (row * pitch + piece * 16u));
+            }
         }
     }
     __device__ __forceinline__ void store(unsigned char* img, int tid) const {

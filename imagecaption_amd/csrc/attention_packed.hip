@@ -203,6 +203,120 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd
     }
 }
 
+// The forward of bf16 matrices with 128 rows a workgroup: 64 keys at a time by DMA, one tile ahead.  Registers for the tile
+// on its way would leave none for reading LDS ahead of the matrix instructions.
+template <int DH>
+__global__ __launch_bounds__(256, 2) void packed16_fwd_kernel(PackedParams p) {
+    using L = DmaTile<DH>;
+    constexpr int KB = 2, BN = 32 * KB, IMG = BN * L::ROWB;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    int head, it;
+    packed_place(p.Hq, head, it);
+    const PackedItem w = p.items[it];
+    const int hk = head / p.group;
+    const __bf16* kg = (const __bf16*)p.k + (size_t)w.k0 * p.ldk + hk * DH;
+    const __bf16* vg = (const __bf16*)p.v + (size_t)w.k0 * p.ldv + hk * DH;
+    const int r0 = w.t0 + wave * 32;              // this wave's first row
+    const int row = r0 + l31, off = w.nk - w.nq;  // causal: row sees keys j <= row + off
+    const int kmax = p.causal ? min(w.nk, min(w.t0 + 128, w.nq) + off) : w.nk;  // of the workgroup's last row
+    const int nt = kmax > 0 ? (kmax + BN - 1) / BN : 0;
+    // keys the wave's rows can see at all, and keys that all of them see (no mask below)
+    const int wave_end = r0 >= w.nq ? 0 : (p.causal ? min(w.nk, min(r0 + 32, w.nq) + off) : w.nk);
+    const int all_see = p.causal ? min(w.nk, r0 + 1 + off) : w.nk;
+    typename L::frag qf[L::NF];
+    L::load_row(qf, (const __bf16*)p.q + (size_t)(w.q0 + row) * p.ldq + head * DH, row < w.nq, half);
+    landed(qf);
+    typename L::template Fetch<BN, 4> fk, fv;
+    fk.init(p.ldk, wave, lane);
+    fv.init(p.ldv, wave, lane);
+    if (nt > 0) {
+        fk(smem, kg, p.ldk, 0, w.nk, wave, lane);
+        fv(smem + IMG, vg, p.ldv, 0, w.nk, wave, lane);
+    }
+    const typename L::lanes ln = L::make_lanes(lane);
+    const float c = p.scale * LOG2E;
+    f32x16 acc[L::NDT];
+#pragma unroll
+    for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
+    Running run;
+    run.init();
+    // the two images are two copies of the loop's body: their LDS addresses are constants
+    auto turn = [&](int t, unsigned char* cur, unsigned char* nx) __attribute__((always_inline)) {
+        const unsigned char* Ks = cur;
+        const unsigned char* Vs = Ks + IMG;
+        dma_sync();
+        if (t + 1 < nt) {
+            fk(nx, kg, p.ldk, (t + 1) * BN, w.nk, wave, lane);
+            fv(nx + IMG, vg, p.ldv, (t + 1) * BN, w.nk, wave, lane);
+        }
+        const int k0 = t * BN;
+        if (k0 < wave_end) {
+            f32x16 s[KB];
+            bf16x8t kf[KB][L::NF], vf[2 * L::NDT];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) L::read_rows(kf[b], Ks + b * 32 * L::ROWB, ln);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) zero16(s[b]);
+#pragma unroll
+            for (int ks = 0; ks < L::NF; ++ks)
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b][ks], qf[ks], s[b], 0, 0, 0);  // S^T[key][query]
+            __builtin_amdgcn_s_setprio(0);
+            L::read_cols(vf, Vs, ln);
+            __builtin_amdgcn_sched_barrier(0);
+            if (k0 + BN > all_see) {
+                const int see = p.causal ? min(w.nk, row + 1 + off) : w.nk;
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[b][r] = k0 + 32 * b + row_of(r, half) < see ? s[b][r] : -INFINITY;
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+            bool raised;
+            const float a = run.raise(top, c, &raised);
+            if (raised) {
+#pragma unroll
+                for (int dt = 0; dt < L::NDT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[dt][r] *= a;
+            }
+            const float base = run.base();
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                float x[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    x[r] = exp2_fast(__fmaf_rn(s[b][r], c, -base));
+                    run.l += x[r];
+                }
+                typename L::weights pw;
+                L::pack(pw, x);
+                L::mma_read_cols(acc, vf, pw);  // O^T[dim][query] += V^T P^T
+                if (b + 1 < KB) L::read_cols(vf, Vs + (b + 1) * 32 * L::ROWB, ln);
+            }
+        }
+    };
+    for (int t = 0; t < nt; t += 2) {
+        turn(t, smem, smem + 2 * IMG);
+        if (t + 1 < nt) turn(t + 1, smem + 2 * IMG, smem);
+    }
+    const float l = run.l + __shfl_xor(run.l, 32, 64);
+    if (row < w.nq) {
+        const bool any = l != 0.f;  // (NaN too: such a row is not an empty one)
+        L::store_row((__bf16*)p.out + (size_t)(w.q0 + row) * p.ldo + head * DH, acc, any ? 1.f / l : 0.f, half);
+        if (p.lse && half == 0)
+            p.lse[(size_t)head * p.stat_rows + w.q0 + row] = any ? (run.base() + __log2f(l)) * LN2 : -INFINITY;
+    }
+}
+
 // dq and delta = rowsum(do * o); blocks and waves as in the forward
 template <typename T, int DH, int RB, int KS, int KB>
 __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH == 64) ? 2 : 1) void packed_bwd_dq_kernel(PackedParams p) {
@@ -448,7 +562,7 @@ __global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd
     constexpr int BOX = DH / 4 * 16 * 64, WALK = 4 * IMG + KIMG;
     static_assert(KB * QS == 4 && KB * (QS - 1) * BOX <= WALK, "the sums of a block fit the images");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[WALK];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const int kb = wave % KB, qs = wave / KB;
     int hk, it;
     packed_place(p.Hkv, hk, it);
@@ -679,7 +793,7 @@ template <typename T, int DH>
 static void launch_fwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t st) {
     if (short_rows(s->tiles)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
     else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
-    else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 4, 1, 2>), 0, p.Hq, 256);
+    else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed16_fwd_kernel<DH>), 0, p.Hq, 256);
 }
 
 template <typename T, int DH>

@@ -112,6 +112,31 @@ struct AttTile<__bf16, DH> {
                 out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.f[m], out[dt], 0, 0, 0);
             }
     }
+    // the two steps of mma_rows / mma_cols apart, for callers that read ahead
+    __device__ static __forceinline__ void read_rows(bf16x8t* f, const unsigned char* img, const lanes& l) {
+#pragma unroll
+        for (int ks = 0; ks < NF; ++ks) f[ks] = *reinterpret_cast<const bf16x8t*>(img + (l.row ^ (ks << 5)));
+    }
+    __device__ static __forceinline__ void read_cols(bf16x8t* f, const unsigned char* img, const lanes& l) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+                const bf16x4t lo = read_tr(img + m * 16 * ROWB + (l.col[0] ^ (dt << 6)));
+                const bf16x4t hi = read_tr(img + m * 16 * ROWB + (l.col[1] ^ (dt << 6)));
+                f[m * NDT + dt] = bf16x8t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            }
+    }
+    __device__ static __forceinline__ void mma_read_rows(f32x16& acc, const bf16x8t* a, const frag* b) {
+#pragma unroll
+        for (int ks = 0; ks < NF; ++ks) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks], b[ks], acc, 0, 0, 0);
+    }
+    __device__ static __forceinline__ void mma_read_cols(f32x16* out, const bf16x8t* a, const weights& w) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[m * NDT + dt], w.f[m], out[dt], 0, 0, 0);
+    }
     // accumulators (rows = head dim, column = this lane's matrix row) -> that row, rounded once to bf16
     __device__ static __forceinline__ void store_row(__bf16* dst, const f32x16* acc, float mul, int half) {
 #pragma unroll
@@ -197,79 +222,56 @@ __device__ __forceinline__ void landed(F (&f)[N]) {
 }
 
 // ---- tiles that travel global -> LDS without registers (bf16) -------------------------------------------------------
-// The transposing reads below are inline assembly because the compiler waits for every DMA in flight before the builtin
-// form (it cannot tell that the DMA fills another image); each block waits for its own reads.
 template <int DH>
 struct DmaTile : AttTile<__bf16, DH> {
     using B = AttTile<__bf16, DH>;
     static constexpr int ROWS_PER = 64 / B::PPR;  // rows of one 1 KiB transfer
-    // rows row0 .. row0 + ROWS - 1 of a matrix (head slice at g) -> image, shared out over NW waves; rows past the last one
-    // (n - 1) are copies of it.  ROWS * ROWB / 1024 / NW transfers a wave.  Uniform base plus a 32-bit lane offset, made anew
-    // every time: kept across a loop, the addresses would take the registers that the accumulators need.
+    // Rows row0 .. row0 + ROWS - 1 of a matrix (head slice at g) -> image, shared out over NW waves; rows past the last one
+    // (n - 1) are copies of it.  ROWS * ROWB / 1024 / NW transfers a wave, each from a uniform base plus a 32-bit lane
+    // offset.  Inline assembly because the compiler, where it knows of a transfer in flight, waits for it before every
+    // transposing LDS read (it cannot tell that the transfer fills another image); the caller waits with dma_sync.  M0 is
+    // written and used here only: the compiler sets it anew before every use of its own.
+    template <int ROWS, int NW>
+    struct Fetch {
+        static constexpr int N = ROWS / ROWS_PER / NW;
+        static_assert(ROWS % (ROWS_PER * NW) == 0, "every wave moves the same number of transfers");
+        unsigned off[N];
+        // lane offsets for rows that lie inside the matrix
+        __device__ __forceinline__ void init(int ld, int wave, int lane) { offsets(off, ld, ROWS, wave, lane); }
+        __device__ static __forceinline__ void offsets(unsigned* o, int ld, int last, int wave, int lane) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int r = (wave * N + j) * ROWS_PER + lane / B::PPR;
+                o[j] = (unsigned)min(r, last) * ((unsigned)ld * 2u) + (((unsigned)(lane % B::PPR)) ^ (unsigned)B::swz(r)) * 16u;
+            }
+        }
+        __device__ static __forceinline__ void send(unsigned char* img, const char* base, const unsigned* o, int wave) {
+            const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(
+                (int)(unsigned)(size_t)(const __attribute__((address_space(3))) unsigned char*)(img + wave * N * 1024));
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + j * 1024), "v"(o[j]), "s"(base) : "memory");
+        }
+        __device__ __forceinline__ void operator()(unsigned char* img, const __bf16* g, int ld, int row0, int n, int wave, int lane) const {
+            const char* base = (const char*)(g + (size_t)row0 * ld);
+            if (row0 + ROWS <= n) {
+                send(img, base, off, wave);
+            } else {
+                unsigned o[N];
+                offsets(o, ld, n - 1 - row0, wave, lane);
+                send(img, base, o, wave);
+            }
+        }
+    };
+    // the same without offsets kept: for kernels whose accumulators leave no registers for them
     template <int ROWS, int NW>
     __device__ static __forceinline__ void fetch(unsigned char* img, const __bf16* g, int ld, int row0, int n, int wave, int lane) {
-        constexpr int N = ROWS / ROWS_PER / NW;
-        static_assert(ROWS % (ROWS_PER * NW) == 0, "every wave moves the same number of transfers");
-        const char* base = (const char*)(g + (size_t)row0 * ld);
-        const unsigned pitch = (unsigned)ld * 2u;
-        const int last = n - 1 - row0;
-        unsigned at = lane;
-        opaque(at);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int r = (wave * N + j) * ROWS_PER + (int)(at / B::PPR);
-            const unsigned piece = (at % B::PPR) ^ (unsigned)B::swz(r);
-            const unsigned off = (unsigned)min(r, last) * pitch + piece * 16u;
-            __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)(base + off),
-                                             (void __attribute__((address_space(3)))*)(img + (wave * N + j) * 1024), 16, 0, 0);
-        }
+        using F = Fetch<ROWS, NW>;
+        unsigned o[F::N];
+        opaque(lane);
+        F::offsets(o, ld, n - 1 - row0, wave, lane);
+        F::send(img, (const char*)(g + (size_t)row0 * ld), o, wave);
     }
-    __device__ static __forceinline__ unsigned lds_addr(const unsigned char* p) {
-        return (unsigned)(size_t)(const __attribute__((address_space(3))) unsigned char*)p;
-    }
-    template <int OFF>
-    __device__ static __forceinline__ void read_cols(bf16x4t* lo, bf16x4t* hi, const unsigned* a0, const unsigned* a1) {
-        if constexpr (B::NDT == 4)
-            asm volatile(
-                "ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
-                "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
-                "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
-                "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\ts_waitcnt lgkmcnt(0)"
-                : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
-                : "v"(a0[0]), "v"(a1[0]), "v"(a0[1]), "v"(a1[1]), "v"(a0[2]), "v"(a1[2]), "v"(a0[3]), "v"(a1[3]), "n"(OFF)
-                : "memory");
-        else
-            asm volatile(
-                "ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
-                "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"
-                : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
-                : "v"(a0[0]), "v"(a1[0]), "v"(a0[1]), "v"(a1[1]), "n"(OFF)
-                : "memory");
-    }
-    // AttTile::mma_cols with its reads as above
-    __device__ static __forceinline__ void mma_cols(f32x16* out, const unsigned char* img, const typename B::lanes& l,
-                                                    const typename B::weights& w) {
-        const unsigned base = lds_addr(img);
-        int c0 = l.col[0], c1 = l.col[1];
-        opaque(c0);
-        opaque(c1);
-        unsigned a0[B::NDT], a1[B::NDT];
-#pragma unroll
-        for (int dt = 0; dt < B::NDT; ++dt) {
-            a0[dt] = base + (unsigned)(c0 ^ (dt << 6));
-            a1[dt] = base + (unsigned)(c1 ^ (dt << 6));
-        }
-        bf16x4t lo[B::NDT], hi[B::NDT];
-        read_cols<0>(lo, hi, a0, a1);
-#pragma unroll
-        for (int dt = 0; dt < B::NDT; ++dt)
-            out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join(lo[dt], hi[dt]), w.f[0], out[dt], 0, 0, 0);
-        read_cols<16 * B::ROWB>(lo, hi, a0, a1);
-#pragma unroll
-        for (int dt = 0; dt < B::NDT; ++dt)
-            out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join(lo[dt], hi[dt]), w.f[1], out[dt], 0, 0, 0);
-    }
-    __device__ static __forceinline__ bf16x8t join(bf16x4t a, bf16x4t b) { return bf16x8t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
 };
 // every transfer of this wave has landed, and every wave of the workgroup has come this far
 __device__ __forceinline__ void dma_sync() {

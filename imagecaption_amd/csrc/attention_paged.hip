@@ -18,10 +18,12 @@
 namespace capdec {
 
 static __device__ unsigned int g_bad_pages;
+static __device__ uint4 g_zero_row[16];  // stands in for the rows of positions that do not exist
 
-constexpr int SPLIT_KEYS = 8192;             // most keys of a split: its page ids fit LDS
-constexpr int SPLIT_IDS = SPLIT_KEYS / 8 + 2;
-constexpr int SPLIT_MIN = 256;               // fewest keys worth a split of their own
+constexpr int SPLIT_PAGES = 512;  // most pages of a split: their offsets fit LDS
+constexpr int SPLIT_IDS = SPLIT_PAGES + 2;
+constexpr int SPLIT_MIN = 512;    // fewest keys worth a split of their own (and a second launch)
+constexpr int SPLIT_WANT = 384;   // splits in all to aim at: three for every two of the 256 CUs, which hold two workgroups each
 
 struct PagedParams {
     const void* k; const void* v; const float* ks; const float* vs;
@@ -40,22 +42,40 @@ struct PagedItem {
     bool ok;
 };
 
-// keys of one split of a sequence of `len` keys: as many splits as there are, of at least SPLIT_MIN keys, in whole runs of 128
-__device__ __forceinline__ int split_size(int len, int splits) {
-    int c = (len + splits - 1) / splits;
+// Keys of a split: the batch's keys shared out evenly over SPLIT_WANT workgroups, so that the longest sequence gets the most
+// splits and all splits take the same time (8 contexts of 9 to 60 thousand tokens, 32 heads over 4, e4m3: 49 us; aiming at 512:
+// 62 us, at 256: 60 us); at least SPLIT_MIN, at least what the grid's splits need for this sequence, in whole runs
+// of 128.  Every workgroup sums the lengths for itself: a read of n integers.
+__device__ __forceinline__ int split_size(const PagedParams& p, int64_t total, int len) {
+    const int64_t share = (total * p.Hkv * p.tiles + SPLIT_WANT - 1) / SPLIT_WANT;
+    int c = max((int)min(share, (int64_t)(1 << 30)), (len + p.splits - 1) / p.splits);
     c = max(c, SPLIT_MIN);
+    c = min(c, (SPLIT_PAGES << p.page_log2) - 128);
     return (c + 127) & ~127;
 }
 
 __device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
-    // the row tiles of one (sequence, head, split) read the same keys: they sit on one XCD (blockIdx % 8)
+    __shared__ int64_t sums[4];
+    const int cap = p.cols << p.page_log2;
+    if (p.splits > 1) {
+        int64_t total = 0;
+        for (int i = threadIdx.x; i < p.n; i += 256) total += min(max(p.lens[i], 0), cap);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            total += (int64_t)(((uint64_t)(uint32_t)__shfl_xor((int)(total >> 32), o, 64) << 32) | (uint32_t)__shfl_xor((int)total, o, 64));
+        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = total;
+    }
+    // The row tiles of one (sequence, head, split) go round the XCDs (blockIdx % 8): kept on one XCD they would share its L2,
+    // but a few such groups of up to 16 tiles do not divide by eight (a prompt chunk over four sequences: 134 us against
+    // 123).  Splits are the slowest index, and every further split turns the (sequence, head) pairs by three places: sequences
+    // that end early leave gaps, and these would all be on the same XCDs otherwise.
     PagedItem w;
-    const int blk = blockIdx.x, idx = blk >> 3;
-    w.tile = idx % p.tiles;
-    const int u = (idx / p.tiles) * 8 + (blk & 7);
-    w.ok = u < p.n * p.Hkv * p.splits;
-    w.split = u % p.splits;
-    const int sh = u / p.splits;
+    const int blk = blockIdx.x, pairs = p.n * p.Hkv;
+    w.tile = blk % p.tiles;
+    const int u = blk / p.tiles;
+    w.ok = u < pairs * p.splits;
+    w.split = u / pairs;
+    const int sh = (int)((u % pairs + 3u * (unsigned)w.split) % (unsigned)pairs);
     w.hk = sh % p.Hkv;
     w.seq = w.ok ? sh / p.Hkv : 0;
     if (p.cu) {
@@ -65,14 +85,21 @@ __device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
         w.a = w.seq;
         w.nq = 1;
     }
-    const int cap = p.cols << p.page_log2;
     const int len = p.lens[w.seq];
     w.len = min(max(len, 0), cap);
     if (len > cap && w.split == 0 && w.tile == 0 && w.hk == 0 && threadIdx.x == 0 && w.ok) atomicAdd(&g_bad_pages, 1u);
-    const int size = split_size(w.len, p.splits);
-    w.nsplit = max(1, (w.len + size - 1) / size);
-    w.kbegin = w.split * size;
-    w.kend = min(w.len, w.kbegin + size);
+    w.nsplit = 1;
+    w.kbegin = 0;
+    w.kend = w.len;
+    if (p.splits > 1) {
+        __syncthreads();
+        int size = split_size(p, sums[0] + sums[1] + sums[2] + sums[3], w.len);
+        w.nsplit = max(1, (w.len + size - 1) / size);
+        size = ((w.len + w.nsplit - 1) / w.nsplit + 127) & ~127;  // all of them alike, not whole ones and a rest
+        w.nsplit = max(1, (w.len + size - 1) / size);
+        w.kbegin = w.split * size;
+        w.kend = min(w.len, w.kbegin + size);
+    }
     w.ok = w.ok && w.split < w.nsplit;
     return w;
 }
@@ -96,43 +123,38 @@ __device__ __forceinline__ void load_pages(int64_t* pages, int* bad, const Paged
     }
 }
 
-// ROWS keys and values of one head on their way pages -> registers -> LDS images, shared out over NT threads in 16-byte
-// pieces; positions past the split's end or on a bad page become zeros
-template <bool E4M3, int DH, int NT, int ROWS>
+// No branches below: positions that do not exist are read from a row of zeros.  With branches the compiler cannot count the
+// requests in flight and waits for all of them where it needs the oldest.  kend - 1 has to be a position of the split.
+__device__ __forceinline__ const unsigned char* row_or_zeros(const void* base, size_t at, bool there) {
+    return there ? (const unsigned char*)base + at : reinterpret_cast<const unsigned char*>(g_zero_row);
+}
+
+// ROWS keys (K) and values of one head on their way pages -> registers -> LDS images, shared out over NT threads in 16-byte
+// pieces
+template <bool E4M3, int DH, int NT, int ROWS, bool K>
 struct PageStage {
     using L = AttTile<__bf16, DH>;
     static constexpr int RB = E4M3 ? DH : 2 * DH, PP = RB / 16, N = ROWS * PP / NT;
     static_assert(ROWS * PP % NT == 0, "every thread moves the same number of pieces");
-    uint4 k[N], v[N];
-    // whole: every position of the run exists (wave-uniform): all page offsets are read, then all rows are requested
-    __device__ __forceinline__ void load(const PagedParams& p, const int64_t* pages, int first_page, int key0, int kend, bool whole, int tid) {
+    uint4 k[K ? N : 1], v[N];
+    __device__ __forceinline__ void load(const PagedParams& p, const int64_t* pages, int first_page, int key0, int kend, int tid) {
         const int mask = (1 << p.page_log2) - 1;
-        size_t at[N];
-        if (whole) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int key = key0 + (j * NT + tid) / PP, piece = (j * NT + tid) % PP;
-                at[j] = (size_t)pages[(key >> p.page_log2) - first_page] + (unsigned)((key & mask) * RB + piece * 16);
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) k[j] = *reinterpret_cast<const uint4*>((const unsigned char*)p.k + at[j]);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = *reinterpret_cast<const uint4*>((const unsigned char*)p.v + at[j]);
-            return;
-        }
+        const unsigned char *ka[N], *va[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int key = key0 + (j * NT + tid) / PP, piece = (j * NT + tid) % PP;
-            k[j] = v[j] = uint4{0, 0, 0, 0};
-            if (key < kend) {
-                const int64_t page = pages[(key >> p.page_log2) - first_page];
-                if (page >= 0) {
-                    at[0] = (size_t)page + (unsigned)((key & mask) * RB + piece * 16);
-                    k[j] = *reinterpret_cast<const uint4*>((const unsigned char*)p.k + at[0]);
-                    v[j] = *reinterpret_cast<const uint4*>((const unsigned char*)p.v + at[0]);
-                }
-            }
+            const int64_t page = pages[(min(key, kend - 1) >> p.page_log2) - first_page];
+            const size_t at = (size_t)page + (unsigned)((key & mask) * RB + piece * 16);
+            const bool there = key < kend && page >= 0;
+            if constexpr (K) ka[j] = row_or_zeros(p.k, at, there);
+            va[j] = row_or_zeros(p.v, at, there);
         }
+        if constexpr (K) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) k[j] = *reinterpret_cast<const uint4*>(ka[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = *reinterpret_cast<const uint4*>(va[j]);
     }
     __device__ static __forceinline__ void put(unsigned char* img, const uint4* r, int tid) {
 #pragma unroll
@@ -147,26 +169,65 @@ struct PageStage {
             }
         }
     }
-    __device__ __forceinline__ void store(unsigned char* kimg, unsigned char* vimg, int tid) const {
-        put(kimg, k, tid);
-        put(vimg, v, tid);
+};
+
+// 32 keys of one head straight into matrix operands: a lane holds every second 16-byte piece of its key's row (its partner
+// lane ^ 32 the others).  The order in which a product takes the head dimension is free as long as both operands agree:
+// an e4m3 piece feeds two k-steps, so the queries' pieces are taken in that order.
+template <bool E4M3, int DH>
+struct KeyFrags {
+    using L = AttTile<__bf16, DH>;
+    static constexpr int RB = E4M3 ? DH : 2 * DH, N = RB / 32;
+    uint4 r[N];
+    float sk, sv;
+    __device__ __forceinline__ void load(const PagedParams& p, const int64_t* pages, int first_page, int key, int kend, int half) {
+        const int64_t page = pages[(min(key, kend - 1) >> p.page_log2) - first_page];
+        const int at = key & ((1 << p.page_log2) - 1);
+        const bool there = key < kend && page >= 0;
+        const unsigned char* row = row_or_zeros(p.k, (size_t)page + (unsigned)(at * RB), there) + 16 * half;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const uint4*>(row + (there ? 32 * i : 0));
+        if constexpr (E4M3) {
+            sk = *(there ? p.ks + (size_t)page / DH + at : reinterpret_cast<const float*>(g_zero_row));
+            sv = *(there ? p.vs + (size_t)page / DH + at : reinterpret_cast<const float*>(g_zero_row));
+        }
+    }
+    // acc[key][row] += keys x rows^T; q: this lane's row in the image of rows, sw: its swizzle
+    __device__ __forceinline__ void mma(f32x16& acc, const unsigned char* q, int sw, int half) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (E4M3) {
+                const int piece = 2 * (2 * i + half);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8t, e4m3_to_bf16(r[i].x, r[i].y)),
+                                                              *reinterpret_cast<const bf16x8t*>(q + ((piece ^ sw) << 4)), acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8t, e4m3_to_bf16(r[i].z, r[i].w)),
+                                                              *reinterpret_cast<const bf16x8t*>(q + (((piece + 1) ^ sw) << 4)), acc, 0, 0, 0);
+            } else {
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8t, r[i]),
+                                                              *reinterpret_cast<const bf16x8t*>(q + (((2 * i + half) ^ sw) << 4)), acc, 0, 0, 0);
+            }
+        }
     }
 };
 
-// scales of one key and its value; zero past the split's end or on a bad page.  there: the position exists
-template <bool E4M3, int DH>
-__device__ __forceinline__ void key_scales(const PagedParams& p, const int64_t* pages, int first_page, int key, int kend, float& sk, float& sv,
-                                           bool& there) {
-    sk = sv = 0.f;
-    there = false;
-    if (key < kend) {
-        const int64_t page = pages[(key >> p.page_log2) - first_page];
-        there = page >= 0;
-        if (E4M3 && there) {
-            const size_t at = (size_t)page / DH + (key & ((1 << p.page_log2) - 1));
-            sk = p.ks[at];
-            sv = p.vs[at];
-        }
+// scales of one key and its value; zero past the split's end or on a bad page (no branches, as above)
+template <int DH>
+__device__ __forceinline__ void key_scales(const PagedParams& p, const int64_t* pages, int first_page, int key, int kend, float& sk, float& sv) {
+    const int64_t page = pages[(min(key, kend - 1) >> p.page_log2) - first_page];
+    const size_t at = (size_t)page / DH + (key & ((1 << p.page_log2) - 1));
+    const bool there = key < kend && page >= 0;
+    sk = *(there ? p.ks + at : reinterpret_cast<const float*>(g_zero_row));
+    sv = *(there ? p.vs + at : reinterpret_cast<const float*>(g_zero_row));
+}
+
+// scores of 32 keys from k0 on that this lane's row does not see, that lie past the split or on a bad page: -infinity
+__device__ __forceinline__ void hide(f32x16& s, const PagedParams& p, const int64_t* pages, int first_page, int k0, int end, bool good, int half) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int key = k0 + row_of(r, half);
+        bool there = key < end;
+        if (!good && there) there = pages[(key >> p.page_log2) - first_page] >= 0;
+        s[r] = there ? s[r] : -INFINITY;
     }
 }
 
@@ -177,12 +238,15 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// R blocks of 32 rows; every wave walks its own runs of 32 keys
+// R blocks of 32 rows; every wave walks its own runs of 32 keys, one run ahead in registers.  The rows are the same for all
+// waves and stay in LDS; values pass through an LDS image (their operand is transposed), keys go to the matrix
+// instructions as they come: less LDS for a workgroup and a shorter way through each run, which is what bounds the kernel (a
+// run's steps depend on each other, so the rate is the number of waves a CU holds).
 template <bool E4M3, int DH, int R>
-__global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedParams p) {
+__global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2)) void paged_keys_kernel(PagedParams p) {
     using L = AttTile<__bf16, DH>;
     constexpr int IMG = 32 * L::ROWB;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[8 * IMG];
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[(4 + R) * IMG];
     __shared__ int64_t pages[SPLIT_IDS];
     __shared__ int s_bad;
     __shared__ __attribute__((aligned(16))) float sc[4][2][32];
@@ -192,24 +256,25 @@ __global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedPa
     if (!w.ok) return;
     const int nrows = w.nq * p.group;
     load_pages(pages, &s_bad, p, w, E4M3 ? DH : 2 * DH, tid, 256);
-    __syncthreads();
-    const bool good = s_bad == 0;
     const int first_page = w.kbegin >> p.page_log2;
     const typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
-    unsigned char* Ks = smem + wave * 2 * IMG;
-    unsigned char* Vs = Ks + IMG;
+    unsigned char* Vs = smem + wave * IMG;
+    unsigned char* Qs = smem + 4 * IMG;
 
     for (int tile = w.tile; tile * 32 * R < nrows; tile += p.tiles) {
-        int see[R], lo_see = 0x7fffffff;
-        typename L::frag qf[R][L::NF];
 #pragma unroll
-        for (int b = 0; b < R; ++b) {
-            const int r = tile * 32 * R + b * 32 + l31, token = r / p.group, g = r % p.group;
-            see[b] = w.len - w.nq + token + 1;
-            lo_see = min(lo_see, w.len - w.nq + (tile * 32 * R + b * 32) / p.group + 1);
-            L::load_row(qf[b], p.q + (size_t)(w.a + token) * p.ldq + (w.hk * p.group + g) * DH, r < nrows, half);
+        for (int j = 0; j < 32 * R * L::PPR / 256; ++j) {
+            const int rl = (j * 256 + tid) / L::PPR, piece = (j * 256 + tid) % L::PPR, r = tile * 32 * R + rl;
+            uint4 v = {0, 0, 0, 0};
+            if (r < nrows)
+                v = *reinterpret_cast<const uint4*>(p.q + (size_t)(w.a + r / p.group) * p.ldq + (w.hk * p.group + r % p.group) * DH + piece * 8);
+            *reinterpret_cast<uint4*>(Qs + rl * L::ROWB + ((piece ^ L::swz(rl & 31)) << 4)) = v;
         }
+        int see[R];
+#pragma unroll
+        for (int b = 0; b < R; ++b) see[b] = min(w.kend, w.len - w.nq + (tile * 32 * R + b * 32 + l31) / p.group + 1);
+        const int all_see = min(w.kend, w.len - w.nq + tile * 32 * R / p.group + 1);
         f32x16 acc[R][L::NDT];
         Running run[R];
 #pragma unroll
@@ -218,53 +283,47 @@ __global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedPa
 #pragma unroll
             for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[b][dt]);
         }
-        PageStage<E4M3, DH, 64, 32> st;
-        float sk, sv;
-        bool there;
+        __syncthreads();  // pages, rows
+        const bool good = s_bad == 0;
+        KeyFrags<E4M3, DH> kf;
+        PageStage<E4M3, DH, 64, 32, false> st;
         int k0 = w.kbegin + wave * 32;
         if (k0 < w.kend) {
-            st.load(p, pages, first_page, k0, w.kend, good && k0 + 32 <= w.kend, lane);
-            key_scales<E4M3, DH>(p, pages, first_page, k0 + l31, w.kend, sk, sv, there);
+            kf.load(p, pages, first_page, k0 + l31, w.kend, half);
+            st.load(p, pages, first_page, k0, w.kend, lane);
         }
-#pragma unroll
-        for (int b = 0; b < R; ++b) landed(qf[b]);
         for (; k0 < w.kend; k0 += 128) {
-            // one wave's LDS operations execute in order: the previous run's reads are done before these writes land
-            st.store(Ks, Vs, lane);
-            if (E4M3 && half == 0) {
-                sc[wave][0][l31] = sk;
-                sc[wave][1][l31] = sv;
-            }
-            const uint32_t exists = (uint32_t)__ballot(there);
-            if (k0 + 128 < w.kend) {
-                st.load(p, pages, first_page, k0 + 128, w.kend, good && k0 + 160 <= w.kend, lane);
-                key_scales<E4M3, DH>(p, pages, first_page, k0 + 128 + l31, w.kend, sk, sv, there);
-            }
-            wave_fence();
-            const bool plain = exists == 0xffffffffu && k0 + 32 <= lo_see;
+            f32x16 s[R];
 #pragma unroll
             for (int b = 0; b < R; ++b) {
-                f32x16 s;
-                zero16(s);
-                L::mma_rows(s, Ks, ln, qf[b]);  // S^T[key][row]
+                zero16(s[b]);
+                kf.mma(s[b], Qs + b * IMG + l31 * L::ROWB, L::swz(l31), half);  // S^T[key][row]
+            }
+            // one wave's LDS operations execute in order: the previous run's reads are done before these writes land
+            if (E4M3 && half == 0) {
+                sc[wave][0][l31] = kf.sk;
+                sc[wave][1][l31] = kf.sv;
+            }
+            st.put(Vs, st.v, lane);
+            if (k0 + 128 < w.kend) {
+                kf.load(p, pages, first_page, k0 + 128 + l31, w.kend, half);
+                st.load(p, pages, first_page, k0 + 128, w.kend, lane);
+            }
+            wave_fence();
+#pragma unroll
+            for (int b = 0; b < R; ++b) {
                 if constexpr (E4M3) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const f32x4t f = *reinterpret_cast<const f32x4t*>(&sc[wave][0][8 * i + 4 * half]);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) s[4 * i + j] *= f[j];
+                        for (int j = 0; j < 4; ++j) s[b][4 * i + j] *= f[j];
                     }
                 }
-                if (!plain) {
+                if (!good || k0 + 32 > all_see) hide(s[b], p, pages, first_page, k0, see[b], good, half);
+                float top = s[b][0];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int kr = row_of(r, half);
-                        s[r] = ((exists >> kr) & 1) && k0 + kr < see[b] ? s[r] : -INFINITY;
-                    }
-                }
-                float top = s[0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[b][r]);
                 bool raised;
                 const float a = run[b].raise(top, c, &raised);
                 if (raised) {
@@ -281,7 +340,7 @@ __global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedPa
                     if constexpr (E4M3) f = *reinterpret_cast<const f32x4t*>(&sc[wave][1][8 * i + 4 * half]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float e = exp2_fast(__fmaf_rn(s[4 * i + j], c, -base));
+                        const float e = exp2_fast(__fmaf_rn(s[b][4 * i + j], c, -base));
                         run[b].l += e;
                         x[4 * i + j] = E4M3 ? e * f[j] : e;
                     }
@@ -292,8 +351,7 @@ __global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedPa
             }
             wave_fence();
         }
-        // join the four waves: statistics first, then the contexts through their (now free) images, in wave order
-        constexpr int PIECES = DH / 4;  // 16-byte pieces of an fp32 row
+        // join the four waves: statistics first, then the contexts, half the dims at a time, through their (now free) images
 #pragma unroll
         for (int b = 0; b < R; ++b) {
             const float l = run[b].l + __shfl_xor(run[b].l, 32, 64);
@@ -306,61 +364,66 @@ __global__ __launch_bounds__(256, R == 1 ? 2 : 1) void paged_keys_kernel(PagedPa
 #pragma unroll
             for (int i = 0; i < 4; ++i) m = fmaxf(m, ml[i][0][l31]);
             const float mine = run[b].m2 == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_fast(run[b].m2 - m);
-            float* ctx = reinterpret_cast<float*>(smem + wave * 2 * IMG);
-#pragma unroll
-            for (int dt = 0; dt < L::NDT; ++dt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int piece = dt * 8 + 2 * i + half;
-                    const f32x4t v = {acc[b][dt][4 * i] * mine, acc[b][dt][4 * i + 1] * mine, acc[b][dt][4 * i + 2] * mine,
-                                      acc[b][dt][4 * i + 3] * mine};
-                    *reinterpret_cast<f32x4t*>(ctx + l31 * DH + ((piece ^ (l31 & 15)) << 2)) = v;
-                }
-            __syncthreads();
             const int rl = tid >> 3, r = tile * 32 * R + b * 32 + rl;  // eight threads a row
-            if (r < nrows) {
-                float mm = -INFINITY, ll = 0.f;
+            float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mm = fmaxf(mm, ml[i][0][rl]);
+            for (int i = 0; i < 4; ++i) mm = fmaxf(mm, ml[i][0][rl]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float mi = ml[i][0][rl], li = ml[i][1][rl];
-                    ll += mi == -INFINITY ? li : li * exp2_fast(mi - mm);
-                }
-                const int token = r / p.group, head = w.hk * p.group + r % p.group, grow = w.a + token;
-                const bool any = ll != 0.f;
-                const size_t at = (size_t)grow * p.Hq + head;
-                const float inv = w.nsplit == 1 ? (any ? 1.f / ll : 0.f) : 1.f;
-                float* po = p.part_o + ((size_t)w.split * p.rows * p.Hq + at) * DH;
+            for (int i = 0; i < 4; ++i) {
+                const float mi = ml[i][0][rl], li = ml[i][1][rl];
+                ll += mi == -INFINITY ? li : li * exp2_fast(mi - mm);
+            }
+            const int token = r / p.group, head = w.hk * p.group + r % p.group, grow = w.a + token;
+            const bool any = ll != 0.f;
+            const size_t at = (size_t)grow * p.Hq + head;
+            const float inv = any ? 1.f / ll : 0.f;
+            constexpr int HD = DH / 2, PIECES = HD / 4;  // dims of a half, 16-byte pieces of an fp32 row of them
+            float* ctx = reinterpret_cast<float*>(Vs);
 #pragma unroll
-                for (int j = 0; j < PIECES / 8; ++j) {
-                    const int piece = j * 8 + (tid & 7);
-                    f32x4t v = {0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < 2; ++h) {
+                if (h) __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        v += *reinterpret_cast<const f32x4t*>(reinterpret_cast<const float*>(smem + i * 2 * IMG) + rl * DH + ((piece ^ (rl & 15)) << 2));
-                    if (w.nsplit == 1) {
-                        const bf16x4t out = {(__bf16)(v[0] * inv), (__bf16)(v[1] * inv), (__bf16)(v[2] * inv), (__bf16)(v[3] * inv)};
-                        *reinterpret_cast<bf16x4t*>(p.o + (size_t)grow * p.ldo + head * DH + piece * 4) = out;
-                    } else {
-                        *reinterpret_cast<f32x4t*>(po + piece * 4) = v;
+                for (int dt = h * L::NDT / 2; dt < (h + 1) * L::NDT / 2; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int piece = (dt - h * L::NDT / 2) * 8 + 2 * i + half;
+                        const f32x4t v = {acc[b][dt][4 * i] * mine, acc[b][dt][4 * i + 1] * mine, acc[b][dt][4 * i + 2] * mine,
+                                          acc[b][dt][4 * i + 3] * mine};
+                        *reinterpret_cast<f32x4t*>(ctx + l31 * HD + ((piece ^ (l31 & 7)) << 2)) = v;
+                    }
+                __syncthreads();
+                if (r < nrows) {
+#pragma unroll
+                    for (int j = 0; j < PIECES / 8; ++j) {
+                        const int piece = j * 8 + (tid & 7);
+                        f32x4t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            v += *reinterpret_cast<const f32x4t*>(reinterpret_cast<const float*>(smem + i * IMG) + rl * HD + ((piece ^ (rl & 7)) << 2));
+                        if (w.nsplit == 1) {
+                            const bf16x4t out = {(__bf16)(v[0] * inv), (__bf16)(v[1] * inv), (__bf16)(v[2] * inv), (__bf16)(v[3] * inv)};
+                            *reinterpret_cast<bf16x4t*>(p.o + (size_t)grow * p.ldo + head * DH + h * HD + piece * 4) = out;
+                        } else {
+                            *reinterpret_cast<f32x4t*>(p.part_o + ((size_t)w.split * p.rows * p.Hq + at) * DH + h * HD + piece * 4) = v;
+                        }
                     }
                 }
-                if ((tid & 7) == 0) {
-                    if (w.nsplit == 1) {
-                        if (p.lse) p.lse[(size_t)head * p.rows + grow] = any ? ((mm == -INFINITY ? 0.f : mm) + __log2f(ll)) * LN2 : -INFINITY;
-                    } else {
-                        p.part_ml[(size_t)w.split * p.rows * p.Hq + at] = float2{mm, ll};
-                    }
-                    if (w.split == 0 && p.part_n) p.part_n[at] = w.nsplit;
+            }
+            if (r < nrows && (tid & 7) == 0) {
+                if (w.nsplit == 1) {
+                    if (p.lse) p.lse[(size_t)head * p.rows + grow] = any ? ((mm == -INFINITY ? 0.f : mm) + __log2f(ll)) * LN2 : -INFINITY;
+                } else {
+                    p.part_ml[(size_t)w.split * p.rows * p.Hq + at] = float2{mm, ll};
                 }
+                if (w.split == 0 && p.part_n) p.part_n[at] = w.nsplit;
             }
             __syncthreads();
         }
     }
 }
 
-// 128 rows, 32 a wave; 64 keys at a time shared by the waves
+// 128 rows, 32 a wave; 64 keys at a time shared by the waves.  bf16 pages travel by DMA one tile ahead; e4m3 pages pass
+// through registers, where they become bf16.
 template <bool E4M3, int DH>
 __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     using L = AttTile<__bf16, DH>;
@@ -369,8 +432,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     __shared__ int64_t pages[SPLIT_IDS];
     __shared__ int s_bad;
     __shared__ __attribute__((aligned(16))) float sc[2][2][BN];
-    __shared__ uint32_t exist[2][KB];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const PagedItem w = paged_place(p);
     if (!w.ok) return;
     const int nrows = w.nq * p.group;
@@ -382,8 +444,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     const float c = p.scale * LOG2E;
     for (int tile = w.tile; tile * 128 < nrows; tile += p.tiles) {
         const int r0 = tile * 128 + wave * 32, r = r0 + l31, token = r / p.group, head = w.hk * p.group + r % p.group;
-        const int see = w.len - w.nq + token + 1;
-        const int all_see = w.len - w.nq + r0 / p.group + 1;
+        const int see = min(w.kend, w.len - w.nq + token + 1);
+        const int all_see = min(w.kend, w.len - w.nq + r0 / p.group + 1);
         const int wave_end = r0 < nrows ? min(w.kend, w.len - w.nq + min(r0 + 31, nrows - 1) / p.group + 1) : 0;
         const int end = min(w.kend, w.len - w.nq + min(tile * 128 + 127, nrows - 1) / p.group + 1);
         const int nt = end > w.kbegin ? (end - w.kbegin + BN - 1) / BN : 0;
@@ -394,67 +456,82 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
         for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
         Running run;
         run.init();
-        PageStage<E4M3, DH, 256, BN> st;
+        PageStage<E4M3, DH, 256, BN, true> st;
         float sk, sv;
-        bool there = false;
-        auto fetch = [&](int t) {
+        // tile t into the images at img: by DMA at once, or into registers (put stores them)
+        auto fetch = [&](int t, unsigned char* img) {
             const int k0 = w.kbegin + t * BN;
-            st.load(p, pages, first_page, k0, w.kend, good && k0 + BN <= w.kend, tid);
-            if (tid < BN) key_scales<E4M3, DH>(p, pages, first_page, k0 + tid, w.kend, sk, sv, there);
+            if constexpr (E4M3) {
+                st.load(p, pages, first_page, k0, w.kend, tid);
+                if (tid < BN) key_scales<DH>(p, pages, first_page, k0 + tid, w.kend, sk, sv);
+            } else {
+                constexpr int PER = 64 / L::PPR, N = BN / PER / 4;  // rows of a 1 KiB transfer, transfers of a wave
+                const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(
+                    (int)(unsigned)(size_t)(const __attribute__((address_space(3))) unsigned char*)(img + wave * N * 1024));
+                const int mask = (1 << p.page_log2) - 1;
+                int64_t at[N];
+                unsigned within[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const int rl = (wave * N + j) * PER + lane / L::PPR, key = min(k0 + rl, w.kend - 1);
+                    at[j] = pages[(key >> p.page_log2) - first_page];
+                    within[j] = (unsigned)((key & mask) * L::ROWB) + (((unsigned)(lane % L::PPR)) ^ (unsigned)L::swz(rl & 31)) * 16u;
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const unsigned char* ka = (const unsigned char*)p.k + at[j] + within[j];
+                    const unsigned char* va = (const unsigned char*)p.v + at[j] + within[j];
+                    if (!good && at[j] < 0) ka = va = reinterpret_cast<const unsigned char*>(g_zero_row) + within[j] % L::ROWB;
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + j * 1024), "v"(ka) : "memory");
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + IMG + j * 1024), "v"(va) : "memory");
+                }
+            }
         };
-        auto put = [&](int t) {
-            unsigned char* img = smem + (t & 1) * 2 * IMG;
-            st.store(img, img + IMG, tid);
-            if (tid < BN) {  // wave 0
-                if (E4M3) {
+        auto put = [&](int t, unsigned char* img) {
+            if constexpr (E4M3) {
+                st.put(img, st.k, tid);
+                st.put(img + IMG, st.v, tid);
+                if (tid < BN) {
                     sc[t & 1][0][tid] = sk;
                     sc[t & 1][1][tid] = sv;
                 }
-                const uint64_t all = __ballot(there);
-                if (tid < KB) exist[t & 1][tid] = (uint32_t)(all >> (32 * tid));
             }
         };
-        __syncthreads();  // page ids; the images of the previous tile are free
-        if (nt > 0) {
-            fetch(0);
-            put(0);
-        }
-        landed(qf);
-        __syncthreads();
-        for (int t = 0; t < nt; ++t) {
-            const unsigned char* Ks = smem + (t & 1) * 2 * IMG;
+        auto turn = [&](int t, unsigned char* cur, unsigned char* nx) __attribute__((always_inline)) {
+            const unsigned char* Ks = cur;
             const unsigned char* Vs = Ks + IMG;
             const bool more = t + 1 < nt;
-            if (more) fetch(t + 1);
+            if constexpr (!E4M3) dma_sync();
+            if (more) fetch(t + 1, nx);
             __builtin_amdgcn_sched_barrier(0);
             const int k0 = w.kbegin + t * BN;
             if (k0 < wave_end) {
                 f32x16 s[KB];
-                uint32_t ex[KB];
-                bool plain = k0 + BN <= all_see;
+                bf16x8t kf[KB][L::NF], vf[2 * L::NDT];
 #pragma unroll
-                for (int b = 0; b < KB; ++b) {
-                    ex[b] = exist[t & 1][b];
-                    plain = plain && ex[b] == 0xffffffffu;
-                    zero16(s[b]);
-                    L::mma_rows(s[b], Ks + b * 32 * L::ROWB, ln, qf);
-                    if constexpr (E4M3) {
+                for (int b = 0; b < KB; ++b) L::read_rows(kf[b], Ks + b * 32 * L::ROWB, ln);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int b = 0; b < KB; ++b) zero16(s[b]);
+#pragma unroll
+                for (int ks = 0; ks < L::NF; ++ks)
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b][ks], qf[ks], s[b], 0, 0, 0);  // S^T[key][row]
+                L::read_cols(vf, Vs, ln);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (E4M3) {
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const f32x4t f = *reinterpret_cast<const f32x4t*>(&sc[t & 1][0][32 * b + 8 * i + 4 * half]);
 #pragma unroll
                             for (int j = 0; j < 4; ++j) s[b][4 * i + j] *= f[j];
                         }
-                    }
                 }
-                if (!plain) {
+                if (!good || k0 + BN > all_see) {
 #pragma unroll
-                    for (int b = 0; b < KB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int kr = row_of(i, half);
-                            s[b][i] = ((ex[b] >> kr) & 1) && k0 + 32 * b + kr < see ? s[b][i] : -INFINITY;
-                        }
+                    for (int b = 0; b < KB; ++b) hide(s[b], p, pages, first_page, k0 + 32 * b, see, good, half);
                 }
                 float top = s[0][0];
 #pragma unroll
@@ -486,13 +563,27 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
                     }
                     typename L::weights pw;
                     L::pack(pw, x);
-                    L::mma_cols(acc, Vs + b * 32 * L::ROWB, ln, pw);
+                    L::mma_read_cols(acc, vf, pw);  // O^T[dim][row] += V^T P^T
+                    if (b + 1 < KB) L::read_cols(vf, Vs + (b + 1) * 32 * L::ROWB, ln);
                 }
             }
-            if (more) {
-                put(t + 1);
-                __syncthreads();
+            if constexpr (E4M3) {
+                if (more) {
+                    put(t + 1, nx);
+                    __syncthreads();
+                }
             }
+        };
+        landed(qf);
+        __syncthreads();  // the images of the previous tile of rows are free
+        if (nt > 0) {
+            fetch(0, smem);
+            put(0, smem);
+        }
+        if constexpr (E4M3) __syncthreads();
+        for (int t = 0; t < nt; t += 2) {
+            turn(t, smem, smem + 2 * IMG);
+            if (t + 1 < nt) turn(t + 1, smem + 2 * IMG, smem);
         }
         const float l = run.l + __shfl_xor(run.l, 32, 64);
         if (r < nrows) {
@@ -512,16 +603,17 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     }
 }
 
-// a workgroup for each (row, head): its four waves take every fourth split's context and join in wave order
-template <int DH>
+// The splits' contexts of one (row, head) by W waves that take every W-th split and join in wave order: four where there
+// are few rows, one where there are many.
+template <int DH, int W>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
-    __shared__ float box[4][DH + 1];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const size_t at = blockIdx.x, all = (size_t)p.rows * p.Hq;
+    __shared__ float box[4][DH + 2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = wave % W;
+    const size_t all = (size_t)p.rows * p.Hq, at = (size_t)blockIdx.x * (4 / W) + wave / W;
     const int grow = (int)(at / p.Hq), head = (int)(at % p.Hq);
-    if (p.cu ? (grow < p.cu[0] || grow >= p.cu[p.n]) : grow >= p.n) return;
-    const int n = min(p.part_n[at], p.splits);
-    if (n <= 1) return;
+    int n = 0;
+    if (at < all && (p.cu ? (grow >= p.cu[0] && grow < p.cu[p.n]) : grow < p.n)) n = min(p.part_n[at], p.splits);
+    if (n <= 1) return;  // W > 1: the whole workgroup has this item
     float m = -INFINITY;
     for (int s = lane; s < n; s += 64) m = fmaxf(m, p.part_ml[s * all + at].x);
     m = wave_max(m);
@@ -529,7 +621,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
     constexpr int E = DH / 64;
     float acc[E] = {};
 #pragma unroll 4
-    for (int s = wave; s < n; s += 4) {
+    for (int s = part; s < n; s += W) {
         const float2 v = p.part_ml[s * all + at];
         const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : 1.f) : exp2_fast(v.x - m);
         l += v.y * f;
@@ -537,15 +629,28 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = __fmaf_rn(src[e], f, acc[e]);
     }
+    if constexpr (W > 1) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) box[wave][lane * E + e] = acc[e];
-    if (lane == 0) box[wave][DH] = l;
-    __syncthreads();
-    if (tid >= DH) return;
-    l = ((box[0][DH] + box[1][DH]) + box[2][DH]) + box[3][DH];
-    const float o = ((box[0][tid] + box[1][tid]) + box[2][tid]) + box[3][tid];
-    p.o[(size_t)grow * p.ldo + head * DH + tid] = (__bf16)(l != 0.f ? o / l : 0.f);
-    if (p.lse && tid == 0) p.lse[(size_t)head * p.rows + grow] = l != 0.f ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
+        for (int e = 0; e < E; ++e) box[wave][lane * E + e] = acc[e];
+        if (lane == 0) box[wave][DH] = l;
+        __syncthreads();
+        if (wave > 0) return;
+        l = ((box[0][DH] + box[1][DH]) + box[2][DH]) + box[3][DH];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = lane * E + e;
+            acc[e] = ((box[0][i] + box[1][i]) + box[2][i]) + box[3][i];
+        }
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    __bf16* dst = p.o + (size_t)grow * p.ldo + head * DH + lane * E;
+    if constexpr (E == 2) {
+        typedef __bf16 pair __attribute__((ext_vector_type(2)));
+        *reinterpret_cast<pair*>(dst) = pair{(__bf16)(acc[0] * inv), (__bf16)(acc[1] * inv)};
+    } else {
+        dst[0] = (__bf16)(acc[0] * inv);
+    }
+    if (p.lse && lane == 0) p.lse[(size_t)head * p.rows + grow] = l != 0.f ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
 }
 
 int paged_bad_count(unsigned int* count, bool reset) {
@@ -568,12 +673,13 @@ static PagedShape paged_shape(const capdec_kv_cache* c, int n, int max_q, int Hq
     s.rows_kernel = rows > 64;
     s.block = s.rows_kernel ? 128 : (rows > 32 ? 64 : 32);
     s.tiles = (int)((rows + s.block - 1) / s.block);
+    // the longest sequence of a ragged batch gets up to four times the even share of splits; workgroups without one end at once
     const int64_t keys = (int64_t)table_cols * c->page, units = (int64_t)n * c->heads * s.tiles;
-    const int64_t want = getenv("PW") ? atoi(getenv("PW")) : 1024;
-    int64_t splits = (want + units - 1) / units;
+    int64_t splits = units >= SPLIT_WANT ? 1 : (4 * SPLIT_WANT + units - 1) / units;
     splits = std::min(splits, (keys + SPLIT_MIN - 1) / SPLIT_MIN);
-    // a split's keys are rounded up to whole runs of 128 and its page ids have to fit LDS
-    splits = std::max(splits, (keys + SPLIT_KEYS - 129) / (SPLIT_KEYS - 128));
+    // (a split's keys are rounded up to whole runs of 128)
+    const int64_t most = (int64_t)SPLIT_PAGES * c->page - 128;
+    splits = std::max(splits, (keys + most - 1) / most);
     s.splits = (int)std::max<int64_t>(splits, 1);
     return s;
 }
@@ -582,10 +688,10 @@ static int paged_check(const char* what, const capdec_kv_cache* c, int n, int ro
     if (int rc = kv_cache_check(what, c)) return rc;
     CAPDEC_REQUIRE(n > 0 && rows >= 0 && max_q > 0 && table_cols > 0, "%s: bad shape n=%d rows=%d max_q=%d table_cols=%d", what, n, rows, max_q, table_cols);
     CAPDEC_REQUIRE(Hq > 0 && Hq % c->heads == 0 && (int64_t)Hq * c->dh < (1 << 24), "%s: Hq=%d must be a multiple of the cache's %d heads", what, Hq, c->heads);
-    CAPDEC_REQUIRE((int64_t)table_cols * c->page < (1ll << 31) - SPLIT_KEYS, "%s: a page table of %d columns passes 2^31 positions", what, table_cols);
+    CAPDEC_REQUIRE((int64_t)table_cols * c->page < (1ll << 31) - (1 << 20), "%s: a page table of %d columns passes 2^31 positions", what, table_cols);
     CAPDEC_REQUIRE((int64_t)rows * (Hq / c->heads) < (1ll << 30) && (int64_t)max_q * (Hq / c->heads) < (1ll << 30), "%s: too many rows", what);
     const PagedShape s = paged_shape(c, n, max_q, Hq, table_cols);
-    CAPDEC_REQUIRE(((int64_t)n * c->heads * s.splits + 7) / 8 * 8 * s.tiles < (1ll << 31) && (int64_t)rows * Hq < (1ll << 31),
+    CAPDEC_REQUIRE((int64_t)n * c->heads * s.splits * s.tiles < (1ll << 31) && (int64_t)rows * Hq < (1ll << 31),
                    "%s: too much work for one launch", what);
     return 0;
 }
@@ -642,7 +748,7 @@ extern "C" int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, in
     p.ldq = ldq; p.ldo = ldo; p.ld_table = ld_table; p.cols = table_cols; p.n = n; p.rows = rows;
     p.Hq = Hq; p.Hkv = cache->heads; p.group = Hq / cache->heads; p.page_log2 = log2_of(cache->page); p.pages = cache->pages;
     p.splits = s.splits; p.tiles = s.tiles; p.scale = scale;
-    const unsigned blocks = (unsigned)(((int64_t)n * cache->heads * s.splits + 7) / 8 * 8 * s.tiles);
+    const unsigned blocks = (unsigned)((int64_t)n * cache->heads * s.splits * s.tiles);
     const bool e = cache->dtype == CAPDEC_E4M3, wide = cache->dh == 128;
     hipStream_t st = (hipStream_t)stream;
 #define CAPDEC_PAGED(E, D)                                                                                       \
@@ -657,9 +763,13 @@ extern "C" int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, in
     else CAPDEC_PAGED(false, 64);
 #undef CAPDEC_PAGED
     if (s.splits > 1) {
-        const dim3 grid((unsigned)((size_t)rows * Hq));
-        if (wide) hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, st, p);
+        const size_t items = (size_t)rows * Hq;
+        const bool few = items < 4096;
+        const dim3 grid((unsigned)(few ? items : (items + 3) / 4));
+        if (wide && few) hipLaunchKernelGGL((paged_join_kernel<128, 4>), grid, dim3(256), 0, st, p);
+        else if (wide) hipLaunchKernelGGL((paged_join_kernel<128, 1>), grid, dim3(256), 0, st, p);
+        else if (few) hipLaunchKernelGGL((paged_join_kernel<64, 4>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((paged_join_kernel<64, 1>), grid, dim3(256), 0, st, p);
     }
     return check_launch("capdec_attn_paged");
 }

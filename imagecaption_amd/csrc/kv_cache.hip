@@ -1,8 +1,8 @@
 // The paged key / value cache: rows written (rounded to e4m3 with one scale for each row of a head, or kept as bf16) and read
 // back.  See include/capdec.h (capdec_kv_write / capdec_kv_read).
 //
-// Pure streaming: DH / 8 lanes own one (token, head) row, 8 elements each, so a bf16 row is one 16-byte load a lane and the
-// row's largest magnitude is a shuffle tree over 8 or 16 lanes -- the row is read once.  Magnitudes are compared as integers
+// Pure streaming: DH / 8 lanes own one (token, head) row of both sides, 8 elements each, so a bf16 row is one 16-byte load a
+// lane and the row's largest magnitude is a shuffle tree over 8 or 16 lanes -- the row is read once.  Magnitudes are compared as integers
 // with the sign bit cleared: the order is the same and a NaN beats everything, so it reaches the scale.
 #include "paged.h"
 
@@ -48,68 +48,89 @@ __device__ __forceinline__ size_t cache_row(int slot, int head, int heads, int p
     return ((((size_t)page * heads + head) << page_log2) + at);
 }
 
-// blockIdx.y: 0 = keys, 1 = values
+// x / scale rounded as IEEE division rounds it, without a division for each element: with y the correctly rounded 1 / scale,
+// q = x y is within an ulp of the quotient and q + (x - q scale) y is the rounded quotient (Markstein's theorem); eight divisions
+// a lane made the write kernel bound by the vector units (40001 rows of 8 heads: 73 us)
+__device__ __forceinline__ float quotient(float x, float scale, float y) {
+    const float q = x * y;
+    return __fmaf_rn(__fmaf_rn(-q, scale, x), y, q);
+}
+
 template <typename T, bool E4M3, int DH>
 __global__ __launch_bounds__(256) void kv_write_kernel(KVParams p) {
     constexpr int LANES = DH / 8, PER = 256 / LANES;
-    const bool val = blockIdx.y != 0;
     const int lane = threadIdx.x % LANES;
     const int64_t item = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
     if (item >= (int64_t)p.rows * p.heads) return;
     const int row = (int)(item / p.heads), head = (int)(item % p.heads);
     const int slot = p.slots[row];
+    float x[2][8];
+    load_row8((const T*)p.rk + (size_t)row * p.ldk + head * DH + lane * 8, x[0]);
+    load_row8((const T*)p.rv + (size_t)row * p.ldv + head * DH + lane * 8, x[1]);
     if (slot < 0 || slot >= p.slots_total) {
-        if (slot >= 0 && lane == 0 && head == 0 && !val) atomicAdd(&g_bad_slots, 1u);
+        if (slot >= 0 && lane == 0 && head == 0) atomicAdd(&g_bad_slots, 1u);
         return;
     }
-    float x[8];
-    load_row8((const T*)(val ? p.rv : p.rk) + (size_t)row * (val ? p.ldv : p.ldk) + head * DH + lane * 8, x);
     const size_t at = cache_row(slot, head, p.heads, p.page_log2);
     if constexpr (E4M3) {
-        uint32_t top = 0;
+        uint32_t top[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        for (int s = 0; s < 2; ++s) {
 #pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-        const float scale = __uint_as_float(max(top, __float_as_uint(AMAX_FLOOR))) / E4M3_MAX;
-        // IEEE division: a code is the value nearest to x / scale, not to x times a rounded reciprocal
-        int lo = 0, hi = 0;
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] / scale, x[1] / scale, lo, false);
-        lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] / scale, x[3] / scale, lo, true);
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[4] / scale, x[5] / scale, hi, false);
-        hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[6] / scale, x[7] / scale, hi, true);
-        *reinterpret_cast<int2*>((unsigned char*)(val ? p.cv : p.ck) + at * DH + lane * 8) = int2{lo, hi};
-        if (lane == 0) (val ? p.sv : p.sk)[at] = scale;
+            for (int e = 0; e < 8; ++e) top[s] = max(top[s], __float_as_uint(x[s][e]) & 0x7fffffffu);
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) top[s] = max(top[s], (uint32_t)__shfl_xor((int)top[s], o, 64));
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const float scale = __uint_as_float(max(top[s], __float_as_uint(AMAX_FLOOR))) / E4M3_MAX, y = 1.f / scale;
+            float c[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c[e] = quotient(x[s][e], scale, y);
+            int lo = 0, hi = 0;
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], lo, false);
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(c[4], c[5], hi, false);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(c[6], c[7], hi, true);
+            *reinterpret_cast<int2*>((unsigned char*)(s ? p.cv : p.ck) + at * DH + lane * 8) = int2{lo, hi};
+            if (lane == 0) (s ? p.sv : p.sk)[at] = scale;
+        }
     } else {
-        store_row8((__bf16*)(val ? p.cv : p.ck) + at * DH + lane * 8, x);
+        store_row8((__bf16*)p.ck + at * DH + lane * 8, x[0]);
+        store_row8((__bf16*)p.cv + at * DH + lane * 8, x[1]);
     }
 }
 
 template <typename T, bool E4M3, int DH>
 __global__ __launch_bounds__(256) void kv_read_kernel(KVParams p) {
     constexpr int LANES = DH / 8, PER = 256 / LANES;
-    const bool val = blockIdx.y != 0;
     const int lane = threadIdx.x % LANES;
     const int64_t item = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
     if (item >= (int64_t)p.rows * p.heads) return;
     const int row = (int)(item / p.heads), head = (int)(item % p.heads);
     const int slot = p.slots[row];
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float x[2][8] = {};
     if (slot >= 0 && slot < p.slots_total) {
         const size_t at = cache_row(slot, head, p.heads, p.page_log2);
         if constexpr (E4M3) {
-            const int2 c = *reinterpret_cast<const int2*>((const unsigned char*)(val ? p.cv : p.ck) + at * DH + lane * 8);
-            const float scale = (val ? p.sv : p.sk)[at];
-            const bf16x8p v = e4m3_to_bf16((uint32_t)c.x, (uint32_t)c.y);
+            const int2 c[2] = {*reinterpret_cast<const int2*>((const unsigned char*)p.ck + at * DH + lane * 8),
+                               *reinterpret_cast<const int2*>((const unsigned char*)p.cv + at * DH + lane * 8)};
+            const float scale[2] = {p.sk[at], p.sv[at]};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (float)v[e] * scale;
+            for (int s = 0; s < 2; ++s) {
+                const bf16x8p v = e4m3_to_bf16((uint32_t)c[s].x, (uint32_t)c[s].y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[s][e] = (float)v[e] * scale[s];
+            }
         } else {
-            load_row8((const __bf16*)(val ? p.cv : p.ck) + at * DH + lane * 8, x);
+            load_row8((const __bf16*)p.ck + at * DH + lane * 8, x[0]);
+            load_row8((const __bf16*)p.cv + at * DH + lane * 8, x[1]);
         }
-    } else if (slot >= 0 && lane == 0 && head == 0 && !val) {
+    } else if (slot >= 0 && lane == 0 && head == 0) {
         atomicAdd(&g_bad_slots, 1u);
     }
-    store_row8((T*)(val ? p.ov : p.ok) + (size_t)row * (val ? p.ldv : p.ldk) + head * DH + lane * 8, x);
+    store_row8((T*)p.ok + (size_t)row * p.ldk + head * DH + lane * 8, x[0]);
+    store_row8((T*)p.ov + (size_t)row * p.ldv + head * DH + lane * 8, x[1]);
 }
 
 int kv_cache_check(const char* what, const capdec_kv_cache* c) {
@@ -153,7 +174,7 @@ using namespace capdec;
 #define CAPDEC_KV_LAUNCH(kernel)                                                                                     \
     do {                                                                                                             \
         const int per = 256 / (cache->dh / 8);                                                                       \
-        const dim3 grid((unsigned)(((int64_t)rows * cache->heads + per - 1) / per), 2);                              \
+        const dim3 grid((unsigned)(((int64_t)rows * cache->heads + per - 1) / per));                                 \
         const bool q8 = cache->dtype == CAPDEC_E4M3, f32 = dtype == CAPDEC_F32, wide = cache->dh == 128;             \
         hipStream_t st = (hipStream_t)stream;                                                                        \
         if (wide) {                                                                                                  \

@@ -949,62 +949,81 @@ class PackedSeqs:
         l = lib()
         self.table = torch.empty(l.capdec_packed_table_bytes(cq, ck, n), dtype=torch.uint8, device=device)
         self.c = _capi.PackedSeqs()
+        self.cref = C.byref(self.c)
         with torch.cuda.device(self.table.device):
             check(l.capdec_packed_plan(cq, ck, n, int(self.causal), ptr(self.table), self.table.numel(), C.byref(self.c)),
                   "capdec_packed_plan")
 
 
-def _on_current(name, *tensors):
-    """Every tensor on the current device: its stream is the one the kernels are launched on."""
-    cur = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != cur:
-            raise _capi.CapdecError(f"{name}: a tensor is on {t.device}, the current device is cuda:{cur}")
+def _here(name, t):
+    """Index of the current device: the tensors of a call lie there, its stream is the one the kernels are launched on."""
+    if not t.is_cuda:
+        raise _capi.CapdecError(f"{name}: tensor is on {t.device}; the capdec ops run on the GPU only (no CPU fallback)")
+    return torch.cuda.current_device() if _capi._cur_device is None else _capi._cur_device()
 
 
-def _packed_mat(t, name, dtype, rows, width):
-    _req(t, name, dtype)
-    piece = 16 // t.element_size()
-    if t.dim() != 2 or t.shape[1] != width or t.shape[0] < rows or (t.shape[0] > 0 and (
-            t.stride(1) != 1 or t.stride(0) < width or t.stride(0) % piece or t.data_ptr() % 16)):
-        raise _capi.CapdecError(f"{name}: need a 16-byte aligned [>= {rows}, {width}] matrix with unit column stride and a row "
-                                f"stride that is a multiple of {piece}, got {tuple(t.shape)} / {t.stride()}")
-    return t
+def _elsewhere(name, t, cur):
+    if not t.is_cuda:
+        raise _capi.CapdecError(f"{name}: tensor is on {t.device}; the capdec ops run on the GPU only (no CPU fallback)")
+    if t.device.index != cur:
+        raise _capi.CapdecError(f"{name}: tensor is on {t.device}, the current device is cuda:{cur}")
+
+
+_ES = {torch.float32: 4, torch.bfloat16: 2}
+
+
+def _rows(t, name, dtype, rows, width, cur):
+    """(pointer, row stride) of a [>= rows, width] matrix of ``dtype`` on device ``cur``, rows in whole 16-byte pieces."""
+    shape, strides, at = t.shape, t.stride(), t.data_ptr()
+    if t.dtype is dtype and len(shape) == 2 and shape[1] == width and shape[0] >= rows and t.get_device() == cur and (
+            shape[0] == 0 or (strides[1] == 1 and width <= strides[0] and not strides[0] * _ES[dtype] % 16 and not at % 16)):
+        return at, (strides[0] if shape[0] else width)
+    _elsewhere(name, t, cur)
+    raise _capi.CapdecError(f"{name}: need a 16-byte aligned {dtype} [>= {rows}, {width}] matrix with unit column stride and a row "
+                            f"stride in whole 16 bytes, got {t.dtype} {tuple(shape)} / {strides}")
+
+
+def _vector(t, name, dtype, n, cur):
+    """Pointer of a dense vector of n entries on device ``cur``."""
+    if t.dtype is dtype and t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1) and t.get_device() == cur:
+        return t.data_ptr()
+    _elsewhere(name, t, cur)
+    raise _capi.CapdecError(f"{name}: need a dense {dtype} vector of {n}, got {t.dtype} {tuple(t.shape)} / {t.stride()}")
 
 
 def _packed_args(name, q, k, v, Hq, Hkv, seqs, scale):
-    if q.dtype not in (torch.float32, torch.bfloat16):
+    if q.dtype not in _ES:
         raise _capi.CapdecError(f"{name}: q is {q.dtype}: fp32 or bf16 matrices")
-    if Hkv <= 0 or Hq <= 0 or Hq % Hkv or q.dim() != 2 or q.shape[1] % Hq or q.shape[1] // Hq not in (64, 128):
+    if Hkv <= 0 or Hq <= 0 or Hq % Hkv or q.dim() != 2 or q.shape[1] not in (64 * Hq, 128 * Hq):
         raise _capi.CapdecError(f"{name}: {tuple(q.shape)} with Hq={Hq}, Hkv={Hkv}: Hq a multiple of Hkv, heads of 64 or 128")
-    dh = q.shape[1] // Hq
-    _packed_mat(q, name + ".q", q.dtype, seqs.rows_q, Hq * dh)
-    _packed_mat(k, name + ".k", q.dtype, seqs.rows_k, Hkv * dh), _packed_mat(v, name + ".v", q.dtype, seqs.rows_k, Hkv * dh)
-    _on_current(name, q, k, v, seqs.table)
+    dh, cur, dt = q.shape[1] // Hq, _here(name, q), q.dtype
+    if seqs.table.get_device() != cur:
+        _elsewhere(name + ".seqs", seqs.table, cur)
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise _capi.CapdecError(f"{name}: scale {scale} must be positive and finite")
-    return dh, F32 if q.dtype == torch.float32 else _capi.BF16S, scale
+    return (dh, cur, F32 if dt is torch.float32 else _capi.BF16S, scale, _rows(q, name + ".q", dt, seqs.rows_q, Hq * dh, cur),
+            _rows(k, name + ".k", dt, seqs.rows_k, Hkv * dh, cur), _rows(v, name + ".v", dt, seqs.rows_k, Hkv * dh, cur))
 
 
 def attn_packed_fwd(q, k, v, Hq, Hkv, seqs, out=None, save_lse=True, scale=None):
     """Attention over packed sequences: q [>= rows_q, Hq * dh], k / v [>= rows_k, Hkv * dh] (row-strided views, all fp32 or
     all bf16, dh 64 or 128), ``seqs`` a PackedSeqs.  Returns (o, lse [Hq, rows of q] or None).  Rows behind the last sequence
     stay as they are in a given ``out`` and are zeros in a new one."""
-    dh, dtype, scale = _packed_args("attn_packed_fwd", q, k, v, Hq, Hkv, seqs, scale)
+    dh, cur, dtype, scale, (pq, lq), (pk, lk), (pv, lv) = _packed_args("attn_packed_fwd", q, k, v, Hq, Hkv, seqs, scale)
+    rows, n = q.shape[0], seqs.rows_q
     if out is None:
-        out = torch.empty((q.shape[0], Hq * dh), dtype=q.dtype, device=q.device)
-        if q.shape[0] > seqs.rows_q:
-            out[seqs.rows_q:].zero_()
-    else:
-        _packed_mat(out, "attn_packed_fwd.out", q.dtype, seqs.rows_q, Hq * dh)
-        _on_current("attn_packed_fwd", out)
-    lse = torch.empty((Hq, q.shape[0]), dtype=torch.float32, device=q.device) if save_lse else None
-    if save_lse and q.shape[0] > seqs.rows_q:
-        lse[:, seqs.rows_q:].zero_()
-    check(lib().capdec_attn_packed_fwd(C.byref(seqs.c), ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0), ptr(out),
-                                       out.stride(0), ptr(lse), q.shape[0], Hq, Hkv, dh, dtype, scale, stream()),
-          "capdec_attn_packed_fwd")
+        out = q.new_empty((rows, Hq * dh))
+        if rows > n:
+            out[n:].zero_()
+    po, lo = _rows(out, "attn_packed_fwd.out", q.dtype, n, Hq * dh, cur)
+    lse = None
+    if save_lse:
+        lse = q.new_empty((Hq, rows), dtype=torch.float32)
+        if rows > n:
+            lse[:, n:].zero_()
+    check(lib().capdec_attn_packed_fwd(seqs.cref, pq, lq, pk, lk, pv, lv, po, lo, None if lse is None else lse.data_ptr(), rows, Hq, Hkv,
+                                       dh, dtype, scale, stream()), "capdec_attn_packed_fwd")
     return out, lse
 
 
@@ -1012,28 +1031,33 @@ def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=Non
     """(dq, dk, dv) of attn_packed_fwd; ``o`` / ``lse`` are its results, ``do`` the gradient of o.  Given dq / dk / dv are
     written in place, rows behind the last sequence stay as they are there and are zeros in new ones."""
     name = "attn_packed_bwd"
-    dh, dtype, scale = _packed_args(name, q, k, v, Hq, Hkv, seqs, scale)
-    _packed_mat(o, name + ".o", q.dtype, seqs.rows_q, Hq * dh), _packed_mat(do, name + ".do", q.dtype, seqs.rows_q, Hq * dh)
-    _req(lse, name + ".lse")
-    if lse.dim() != 2 or lse.shape[0] != Hq or lse.shape[1] < seqs.rows_q or not lse.is_contiguous():
+    dh, cur, dtype, scale, (pq, lq), (pk, lk), (pv, lv) = _packed_args(name, q, k, v, Hq, Hkv, seqs, scale)
+    dt, n, nk, wide, narrow = q.dtype, seqs.rows_q, seqs.rows_k, Hq * dh, Hkv * dh
+    po, lo = _rows(o, name + ".o", dt, n, wide, cur)
+    pdo, ldo = _rows(do, name + ".do", dt, n, wide, cur)
+    if lse.dtype is not torch.float32 or lse.dim() != 2 or lse.shape[0] != Hq or lse.shape[1] < n or not lse.is_contiguous() \
+            or lse.get_device() != cur:
+        _elsewhere(name + ".lse", lse, cur)
         raise _capi.CapdecError(f"{name}: lse {tuple(lse.shape)} must be the contiguous [Hq, rows] block that attn_packed_fwd returned")
-    out = []
-    for t, n, like, rows, width in ((dq, ".dq", q, seqs.rows_q, Hq * dh), (dk, ".dk", k, seqs.rows_k, Hkv * dh),
-                                    (dv, ".dv", v, seqs.rows_k, Hkv * dh)):
-        if t is None:
-            t = torch.empty((like.shape[0], width), dtype=q.dtype, device=q.device)
-            if like.shape[0] > rows:
-                t[rows:].zero_()
-        else:
-            _packed_mat(t, name + n, q.dtype, rows, width)
-        out.append(t)
-    _on_current(name, o, do, lse, *out)
+    if dq is None:
+        dq = q.new_empty((q.shape[0], wide))
+        if q.shape[0] > n:
+            dq[n:].zero_()
+    if dk is None:
+        dk = k.new_empty((k.shape[0], narrow))
+        if k.shape[0] > nk:
+            dk[nk:].zero_()
+    if dv is None:
+        dv = v.new_empty((v.shape[0], narrow))
+        if v.shape[0] > nk:
+            dv[nk:].zero_()
+    pdq, ldq = _rows(dq, name + ".dq", dt, n, wide, cur)
+    pdk, ldk = _rows(dk, name + ".dk", dt, nk, narrow, cur)
+    pdv, ldv = _rows(dv, name + ".dv", dt, nk, narrow, cur)
     # scratch: rowsum(do * o), with bf16 matrices 16 bytes for each (head, row)
-    delta = torch.empty(lse.numel() * (1 if q.dtype == torch.float32 else 4), dtype=torch.float32, device=q.device)
-    dq, dk, dv = out
-    check(lib().capdec_attn_packed_bwd(C.byref(seqs.c), ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0), ptr(o),
-                                       o.stride(0), ptr(do), do.stride(0), ptr(lse), ptr(delta), lse.shape[1], ptr(dq), dq.stride(0),
-                                       ptr(dk), dk.stride(0), ptr(dv), dv.stride(0), Hq, Hkv, dh, dtype, scale, stream()),
+    delta = lse.new_empty(lse.numel() * (1 if dtype == F32 else 4))
+    check(lib().capdec_attn_packed_bwd(seqs.cref, pq, lq, pk, lk, pv, lv, po, lo, pdo, ldo, lse.data_ptr(), delta.data_ptr(),
+                                       lse.shape[1], pdq, ldq, pdk, ldk, pdv, ldv, Hq, Hkv, dh, dtype, scale, stream()),
           "capdec_attn_packed_bwd")
     return dq, dk, dv
 
@@ -1063,6 +1087,7 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page, self.dh = pages, heads, page, dh
         self.c = _capi.KVCache(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, heads, page, dh, _capi.E4M3 if e4m3 else _capi.BF16S)
+        self.cref = C.byref(self.c)
 
     @classmethod
     def new(cls, pages, heads, page, dh, dtype=torch.bfloat16, device="cuda"):
@@ -1084,42 +1109,33 @@ def _on_one(name, *tensors):
         raise _capi.CapdecError(f"{name}: tensors on different devices ({', '.join(sorted(map(str, devices)))})")
 
 
-def _ints(t, name, n):
-    """A dense int32 vector of n entries."""
-    _req(t, name, torch.int32)
-    if t.dim() != 1 or t.numel() != n or (n > 1 and t.stride(0) != 1):
-        raise _capi.CapdecError(f"{name}: need a dense int32 vector of {n}, got {tuple(t.shape)} / {t.stride()}")
-    return t
-
-
 def _cache_rows(name, cache, k, v, slots):
-    if k.dtype not in (torch.float32, torch.bfloat16):
+    if k.dtype not in _ES:
         raise _capi.CapdecError(f"{name}: rows are {k.dtype}: fp32 or bf16")
-    rows, width = slots.numel(), cache.heads * cache.dh
-    _ints(slots, name + ".slots", rows)
-    _packed_mat(k, name + ".k", k.dtype, rows, width), _packed_mat(v, name + ".v", k.dtype, rows, width)
-    _on_current(name, k, v, slots, cache.k)
-    return rows, F32 if k.dtype == torch.float32 else _capi.BF16S
+    rows, width, cur, dt = slots.numel(), cache.heads * cache.dh, _here(name, k), k.dtype
+    if cache.k.get_device() != cur:
+        _elsewhere(name + ".cache", cache.k, cur)
+    pk, lk = _rows(k, name + ".k", dt, rows, width, cur)
+    pv, lv = _rows(v, name + ".v", dt, rows, width, cur)
+    return rows, F32 if dt is torch.float32 else _capi.BF16S, pk, lk, pv, lv, _vector(slots, name + ".slots", torch.int32, rows, cur)
 
 
 def kv_cache_write(cache, k, v, slots):
     """Row r of k / v ([>= rows, heads * dh], fp32 or bf16, row-strided views) into slot ``slots[r]`` (int32 [rows]; negative:
     skipped) of a PagedKVCache, rounded to e4m3 with a scale of its own for each head where the cache holds e4m3.  The slots of
     one call must differ."""
-    rows, dtype = _cache_rows("kv_cache_write", cache, k, v, slots)
-    check(lib().capdec_kv_write(C.byref(cache.c), ptr(k), k.stride(0), ptr(v), v.stride(0), dtype, ptr(slots), rows, stream()),
-          "capdec_kv_write")
+    rows, dtype, pk, lk, pv, lv, ps = _cache_rows("kv_cache_write", cache, k, v, slots)
+    check(lib().capdec_kv_write(cache.cref, pk, lk, pv, lv, dtype, ps, rows, stream()), "capdec_kv_write")
 
 
 def kv_cache_read(cache, slots, k=None, v=None, dtype=torch.bfloat16):
     """(k, v): the rows of ``slots`` (int32 [rows]; negative: zeros) as [rows, heads * dh] matrices of ``dtype`` (or into given
     ones)."""
-    new = lambda: torch.empty((slots.numel(), cache.heads * cache.dh), dtype=dtype, device=cache.k.device)
-    k = new() if k is None else k
-    v = new() if v is None else v
-    rows, dt = _cache_rows("kv_cache_read", cache, k, v, slots)
-    check(lib().capdec_kv_read(C.byref(cache.c), ptr(slots), rows, ptr(k), k.stride(0), ptr(v), v.stride(0), dt, stream()),
-          "capdec_kv_read")
+    shape = (slots.numel(), cache.heads * cache.dh)
+    k = torch.empty(shape, dtype=dtype, device=cache.k.device) if k is None else k
+    v = torch.empty(shape, dtype=dtype, device=cache.k.device) if v is None else v
+    rows, dt, pk, lk, pv, lv, ps = _cache_rows("kv_cache_read", cache, k, v, slots)
+    check(lib().capdec_kv_read(cache.cref, ps, rows, pk, lk, pv, lv, dt, stream()), "capdec_kv_read")
     return k, v
 
 
@@ -1139,34 +1155,33 @@ def attn_paged(q, cache, page_table, kv_lens, Hq, cu_q=None, max_q=1, out=None, 
     [n, columns].  Causal: new token i of nq sees the positions up to kv_lens - nq + i.  Returns o (rows of no sequence stay as
     they are in a given ``out`` and are zeros in a new one), or (o, lse [Hq, rows])."""
     name = "attn_paged"
-    n = kv_lens.numel()
-    _packed_mat(q, name + ".q", torch.bfloat16, 0 if cu_q is not None else n, Hq * cache.dh)
-    _ints(kv_lens, name + ".kv_lens", n)
-    if cu_q is not None:
-        _ints(cu_q, name + ".cu_q", n + 1)
-    _req(page_table, name + ".page_table", torch.int32)
-    if page_table.dim() != 2 or page_table.shape[0] != n or page_table.shape[1] == 0 or page_table.stride(1) != 1 \
-            or (n > 1 and page_table.stride(0) < page_table.shape[1]) or n == 0:
-        raise _capi.CapdecError(f"{name}: page_table {tuple(page_table.shape)} / {page_table.stride()} must be int32 [{n}, columns] "
-                                "with unit column stride")
-    if Hq <= 0 or Hq % cache.heads or max_q <= 0:
-        raise _capi.CapdecError(f"{name}: Hq={Hq} must be a multiple of the cache's {cache.heads} heads, max_q={max_q} positive")
-    scale = 1.0 / math.sqrt(cache.dh) if scale is None else float(scale)
-    rows, cols = q.shape[0], page_table.shape[1]
+    n, cur, dh, heads = kv_lens.numel(), _here(name, q), cache.dh, cache.heads
+    if Hq <= 0 or Hq % heads or max_q <= 0:
+        raise _capi.CapdecError(f"{name}: Hq={Hq} must be a multiple of the cache's {heads} heads, max_q={max_q} positive")
+    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
+    if cache.k.get_device() != cur:
+        _elsewhere(name + ".cache", cache.k, cur)
+    pq, lq = _rows(q, name + ".q", torch.bfloat16, 0 if cu_q is not None else n, Hq * dh, cur)
+    pl = _vector(kv_lens, name + ".kv_lens", torch.int32, n, cur)
+    pc = None if cu_q is None else _vector(cu_q, name + ".cu_q", torch.int32, n + 1, cur)
+    shape, strides = page_table.shape, page_table.stride()
+    if page_table.dtype is not torch.int32 or len(shape) != 2 or shape[0] != n or shape[1] == 0 or strides[1] != 1 or n == 0 \
+            or (n > 1 and strides[0] < shape[1]) or page_table.get_device() != cur:
+        _elsewhere(name + ".page_table", page_table, cur)
+        raise _capi.CapdecError(f"{name}: page_table {page_table.dtype} {tuple(shape)} / {strides} must be int32 [{n}, columns] with unit "
+                                "column stride")
+    rows, cols = q.shape[0], shape[1]
     if out is None:
         # (which rows belong to no sequence is known on the device only)
-        out = (torch.empty if cu_q is None and rows == n else torch.zeros)((rows, Hq * cache.dh), dtype=q.dtype, device=q.device)
-    else:
-        _packed_mat(out, name + ".out", torch.bfloat16, rows, Hq * cache.dh)
-    _on_current(name, q, out, kv_lens, cu_q, page_table, cache.k)
+        out = q.new_empty((rows, Hq * dh)) if cu_q is None and rows == n else q.new_zeros((rows, Hq * dh))
+    po, lo = _rows(out, name + ".out", torch.bfloat16, rows, Hq * dh, cur)
     lse = torch.zeros((Hq, rows), dtype=torch.float32, device=q.device) if return_lse else None
     l = lib()
-    need = l.capdec_attn_paged_workspace_bytes(C.byref(cache.c), n, rows, int(max_q), Hq, cols)
+    need = l.capdec_attn_paged_workspace_bytes(cache.cref, n, rows, int(max_q), Hq, cols)
     # a block of its own for every call: the allocator keeps it from calls on other streams and from other captured graphs
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    check(l.capdec_attn_paged(C.byref(cache.c), ptr(q), q.stride(0), ptr(cu_q), ptr(kv_lens), ptr(page_table),
-                              page_table.stride(0) if n > 1 else cols, cols, n, rows, int(max_q), Hq, scale, ptr(out), out.stride(0),
-                              ptr(lse), ptr(ws), need, stream()), "capdec_attn_paged")
+    check(l.capdec_attn_paged(cache.cref, pq, lq, pc, pl, page_table.data_ptr(), strides[0] if n > 1 else cols, cols, n, rows,
+                              int(max_q), Hq, scale, po, lo, ptr(lse), ptr(ws), need, stream()), "capdec_attn_paged")
     return (out, lse) if return_lse else out
 
 
@@ -1175,39 +1190,43 @@ def draft_verify(target, draft, tokens, u_accept, u_sample, num_draft=None, pad=
     (None: a drafter sure of its tokens), fp32 probabilities with unit stride along the vocabulary; tokens int64 [n, drafts];
     u_accept [n, drafts] / u_sample [n] uniforms in [0, 1); num_draft int32 [n] (None: all).  Returns (out int64
     [n, drafts + 1]: accepted tokens, the drawn one, then ``pad``; accepted int32 [n])."""
-    name = "draft_verify"
-    _req(target, name + ".target")
-    if target.dim() != 3 or target.shape[1] == 0 or target.shape[2] == 0 or (target.numel() and target.stride(2) != 1):
-        raise _capi.CapdecError(f"{name}: target {tuple(target.shape)} / {target.stride()} must be [n, drafts + 1, V] with unit stride "
-                                "along the vocabulary")
+    name, f32 = "draft_verify", torch.float32
+    cur = _here(name, target)
+    if target.dim() != 3 or target.shape[1] == 0 or target.shape[2] == 0:
+        raise _capi.CapdecError(f"{name}: target {tuple(target.shape)} must be [n, drafts + 1, V]")
     n, d, V = target.shape[0], target.shape[1] - 1, target.shape[2]
     if d > 64:
         raise _capi.CapdecError(f"{name}: {d} drafted tokens; at most 64")
-    if draft is not None:
-        _req(draft, name + ".draft")
-        if tuple(draft.shape) != (n, d, V) or (draft.numel() and draft.stride(2) != 1):
-            raise _capi.CapdecError(f"{name}: draft {tuple(draft.shape)} / {draft.stride()} must be {(n, d, V)} with unit stride along "
-                                    "the vocabulary")
-    for t, what, dt in ((tokens, ".tokens", torch.int64), (u_accept, ".u_accept", torch.float32)):
-        _req(t, name + what, dt)
-        if tuple(t.shape) != (n, d) or (d > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < d):
-            raise _capi.CapdecError(f"{name}{what}: need {(n, d)} with unit column stride, got {tuple(t.shape)} / {t.stride()}")
-    _req(u_sample, name + ".u_sample")
-    if tuple(u_sample.shape) != (n,) or (n > 1 and u_sample.stride(0) != 1):
-        raise _capi.CapdecError(f"{name}.u_sample: need a dense vector of {n}, got {tuple(u_sample.shape)}")
-    if num_draft is not None:
-        _ints(num_draft, name + ".num_draft", n)
-    for t, rows in ((target, d + 1), (draft, d)):
-        if t is not None and t.numel() and ((rows > 1 and t.stride(1) < V) or (n > 1 and t.stride(0) < 0)):
-            raise _capi.CapdecError(f"{name}: rows of probabilities overlap: strides {t.stride()}")
-    _on_current(name, target, draft, tokens, u_accept, u_sample, num_draft)
-    out = torch.empty((n, d + 1), dtype=torch.int64, device=target.device)
-    accepted = torch.empty(n, dtype=torch.int32, device=target.device)
-    step = lambda t, rows: max(t.stride(1), V) if rows > 1 else V
-    check(lib().capdec_draft_verify(ptr(target), target.stride(0), step(target, d + 1), ptr(draft), draft.stride(0) if draft is not None else 0,
-                                    step(draft, d) if draft is not None else 0, ptr(tokens), max(tokens.stride(0), d), ptr(num_draft),
-                                    ptr(u_accept), max(u_accept.stride(0), d), ptr(u_sample), n, d, V, int(pad), ptr(out), ptr(accepted),
-                                    stream()), "capdec_draft_verify")
+
+    def block(t, what, rows):
+        """(pointer, sequence stride, row stride) of [n, rows, V] probabilities."""
+        strides = t.stride()
+        if t.dtype is not f32 or tuple(t.shape) != (n, rows, V) or t.get_device() != cur or (n and rows and (
+                strides[2] != 1 and V > 1 or rows > 1 and strides[1] < V or strides[0] < 0)):
+            _elsewhere(name + what, t, cur)
+            raise _capi.CapdecError(f"{name}{what}: need fp32 {(n, rows, V)} with unit stride along the vocabulary and rows that do not "
+                                    f"overlap, got {t.dtype} {tuple(t.shape)} / {strides}")
+        return t.data_ptr(), strides[0], strides[1] if rows > 1 else V
+
+    def small(t, what, dtype):
+        """(pointer, row stride) of an [n, d] matrix."""
+        strides = t.stride()
+        if t.dtype is not dtype or tuple(t.shape) != (n, d) or t.get_device() != cur or (
+                n and d and (d > 1 and strides[1] != 1 or n > 1 and strides[0] < d)):
+            _elsewhere(name + what, t, cur)
+            raise _capi.CapdecError(f"{name}{what}: need {dtype} {(n, d)} with unit column stride, got {t.dtype} {tuple(t.shape)} / {strides}")
+        return t.data_ptr(), max(strides[0], d)
+
+    pt, ts, tr = block(target, ".target", d + 1)
+    pd, ds, dr = (None, 0, 0) if draft is None else block(draft, ".draft", d)
+    pk, lk = small(tokens, ".tokens", torch.int64)
+    pu, lu = small(u_accept, ".u_accept", f32)
+    us = _vector(u_sample, name + ".u_sample", f32, n, cur)
+    nd = None if num_draft is None else _vector(num_draft, name + ".num_draft", torch.int32, n, cur)
+    out = tokens.new_empty((n, d + 1))
+    accepted = tokens.new_empty(n, dtype=torch.int32)
+    check(lib().capdec_draft_verify(pt, ts, tr, pd, ds, dr, pk, lk, nd, pu, lu, us, n, d, V, int(pad), out.data_ptr(),
+                                    accepted.data_ptr(), stream()), "capdec_draft_verify")
     return out, accepted
 
 

@@ -317,6 +317,38 @@ __global__ __launch_bounds__(256, 2) void packed16_fwd_kernel(PackedParams p) {
     }
 }
 
+// rowsum(do * o) of this lane's row, whose do fragments stay in df
+template <typename T, int DH>
+__device__ __forceinline__ float row_delta(const PackedParams& p, typename AttTile<T, DH>::frag* df, size_t grow, int head, bool mine, int half) {
+    using L = AttTile<T, DH>;
+    typename L::frag of[L::NF];
+    L::load_row(of, (const T*)p.o + grow * p.ldo + head * DH, mine, half);
+    L::load_row(df, (const T*)p.dout + grow * p.lddo + head * DH, mine, half);
+    const float d = L::dot(df, of);
+    return d + __shfl_xor(d, 32, 64);
+}
+
+// lse times log2 e of this lane's row: p = exp2(s c - lse2); a row that sees nothing has lse = -inf, its weights are zeros.
+// Leaves the row's statistics for the dk / dv kernel (write: this lane does).
+template <typename T>
+__device__ __forceinline__ float row_stats(const PackedParams& p, float dsum, size_t grow, int head, bool mine, bool write) {
+    const size_t at = (size_t)head * p.stat_rows + grow;
+    float lse2 = mine ? p.lse[at] * LOG2E : INFINITY;
+    if (lse2 == -INFINITY) lse2 = INFINITY;
+    if (mine && write) {
+        if (sizeof(T) == 2 && p.stats) {
+            // -lse / scale and -delta, three bf16 terms each; a row that sees nothing gets weights of zero
+            const float l = lse2 == INFINITY ? -1e30f : -lse2 / (p.scale * LOG2E), d = -dsum;
+            const __bf16 l0 = (__bf16)l, l1 = (__bf16)(l - (float)l0), l2 = (__bf16)(l - (float)l0 - (float)l1);
+            const __bf16 d0 = (__bf16)d, d1 = (__bf16)(d - (float)d0), d2 = (__bf16)(d - (float)d0 - (float)d1);
+            reinterpret_cast<bf16x8t*>(p.stats)[at] = bf16x8t{l0, l1, l2, (__bf16)0.f, d0, d1, d2, (__bf16)0.f};
+        } else {
+            p.delta[at] = dsum;
+        }
+    }
+    return lse2;
+}
+
 // dq and delta = rowsum(do * o); blocks and waves as in the forward
 template <typename T, int DH, int RB, int KS, int KB>
 __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH == 64) ? 2 : 1) void packed_bwd_dq_kernel(PackedParams p) {
@@ -342,30 +374,9 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
     const size_t grow = (size_t)(w.q0 + row);
 
     typename L::frag qf[L::NF], df[L::NF];
-    float dsum;
-    {
-        typename L::frag of[L::NF];
-        L::load_row(of, (const T*)p.o + grow * p.ldo + head * DH, mine, half);
-        L::load_row(df, (const T*)p.dout + grow * p.lddo + head * DH, mine, half);
-        dsum = L::dot(df, of);
-        dsum += __shfl_xor(dsum, 32, 64);
-    }
+    const float dsum = row_delta<T, DH>(p, df, grow, head, mine, half);
     L::load_row(qf, (const T*)p.q + grow * p.ldq + head * DH, mine, half);
-    // p = exp2(s c - lse2); a row that sees nothing has lse = -inf: its weights are zeros
-    float lse2 = mine ? p.lse[(size_t)head * p.stat_rows + grow] * LOG2E : INFINITY;
-    if (lse2 == -INFINITY) lse2 = INFINITY;
-    if (mine && half == 0 && ksp == 0) {
-        const size_t at = (size_t)head * p.stat_rows + grow;
-        if (sizeof(T) == 2 && p.stats) {
-            // -lse / scale and -delta, three bf16 terms each; a row that sees nothing gets weights of zero
-            const float l = lse2 == INFINITY ? -1e30f : -lse2 / (p.scale * LOG2E), d = -dsum;
-            const __bf16 l0 = (__bf16)l, l1 = (__bf16)(l - (float)l0), l2 = (__bf16)(l - (float)l0 - (float)l1);
-            const __bf16 d0 = (__bf16)d, d1 = (__bf16)(d - (float)d0), d2 = (__bf16)(d - (float)d0 - (float)d1);
-            reinterpret_cast<bf16x8t*>(p.stats)[at] = bf16x8t{l0, l1, l2, (__bf16)0.f, d0, d1, d2, (__bf16)0.f};
-        } else {
-            p.delta[at] = dsum;
-        }
-    }
+    const float lse2 = row_stats<T>(p, dsum, grow, head, mine, half == 0 && ksp == 0);
     Staged<T, DH, NT, BN> ks, vs;
     if (nt > 0) {
         ks.load(kg, p.ldk, 0, w.nk, tid);
@@ -428,6 +439,79 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
         for (int o = 0; o < KS - 1; ++o) add_sums<L::NDT>(smem + (rb * (KS - 1) + o) * BOX, acc, lane, 1.f, 1.f);
     }
     if (mine) L::store_row((T*)p.dq + grow * p.lddq + head * DH, acc, p.scale, half);
+}
+
+// dq of bf16 matrices with 128 rows a workgroup, fed as the forward is
+template <int DH>
+__global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p) {
+    using L = DmaTile<DH>;
+    constexpr int KB = 2, BN = 32 * KB, IMG = BN * L::ROWB;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
+    int head, it;
+    packed_place(p.Hq, head, it);
+    const PackedItem w = p.items[it];
+    const int hk = head / p.group;
+    const __bf16* kg = (const __bf16*)p.k + (size_t)w.k0 * p.ldk + hk * DH;
+    const __bf16* vg = (const __bf16*)p.v + (size_t)w.k0 * p.ldv + hk * DH;
+    const int r0 = w.t0 + wave * 32;
+    const int row = r0 + l31, off = w.nk - w.nq;
+    const int kmax = p.causal ? min(w.nk, min(w.t0 + 128, w.nq) + off) : w.nk;
+    const int nt = kmax > 0 ? (kmax + BN - 1) / BN : 0;
+    const int wave_end = r0 >= w.nq ? 0 : (p.causal ? min(w.nk, min(r0 + 32, w.nq) + off) : w.nk);
+    const int all_see = p.causal ? min(w.nk, r0 + 1 + off) : w.nk;
+    const bool mine = row < w.nq;
+    const size_t grow = (size_t)(w.q0 + row);
+    if (nt > 0) {
+        L::template fetch<BN, 4>(smem, kg, p.ldk, 0, w.nk, wave, lane);
+        L::template fetch<BN, 4>(smem + IMG, vg, p.ldv, 0, w.nk, wave, lane);
+    }
+    typename L::frag qf[L::NF], df[L::NF];
+    const float dsum = row_delta<__bf16, DH>(p, df, grow, head, mine, half);
+    L::load_row(qf, (const __bf16*)p.q + grow * p.ldq + head * DH, mine, half);
+    const float lse2 = row_stats<__bf16>(p, dsum, grow, head, mine, half == 0);
+    landed(qf);
+    typename L::lanes ln = L::make_lanes(lane);
+    const float c = p.scale * LOG2E;
+    f32x16 acc[L::NDT];
+#pragma unroll
+    for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
+    auto turn = [&](int t, unsigned char* cur, unsigned char* nx) __attribute__((always_inline)) {
+        const unsigned char* Ks = cur;
+        const unsigned char* Vs = Ks + IMG;
+        dma_sync();
+        if (t + 1 < nt) {
+            L::template fetch<BN, 4>(nx, kg, p.ldk, (t + 1) * BN, w.nk, wave, lane);
+            L::template fetch<BN, 4>(nx + IMG, vg, p.ldv, (t + 1) * BN, w.nk, wave, lane);
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int k0 = t * BN + 32 * b;
+            if (k0 < wave_end) {
+                f32x16 s, dp;
+                zero16(s);
+                zero16(dp);
+                L::mma_rows(s, Ks + b * 32 * L::ROWB, ln, qf);   // S^T[key][query]
+                L::mma_rows(dp, Vs + b * 32 * L::ROWB, ln, df);  // dP^T[key][query]
+                if (k0 + 32 > all_see) {
+                    const int see = p.causal ? min(w.nk, row + 1 + off) : w.nk;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = k0 + row_of(r, half) < see ? s[r] : -INFINITY;
+                }
+                float x[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = exp2_fast(__fmaf_rn(s[r], c, -lse2)) * (dp[r] - dsum);
+                typename L::weights dw;
+                L::pack(dw, x);
+                L::mma_cols(acc, Ks + b * 32 * L::ROWB, ln, dw);  // dQ^T[dim][query] += K^T dS^T
+            }
+        }
+    };
+    for (int t = 0; t < nt; t += 2) {
+        turn(t, smem, smem + 2 * IMG);
+        if (t + 1 < nt) turn(t + 1, smem + 2 * IMG, smem);
+    }
+    if (mine) L::store_row((__bf16*)p.dq + grow * p.lddq + head * DH, acc, p.scale, half);
 }
 
 // dk, dv: KB blocks of 32 key rows of one key / value head, every block walked by QS waves that take every QS-th query tile
@@ -803,7 +887,7 @@ static void launch_bwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t
     if (s->tiles[0] > 0) {
         if (short_rows(s->tiles)) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
         else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
-        else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 4, 1, 2>), 0, p.Hq, 256);
+        else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed16_bwd_dq_kernel<DH>), 0, p.Hq, 256);
     }
     if (s->tiles[3] > 0) {
         if (one) CAPDEC_PACKED((packed_bwd_dkv_kernel<T, DH, 1, 1>), 5, p.Hkv, 64);

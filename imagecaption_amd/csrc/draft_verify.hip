@@ -48,15 +48,16 @@ __global__ __launch_bounds__(VWAVES * 64) void draft_verify_kernel(VerifyParams 
     const int b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t* tok = p.tokens + (size_t)b * p.ldt;
     if (wave == 0) {
+        // (the loads do not wait for one another: the count, then every lane its token and uniform, then the probabilities)
+        const int mine = min(lane, p.drafts - 1);
+        const int64_t x = p.drafts ? tok[mine] : -1;
+        const float u = p.drafts ? p.u_accept[(size_t)b * p.ldu + mine] : 1.f;
         const int num = p.num_draft ? min(max(p.num_draft[b], 0), p.drafts) : p.drafts;
         bool take = false;
-        if (lane < num) {
-            const int64_t x = tok[lane];
-            if (x >= 0 && x < p.V) {
-                const double pt = p.target[(size_t)b * p.target_seq + (size_t)lane * p.target_row + x];
-                const double q = p.draft ? (double)p.draft[(size_t)b * p.draft_seq + (size_t)lane * p.draft_row + x] : 1.0;
-                take = (double)p.u_accept[(size_t)b * p.ldu + lane] * q < pt;  // exact: two 24-bit factors
-            }
+        if (x >= 0 && x < p.V) {
+            const double pt = p.target[(size_t)b * p.target_seq + (size_t)mine * p.target_row + x];
+            const double q = p.draft ? (double)p.draft[(size_t)b * p.draft_seq + (size_t)mine * p.draft_row + x] : 1.0;
+            take = lane < num && (double)u * q < pt;  // exact: two 24-bit factors
         }
         const unsigned long long ok = __ballot(take);
         if (lane == 0) {

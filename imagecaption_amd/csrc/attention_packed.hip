@@ -228,8 +228,8 @@ __global__ __launch_bounds__(256, 2) void packed16_fwd_kernel(PackedParams p) {
     L::load_row(qf, (const __bf16*)p.q + (size_t)(w.q0 + row) * p.ldq + head * DH, row < w.nq, half);
     landed(qf);
     typename L::template Fetch<BN, 4> fk, fv;
-    fk.init(p.ldk, wave, lane);
-    fv.init(p.ldv, wave, lane);
+    fk.init(p.ldk, lane);
+    fv.init(p.ldv, lane);
     if (nt > 0) {
         fk(smem, kg, p.ldk, 0, w.nk, wave, lane);
         fv(smem + IMG, vg, p.ldv, 0, w.nk, wave, lane);
@@ -462,9 +462,12 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
     const int all_see = p.causal ? min(w.nk, r0 + 1 + off) : w.nk;
     const bool mine = row < w.nq;
     const size_t grow = (size_t)(w.q0 + row);
+    typename L::template Fetch<BN, 4> fk, fv;
+    fk.init(p.ldk, lane);
+    fv.init(p.ldv, lane);
     if (nt > 0) {
-        L::template fetch<BN, 4>(smem, kg, p.ldk, 0, w.nk, wave, lane);
-        L::template fetch<BN, 4>(smem + IMG, vg, p.ldv, 0, w.nk, wave, lane);
+        fk(smem, kg, p.ldk, 0, w.nk, wave, lane);
+        fv(smem + IMG, vg, p.ldv, 0, w.nk, wave, lane);
     }
     typename L::frag qf[L::NF], df[L::NF];
     const float dsum = row_delta<__bf16, DH>(p, df, grow, head, mine, half);
@@ -481,8 +484,8 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
         const unsigned char* Vs = Ks + IMG;
         dma_sync();
         if (t + 1 < nt) {
-            L::template fetch<BN, 4>(nx, kg, p.ldk, (t + 1) * BN, w.nk, wave, lane);
-            L::template fetch<BN, 4>(nx + IMG, vg, p.ldv, (t + 1) * BN, w.nk, wave, lane);
+            fk(nx, kg, p.ldk, (t + 1) * BN, w.nk, wave, lane);
+            fv(nx + IMG, vg, p.ldv, (t + 1) * BN, w.nk, wave, lane);
         }
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
@@ -491,8 +494,10 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
                 f32x16 s, dp;
                 zero16(s);
                 zero16(dp);
+                __builtin_amdgcn_s_setprio(1);
                 L::mma_rows(s, Ks + b * 32 * L::ROWB, ln, qf);   // S^T[key][query]
                 L::mma_rows(dp, Vs + b * 32 * L::ROWB, ln, df);  // dP^T[key][query]
+                __builtin_amdgcn_s_setprio(0);
                 if (k0 + 32 > all_see) {
                     const int see = p.causal ? min(w.nk, row + 1 + off) : w.nk;
 #pragma unroll
@@ -661,11 +666,14 @@ __global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd
     const s16x4t* stats = reinterpret_cast<const s16x4t*>(p.stats);
     s16x4t st;
     int fh = hk * p.group, fq = first;  // the next tile to fetch: head, tile
-    auto fetch = [&](int b) {
+    typename L::template Fetch<BN, 4> fetch_q, fetch_do;
+    fetch_q.init(p.ldq, lane);
+    fetch_do.init(p.lddo, lane);
+    auto fetch = [&](unsigned char* to) __attribute__((always_inline)) {
         const int q0 = fq * BN;
         st = stats[2 * ((size_t)fh * p.stat_rows + w.q0 + min(q0 + 32 * qs + l31, w.nq - 1)) + half];
-        L::template fetch<BN, 4>(smem + b * 2 * IMG, (const __bf16*)p.q + (size_t)w.q0 * p.ldq + fh * DH, p.ldq, q0, w.nq, wave, lane);
-        L::template fetch<BN, 4>(smem + b * 2 * IMG + IMG, (const __bf16*)p.dout + (size_t)w.q0 * p.lddo + fh * DH, p.lddo, q0, w.nq, wave, lane);
+        fetch_q(to, (const __bf16*)p.q + (size_t)w.q0 * p.ldq + fh * DH, p.ldq, q0, w.nq, wave, lane);
+        fetch_do(to + IMG, (const __bf16*)p.dout + (size_t)w.q0 * p.lddo + fh * DH, p.lddo, q0, w.nq, wave, lane);
         if (++fq == first + per) {
             fq = first;
             ++fh;
@@ -674,8 +682,10 @@ __global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd
     typename L::frag kf[L::NF];
     L::load_row(kf, (const __bf16*)p.k + (size_t)(w.k0 + key) * p.ldk + hk * DH, mine, half);
     if (nt > 0) {
-        L::template fetch<32 * KB, 4>(Vs, (const __bf16*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, w.t0, w.nk, wave, lane);
-        fetch(0);
+        typename L::template Fetch<32 * KB, 4> fv;
+        fv.init(p.ldv, lane);
+        fv(Vs, (const __bf16*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, w.t0, w.nk, wave, lane);
+        fetch(smem);
     }
     typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
@@ -695,10 +705,12 @@ __global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd
         dma_sync();
         s16x4t now = st;
         asm volatile("" : "+v"(now));  // taken here, where it has landed: a wait further down would include the next tile's transfers
-        if (t + 1 < nt) fetch((t + 1) & 1);
+        if (t + 1 < nt) fetch(smem + ((t + 1) & 1) * 2 * IMG);
         const int q0 = qt * BN + 32 * qs;
         if (++qt == first + per) qt = first;
-        opaque(ln.row);
+        opaque(ln.row);  // addresses are made anew every turn: kept, they would take registers that the sums need
+        opaque(ln.col[0]);
+        opaque(ln.col[1]);
         const unsigned char* Qs = smem + (t & 1) * 2 * IMG + 32 * qs * L::ROWB;
         const unsigned char* Ds = Qs + IMG;
         if (r0 < w.nk && q0 < w.nq && (!p.causal || r0 <= q0 + 31 + off)) {

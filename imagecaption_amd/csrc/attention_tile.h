@@ -231,47 +231,42 @@ struct DmaTile : AttTile<__bf16, DH> {
     // offset.  Inline assembly because the compiler, where it knows of a transfer in flight, waits for it before every
     // transposing LDS read (it cannot tell that the transfer fills another image); the caller waits with dma_sync.  M0 is
     // written and used here only: the compiler sets it anew before every use of its own.
+    // Lane offsets: the swizzle is linear over XOR, so the row block of a transfer only flips bits of the lane's piece, and
+    // its rows go into the uniform base: one vector instruction a transfer, two registers kept.
     template <int ROWS, int NW>
     struct Fetch {
         static constexpr int N = ROWS / ROWS_PER / NW;
         static_assert(ROWS % (ROWS_PER * NW) == 0, "every wave moves the same number of transfers");
-        unsigned off[N];
-        // lane offsets for rows that lie inside the matrix
-        __device__ __forceinline__ void init(int ld, int wave, int lane) { offsets(off, ld, ROWS, wave, lane); }
-        __device__ static __forceinline__ void offsets(unsigned* o, int ld, int last, int wave, int lane) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int r = (wave * N + j) * ROWS_PER + lane / B::PPR;
-                o[j] = (unsigned)min(r, last) * ((unsigned)ld * 2u) + (((unsigned)(lane % B::PPR)) ^ (unsigned)B::swz(r)) * 16u;
-            }
-        }
-        __device__ static __forceinline__ void send(unsigned char* img, const char* base, const unsigned* o, int wave) {
-            const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(
-                (int)(unsigned)(size_t)(const __attribute__((address_space(3))) unsigned char*)(img + wave * N * 1024));
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + j * 1024), "v"(o[j]), "s"(base) : "memory");
+        unsigned piece, row;  // byte offsets of the lane's piece in row block 0 and of its row there
+        __device__ __forceinline__ void init(int ld, int lane) {
+            const int r = lane / B::PPR;
+            piece = (((unsigned)(lane % B::PPR)) ^ (unsigned)B::swz(r)) * 16u;
+            row = (unsigned)r * ((unsigned)ld * 2u);
         }
         __device__ __forceinline__ void operator()(unsigned char* img, const __bf16* g, int ld, int row0, int n, int wave, int lane) const {
             const char* base = (const char*)(g + (size_t)row0 * ld);
+            const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(
+                (int)(unsigned)(size_t)(const __attribute__((address_space(3))) unsigned char*)(img + wave * N * 1024));
             if (row0 + ROWS <= n) {
-                send(img, base, off, wave);
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const int r0 = (wave * N + j) * ROWS_PER;
+                    send(to + j * 1024, base + (size_t)r0 * ((unsigned)ld * 2u), (piece ^ ((unsigned)B::swz(r0) << 4)) + row);
+                }
             } else {
-                unsigned o[N];
-                offsets(o, ld, n - 1 - row0, wave, lane);
-                send(img, base, o, wave);
+                int own = lane / B::PPR;
+                opaque(own);
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const int r0 = (wave * N + j) * ROWS_PER, r = min(r0 + own, n - 1 - row0);
+                    send(to + j * 1024, base, (piece ^ ((unsigned)B::swz(r0) << 4)) + (unsigned)r * ((unsigned)ld * 2u));
+                }
             }
         }
+        __device__ static __forceinline__ void send(unsigned to, const char* base, unsigned off) {
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+        }
     };
-    // the same without offsets kept: for kernels whose accumulators leave no registers for them
-    template <int ROWS, int NW>
-    __device__ static __forceinline__ void fetch(unsigned char* img, const __bf16* g, int ld, int row0, int n, int wave, int lane) {
-        using F = Fetch<ROWS, NW>;
-        unsigned o[F::N];
-        opaque(lane);
-        F::offsets(o, ld, n - 1 - row0, wave, lane);
-        F::send(img, (const char*)(g + (size_t)row0 * ld), o, wave);
-    }
 };
 // every transfer of this wave has landed, and every wave of the workgroup has come this far
 __device__ __forceinline__ void dma_sync() {

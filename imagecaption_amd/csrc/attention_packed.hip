@@ -328,25 +328,41 @@ __device__ __forceinline__ float row_delta(const PackedParams& p, typename AttTi
     return d + __shfl_xor(d, 32, 64);
 }
 
-// lse times log2 e of this lane's row: p = exp2(s c - lse2); a row that sees nothing has lse = -inf, its weights are zeros.
-// Leaves the row's statistics for the dk / dv kernel (write: this lane does).
+// lse times log2 e of this lane's row: p = exp2(s c - lse2); a row that sees nothing has lse = -inf, its weights are zeros
+__device__ __forceinline__ float row_lse2(const PackedParams& p, size_t grow, int head, bool mine) {
+    const float lse2 = mine ? p.lse[(size_t)head * p.stat_rows + grow] * LOG2E : INFINITY;
+    return lse2 == -INFINITY ? INFINITY : lse2;
+}
+
+// the row's statistics for the dk / dv kernel
 template <typename T>
-__device__ __forceinline__ float row_stats(const PackedParams& p, float dsum, size_t grow, int head, bool mine, bool write) {
+__device__ __forceinline__ void leave_stats(const PackedParams& p, float lse2, float dsum, size_t grow, int head) {
     const size_t at = (size_t)head * p.stat_rows + grow;
-    float lse2 = mine ? p.lse[at] * LOG2E : INFINITY;
-    if (lse2 == -INFINITY) lse2 = INFINITY;
-    if (mine && write) {
-        if (sizeof(T) == 2 && p.stats) {
-            // -lse / scale and -delta, three bf16 terms each; a row that sees nothing gets weights of zero
-            const float l = lse2 == INFINITY ? -1e30f : -lse2 / (p.scale * LOG2E), d = -dsum;
-            const __bf16 l0 = (__bf16)l, l1 = (__bf16)(l - (float)l0), l2 = (__bf16)(l - (float)l0 - (float)l1);
-            const __bf16 d0 = (__bf16)d, d1 = (__bf16)(d - (float)d0), d2 = (__bf16)(d - (float)d0 - (float)d1);
-            reinterpret_cast<bf16x8t*>(p.stats)[at] = bf16x8t{l0, l1, l2, (__bf16)0.f, d0, d1, d2, (__bf16)0.f};
-        } else {
-            p.delta[at] = dsum;
-        }
+    if (sizeof(T) == 2 && p.stats) {
+        // -lse / scale and -delta, three bf16 terms each; a row that sees nothing gets weights of zero
+        const float l = lse2 == INFINITY ? -1e30f : -lse2 / (p.scale * LOG2E), d = -dsum;
+        const __bf16 l0 = (__bf16)l, l1 = (__bf16)(l - (float)l0), l2 = (__bf16)(l - (float)l0 - (float)l1);
+        const __bf16 d0 = (__bf16)d, d1 = (__bf16)(d - (float)d0), d2 = (__bf16)(d - (float)d0 - (float)d1);
+        reinterpret_cast<bf16x8t*>(p.stats)[at] = bf16x8t{l0, l1, l2, (__bf16)0.f, d0, d1, d2, (__bf16)0.f};
+    } else {
+        p.delta[at] = dsum;
     }
-    return lse2;
+}
+
+// Score gradients of one block: x = p (dp - delta).  Rows whose keys all lie in this block take delta = sum p dp from the
+// block itself: from the rounded o it is off by 2^-9 |do . o|, which is all that dq and dk of such rows consist of when they
+// see one key (their true value is zero) and more than the other roundings when they see a few.
+__device__ __forceinline__ void score_grads(float* x, const f32x16& s, const f32x16& dp, float c, float lse2, bool one_block, float& dsum) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = exp2_fast(__fmaf_rn(s[r], c, -lse2));
+    if (one_block) {
+        float d = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) d = __fmaf_rn(x[r], x[r] > 0.f ? dp[r] : 0.f, d);
+        dsum = d + __shfl_xor(d, 32, 64);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= dp[r] - dsum;
 }
 
 // dq and delta = rowsum(do * o); blocks and waves as in the forward
@@ -374,9 +390,10 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
     const size_t grow = (size_t)(w.q0 + row);
 
     typename L::frag qf[L::NF], df[L::NF];
-    const float dsum = row_delta<T, DH>(p, df, grow, head, mine, half);
+    float dsum = row_delta<T, DH>(p, df, grow, head, mine, half);
     L::load_row(qf, (const T*)p.q + grow * p.ldq + head * DH, mine, half);
-    const float lse2 = row_stats<T>(p, dsum, grow, head, mine, half == 0 && ksp == 0);
+    const float lse2 = row_lse2(p, grow, head, mine);
+    const bool one_block = wave_end <= 32;
     Staged<T, DH, NT, BN> ks, vs;
     if (nt > 0) {
         ks.load(kg, p.ldk, 0, w.nk, tid);
@@ -416,8 +433,7 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
                     for (int r = 0; r < 16; ++r) s[r] = k0 + row_of(r, half) < see ? s[r] : -INFINITY;
                 }
                 float x[16];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = exp2_fast(__fmaf_rn(s[r], c, -lse2)) * (dp[r] - dsum);
+                score_grads(x, s, dp, c, lse2, one_block, dsum);
                 typename L::weights dw;
                 L::pack(dw, x);
                 L::mma_cols(acc, Ks + b * 32 * L::ROWB, ln, dw);  // dQ^T[dim][query] += K^T dS^T
@@ -438,7 +454,10 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
 #pragma unroll
         for (int o = 0; o < KS - 1; ++o) add_sums<L::NDT>(smem + (rb * (KS - 1) + o) * BOX, acc, lane, 1.f, 1.f);
     }
-    if (mine) L::store_row((T*)p.dq + grow * p.lddq + head * DH, acc, p.scale, half);
+    if (mine) {
+        L::store_row((T*)p.dq + grow * p.lddq + head * DH, acc, p.scale, half);
+        if (half == 0) leave_stats<T>(p, lse2, dsum, grow, head);
+    }
 }
 
 // dq of bf16 matrices with 128 rows a workgroup, fed as the forward is
@@ -470,9 +489,10 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
         fv(smem + IMG, vg, p.ldv, 0, w.nk, wave, lane);
     }
     typename L::frag qf[L::NF], df[L::NF];
-    const float dsum = row_delta<__bf16, DH>(p, df, grow, head, mine, half);
+    float dsum = row_delta<__bf16, DH>(p, df, grow, head, mine, half);
     L::load_row(qf, (const __bf16*)p.q + grow * p.ldq + head * DH, mine, half);
-    const float lse2 = row_stats<__bf16>(p, dsum, grow, head, mine, half == 0);
+    const float lse2 = row_lse2(p, grow, head, mine);
+    const bool one_block = wave_end <= 32;
     landed(qf);
     typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
@@ -504,8 +524,7 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
                     for (int r = 0; r < 16; ++r) s[r] = k0 + row_of(r, half) < see ? s[r] : -INFINITY;
                 }
                 float x[16];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = exp2_fast(__fmaf_rn(s[r], c, -lse2)) * (dp[r] - dsum);
+                score_grads(x, s, dp, c, lse2, one_block, dsum);
                 typename L::weights dw;
                 L::pack(dw, x);
                 L::mma_cols(acc, Ks + b * 32 * L::ROWB, ln, dw);  // dQ^T[dim][query] += K^T dS^T
@@ -516,7 +535,10 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
         turn(t, smem, smem + 2 * IMG);
         if (t + 1 < nt) turn(t + 1, smem + 2 * IMG, smem);
     }
-    if (mine) L::store_row((__bf16*)p.dq + grow * p.lddq + head * DH, acc, p.scale, half);
+    if (mine) {
+        L::store_row((__bf16*)p.dq + grow * p.lddq + head * DH, acc, p.scale, half);
+        if (half == 0) leave_stats<__bf16>(p, lse2, dsum, grow, head);
+    }
 }
 
 // dk, dv: KB blocks of 32 key rows of one key / value head, every block walked by QS waves that take every QS-th query tile

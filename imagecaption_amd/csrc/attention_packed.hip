@@ -106,7 +106,7 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd
         ks.store(smem, tid);
         vs.store(smem + IMG, tid);
     }
-    const typename L::lanes ln = L::make_lanes(lane);
+    typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
     f32x16 acc[L::NDT];
 #pragma unroll
@@ -124,6 +124,7 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd
             vs.load(vg, p.ldv, (t + 1) * BN, w.nk, tid);
         }
         __builtin_amdgcn_sched_barrier(0);
+        renew<DH>(ln);
         const int k0 = t * BN + ksp * 32 * KB;
         if (k0 < wave_end) {
             f32x16 s[KB];
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
         ks.store(smem, tid);
         vs.store(smem + IMG, tid);
     }
-    const typename L::lanes ln = L::make_lanes(lane);
+    typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
     f32x16 acc[L::NDT];
 #pragma unroll
@@ -418,6 +419,7 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
             vs.load(vg, p.ldv, (t + 1) * BN, w.nk, tid);
         }
         __builtin_amdgcn_sched_barrier(0);
+        renew<DH>(ln);
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
             const int k0 = t * BN + (ksp * KB + b) * 32;
@@ -544,11 +546,11 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
 // dk, dv: KB blocks of 32 key rows of one key / value head, every block walked by QS waves that take every QS-th query tile
 // of every query head of the group and add up at the end.  Runs after packed_bwd_dq_kernel (reads delta).
 template <typename T, int DH, int KB, int QS>
-__global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && sizeof(T) == 2 ? 2 : 1) void packed_bwd_dkv_kernel(PackedParams p) {
+__global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && (sizeof(T) == 2 || DH == 64) ? 2 : 1) void packed_bwd_dkv_kernel(PackedParams p) {
     using L = AttTile<T, DH>;
     constexpr int NT = KB * QS * 64, BN = 32 * QS, IMG = BN * L::ROWB, KIMG = 32 * KB * L::ROWB;
-    constexpr bool V_LDS = sizeof(T) == 2 && DH == 128 && NT > 64;
-    constexpr int BOX = DH / 4 * 16 * 64, JOIN = KB * (QS - 1) * BOX, WALK = 2 * IMG + (V_LDS ? KIMG : 0);
+    constexpr bool OWN_LDS = sizeof(T) == 4 && DH == 64 && NT > 64;  // the block's own rows stay in LDS: two waves a SIMD
+    constexpr int BOX = DH / 4 * 16 * 64, JOIN = KB * (QS - 1) * BOX, WALK = 2 * IMG + (OWN_LDS ? 2 * KIMG : 0);
     __shared__ __attribute__((aligned(1024))) unsigned char smem[WALK > JOIN ? WALK : JOIN];
     __shared__ float stat[2][BN];  // [lse2 | delta][query]
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
@@ -563,15 +565,20 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && sizeof(T) == 2 ? 2 : 
     const int first = p.causal ? max(0, w.t0 - off) / BN : 0;
     const int per = max(0, (w.nq + BN - 1) / BN - first), nt = per * p.group;
 
-    typename L::frag kf[L::NF], vf[V_LDS ? 1 : L::NF];
-    L::load_row(kf, (const T*)p.k + (size_t)(w.k0 + key) * p.ldk + hk * DH, mine, half);
-    unsigned char* Vs = smem + 2 * IMG;
-    if constexpr (V_LDS) {
-        Staged<T, DH, NT, 32 * KB> vs;
-        vs.load((const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, w.t0, w.nk, tid);
-        vs.store(Vs, tid);
+    typename L::frag kf[OWN_LDS ? 1 : L::NF], vf[OWN_LDS ? 1 : L::NF];
+    unsigned char* Ks = smem + 2 * IMG;
+    unsigned char* Vs = Ks + KIMG;
+    if constexpr (OWN_LDS) {
+        Staged<T, DH, NT, 32 * KB> own;
+        own.load((const T*)p.k + (size_t)w.k0 * p.ldk + hk * DH, p.ldk, w.t0, w.nk, tid);
+        own.store(Ks, tid);
+        own.load((const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, w.t0, w.nk, tid);
+        own.store(Vs, tid);
     } else {
+        L::load_row(kf, (const T*)p.k + (size_t)(w.k0 + key) * p.ldk + hk * DH, mine, half);
         L::load_row(vf, (const T*)p.v + (size_t)(w.k0 + key) * p.ldv + hk * DH, mine, half);
+        landed(kf);
+        landed(vf);
     }
     Staged<T, DH, NT, BN> qst, dst;
     float st = 0.f;  // threads 0 .. BN - 1: a row's lse2, the next BN: its delta
@@ -591,7 +598,7 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && sizeof(T) == 2 ? 2 : 
         }
     };
     if (nt > 0) fetch(0);
-    const typename L::lanes ln = L::make_lanes(lane);
+    typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
     f32x16 dk[L::NDT], dv[L::NDT];
 #pragma unroll
@@ -599,8 +606,6 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && sizeof(T) == 2 ? 2 : 
         zero16(dk[dt]);
         zero16(dv[dt]);
     }
-    landed(kf);
-    if constexpr (!V_LDS) landed(vf);
     for (int t = 0; t < nt; ++t) {
         qst.store(smem, tid);
         dst.store(smem + IMG, tid);
@@ -608,20 +613,22 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && sizeof(T) == 2 ? 2 : 
         __syncthreads();
         if (t + 1 < nt) fetch(t + 1);
         __builtin_amdgcn_sched_barrier(0);
+        renew<DH>(ln);
         const int q0 = (first + t % per) * BN + 32 * qs;
         const unsigned char* Qs = smem + 32 * qs * L::ROWB;
         const unsigned char* Ds = Qs + IMG;
         if (r0 < w.nk && q0 < w.nq && (!p.causal || r0 <= q0 + 31 + off)) {
             f32x16 s, dp;
             zero16(s);
-            L::mma_rows(s, Qs, ln, kf);  // S[query][key]
+            if constexpr (OWN_LDS) L::mma_images(s, Qs, Ks + kb * 32 * L::ROWB, ln);  // S[query][key]
+            else L::mma_rows(s, Qs, ln, kf);
             // queries past the end have lse2 = +inf (weight zero); keys past the end are nobody's
             if (p.causal && q0 + off < r0 + 31) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = key <= q0 + row_of(r, half) + off ? s[r] : -INFINITY;
             }
             zero16(dp);  // dP[query][key]
-            if constexpr (V_LDS) L::mma_images(dp, Ds, Vs + kb * 32 * L::ROWB, ln);
+            if constexpr (OWN_LDS) L::mma_images(dp, Ds, Vs + kb * 32 * L::ROWB, ln);
             else L::mma_rows(dp, Ds, ln, vf);
             float x[16], y[16];
 #pragma unroll

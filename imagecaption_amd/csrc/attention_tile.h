@@ -182,6 +182,15 @@ struct AttTile<float, DH> {
             for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[i][j], acc, 0, 0, 0);
         }
     }
+    __device__ static __forceinline__ void mma_images(f32x16& acc, const unsigned char* img, const unsigned char* own, const lanes& l) {
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            const int at = l.l31 * ROWB + (((2 * i + l.half) ^ swz(l.l31)) << 4);
+            const f32x4t a = *reinterpret_cast<const f32x4t*>(img + at), b = *reinterpret_cast<const f32x4t*>(own + at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc, 0, 0, 0);
+        }
+    }
     __device__ static __forceinline__ void pack(weights& w, const float* x) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) w.f[r] = x[r];
@@ -220,6 +229,13 @@ __device__ __forceinline__ void landed(F (&f)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
 }
+
+// lane constants made anew: the LDS addresses of a turn are not kept for the next one (fp32 has 16 of them for every 32 head
+// dims; kept, they push the accumulators out of the registers)
+template <int DH>
+__device__ __forceinline__ void renew(typename AttTile<float, DH>::lanes& l) { opaque(l.l31); }
+template <int DH>
+__device__ __forceinline__ void renew(typename AttTile<__bf16, DH>::lanes&) {}
 
 // ---- tiles that travel global -> LDS without registers (bf16) -------------------------------------------------------
 template <int DH>

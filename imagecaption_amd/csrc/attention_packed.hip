@@ -883,7 +883,7 @@ static int packed_check(const char* what, const capdec_packed_seqs* s, int Hq, i
     CAPDEC_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "%s: Hq=%d must be a positive multiple of Hkv=%d", what, Hq, Hkv);
     CAPDEC_REQUIRE(dh == 64 || dh == 128, "%s: head dim %d not in {64,128}", what, dh);
     CAPDEC_REQUIRE(dtype == CAPDEC_F32 || dtype == CAPDEC_BF16S, "%s: dtype %d: fp32 (CAPDEC_F32) or bf16 (CAPDEC_BF16S) matrices", what, dtype);
-    CAPDEC_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite", what);
+    CAPDEC_REQUIRE(scale_ok(scale), "%s: scale must lie between 2^-60 and 2^60", what);
     CAPDEC_REQUIRE((int64_t)Hq * dh < (1 << 24), "%s: Hq=%d heads of %d: too wide", what, Hq, dh);
     const int64_t most = std::max(s->tiles[2], s->tiles[5]);
     CAPDEC_REQUIRE(most * Hq < (1ll << 31), "%s: too many tiles for one launch", what);
@@ -981,8 +981,9 @@ extern "C" int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void
                        packed_mat(dk, lddk, Hkv * dh, es, seqs->rows_k) && packed_mat(dv, lddv, Hkv * dh, es, seqs->rows_k),
                    "capdec_attn_packed_bwd: matrices must be non-null, 16-byte aligned, with row strides that are multiples of 16 "
                    "bytes, cover the heads and do not pass 2^25 bytes");
-    CAPDEC_REQUIRE(seqs->rows_q == 0 || (lse && delta && stat_rows >= (size_t)seqs->rows_q),
-                   "capdec_attn_packed_bwd: lse / delta missing, or stat_rows=%zu below the %d query rows", stat_rows, seqs->rows_q);
+    CAPDEC_REQUIRE(seqs->rows_q == 0 || (lse && delta && aligned16(delta) && stat_rows >= (size_t)seqs->rows_q),
+                   "capdec_attn_packed_bwd: lse / delta missing, delta not 16-byte aligned, or stat_rows=%zu below the %d query rows", stat_rows,
+                   seqs->rows_q);
     PackedParams p;
     memset(&p, 0, sizeof(p));
     p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.lse = (float*)lse; p.delta = (float*)delta;

@@ -722,7 +722,7 @@ extern "C" int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, in
     CAPDEC_REQUIRE(kv_lens && page_table && ld_table >= table_cols, "capdec_attn_paged: lengths / page table missing, or ld_table=%d below %d columns",
                    ld_table, table_cols);
     CAPDEC_REQUIRE(cu_q || rows >= n, "capdec_attn_paged: %d rows for %d sequences of one token", rows, n);
-    CAPDEC_REQUIRE(scale > 0.f && scale < INFINITY, "capdec_attn_paged: scale must be positive and finite");
+    CAPDEC_REQUIRE(scale_ok(scale), "capdec_attn_paged: scale must lie between 2^-60 and 2^60");
     if (rows == 0) return 0;
     CAPDEC_REQUIRE(q && o && aligned16(q) && aligned16(o) && ldq % 8 == 0 && ldo % 8 == 0 && ldq >= Hq * cache->dh && ldo >= Hq * cache->dh,
                    "capdec_attn_paged: q / o must be non-null, 16-byte aligned bf16 matrices with row strides that are multiples of 8 and cover "

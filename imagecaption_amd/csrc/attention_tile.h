@@ -127,10 +127,6 @@ struct AttTile<__bf16, DH> {
                 f[m * NDT + dt] = bf16x8t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             }
     }
-    __device__ static __forceinline__ void mma_read_rows(f32x16& acc, const bf16x8t* a, const frag* b) {
-#pragma unroll
-        for (int ks = 0; ks < NF; ++ks) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks], b[ks], acc, 0, 0, 0);
-    }
     __device__ static __forceinline__ void mma_read_cols(f32x16* out, const bf16x8t* a, const weights& w) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -290,6 +286,9 @@ __device__ __forceinline__ void dma_sync() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
+
+// scores are scaled by any factor from 2^-60 to 2^60 (beyond, lse / scale and its like leave fp32)
+static inline bool scale_ok(float s) { return s >= 0x1p-60f && s <= 0x1p60f; }
 
 // ROWS consecutive rows of a matrix on their way global -> registers -> LDS image, shared out over NT threads in
 // 16-byte pieces.  Rows at or past `n` become zeros: a weight of zero times whatever lies behind the last row (the next

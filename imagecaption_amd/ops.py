@@ -975,9 +975,12 @@ _ES = {torch.float32: 4, torch.bfloat16: 2}
 def _rows(t, name, dtype, rows, width, cur):
     """(pointer, row stride) of a [>= rows, width] matrix of ``dtype`` on device ``cur``, rows in whole 16-byte pieces."""
     shape, strides, at = t.shape, t.stride(), t.data_ptr()
-    if t.dtype is dtype and len(shape) == 2 and shape[1] == width and shape[0] >= rows and t.get_device() == cur and (
-            shape[0] == 0 or (strides[1] == 1 and width <= strides[0] and not strides[0] * _ES[dtype] % 16 and not at % 16)):
-        return at, (strides[0] if shape[0] else width)
+    if t.dtype is dtype and len(shape) == 2 and shape[1] == width and shape[0] >= rows and t.get_device() == cur:
+        if shape[0] > 1:
+            if strides[1] == 1 and width <= strides[0] and not strides[0] * _ES[dtype] % 16 and not at % 16:
+                return at, strides[0]
+        elif shape[0] == 0 or (strides[1] == 1 and not at % 16):  # (the stride of a single row means nothing)
+            return at, width
     _elsewhere(name, t, cur)
     raise _capi.CapdecError(f"{name}: need a 16-byte aligned {dtype} [>= {rows}, {width}] matrix with unit column stride and a row "
                             f"stride in whole 16 bytes, got {t.dtype} {tuple(shape)} / {strides}")
@@ -1000,8 +1003,6 @@ def _packed_args(name, q, k, v, Hq, Hkv, seqs, scale):
     if seqs.table.get_device() != cur:
         _elsewhere(name + ".seqs", seqs.table, cur)
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise _capi.CapdecError(f"{name}: scale {scale} must be positive and finite")
     return (dh, cur, F32 if dt is torch.float32 else _capi.BF16S, scale, _rows(q, name + ".q", dt, seqs.rows_q, Hq * dh, cur),
             _rows(k, name + ".k", dt, seqs.rows_k, Hkv * dh, cur), _rows(v, name + ".v", dt, seqs.rows_k, Hkv * dh, cur))
 

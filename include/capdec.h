@@ -352,9 +352,11 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
  *   o[i,h,:] = sum_j softmax_j(scale q[i,h,:].k[j,h',:]) v[j,h',:] over the rows j of i's own sequence; causal: row i of
  *   nq sees the rows j <= i + nk - nq.  A row that sees nothing (lens_k = 0, or causal with nk < nq) gets o = 0 and
  *   lse = -inf, and gradients of zero.  Rows behind the last sequence are not touched.
- *   lse / delta: fp32 [Hq, stat_rows], entry head * stat_rows + row; lse (natural log-sum-exp of the scaled scores) may be
- *   NULL in fwd; delta is scratch that bwd fills (rowsum(do * o)).
+ *   lse: fp32 [Hq, stat_rows], entry head * stat_rows + row, the natural log-sum-exp of the scaled scores; may be NULL in
+ *   fwd.  delta: 16-byte aligned scratch that bwd fills, Hq * stat_rows * 4 bytes with CAPDEC_F32, Hq * stat_rows * 16
+ *   bytes with CAPDEC_BF16S.
  *   bwd: dq, dk, dv from do; dk / dv sum over the query heads of their group.  No atomics: bitwise reproducible.
+ *   scale between 2^-60 and 2^60.
  * dtype CAPDEC_F32: every matrix fp32, exact fp32 products; CAPDEC_BF16S: every matrix bf16, fp32 accumulation, softmax and
  * statistics, probabilities and score gradients rounded to bf16 for the products that take them (the only roundings
  * besides the results').  dh in {64, 128}; 16-byte aligned matrices, row strides multiples of 16 bytes, at most 2^25 bytes.  Non-finite values:
@@ -399,7 +401,8 @@ int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ld
  *   NULL: one token each, row s).  max_q is the largest nq (a hint: more rows are still computed, more slowly).  Query head h
  *   reads key / value head h / (Hq / heads).  Products in bf16 with fp32 accumulation, softmax in fp32; weights are rounded
  *   to bf16 for the context product (after the value's scale is multiplied in), the result once.  A token that sees nothing
- *   gets o = 0, lse = -inf; lse (fp32 [Hq, rows]) may be NULL.  Rows behind the last sequence stay as they are.
+ *   gets o = 0, lse = -inf; lse (fp32 [Hq, rows]) may be NULL.  Rows behind the last sequence stay as they are.  scale between
+ *   2^-60 and 2^60.
  *   Everything that varies from step to step (cu_q, kv_lens, page_table) is read on the device, so a captured call can be
  *   replayed with new contents.  The keys are split over workgroups and joined in a second launch when there are few rows;
  *   the workspace (capdec_attn_paged_workspace_bytes, 16-byte aligned) needs no clearing and must not be shared by calls

@@ -218,6 +218,49 @@ def test_autograd_against_differences():
 
 
 @pytest.mark.gpu
+def test_a_single_row_and_gradients_of_any_layout():
+    """One packed row (whose row stride means nothing), gradients that arrive expanded or transposed, bf16 leaves."""
+    from imagecaption_amd import functional
+    ops = _ops()
+    for lq in ([1], [3, 40]):
+        q, k, v, do = _inputs(lq, lq, 2, 1, 64, torch.bfloat16, 61)
+        seqs = ops.PackedSeqs(lq, device=DEV)
+        o, lse = ops.attn_packed_fwd(q, k, v, 2, 1, seqs)
+        for grad in (torch.ones_like(o), do):
+            want = ops.attn_packed_bwd(q, k, v, o, grad.contiguous(), lse, 2, 1, seqs)
+            leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+            got = functional.attn_packed(*leaves, 2, 1, seqs)
+            assert torch.equal(got, o)
+            if grad is do:
+                got.backward(do.t().contiguous().t())
+            else:
+                got.sum().backward()
+            assert all(torch.equal(a.grad, b) for a, b in zip(leaves, want))
+        if lq == [1]:  # one key: the softmax is 1 whatever the score
+            assert bool((want[0] == 0).all()) and bool((want[1] == 0).all()) and torch.equal(o[:, :64], v)
+            turned = q.reshape(-1, 1).contiguous().t()
+            assert turned.stride(0) == 1
+            assert torch.equal(ops.attn_packed_fwd(turned, k, v, 2, 1, seqs)[0], o)
+
+
+@pytest.mark.gpu
+def test_extreme_scales():
+    """Scores that all but vanish, and scores that leave one key of each row."""
+    ops = _ops()
+    lq, Hq, Hkv, dh = [130, 5], 2, 2, 64
+    for scale in (2.0 ** -60, 1e-6, 8.0):
+        for dtype in (torch.bfloat16, torch.float32):
+            q, k, v, do = _inputs(lq, lq, Hq, Hkv, dh, dtype, 71)
+            seqs = ops.PackedSeqs(lq, device=DEV)
+            ref = reference(q, k, v, do, lq, lq, Hq, Hkv, True, scale, E16 if dtype == torch.bfloat16 else 0.0)
+            o, lse = ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs, scale=scale)
+            within("o", o, ref)
+            within("lse", lse, ref)
+            for n, t in zip(("dq", "dk", "dv"), ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, scale=scale)):
+                within(n, t, ref)
+
+
+@pytest.mark.gpu
 def test_captured_calls_and_other_streams():
     ops = _ops()
     lq, Hq, Hkv, dh = [20, 150, 9], 4, 2, 64
@@ -269,7 +312,7 @@ def test_plans_and_arguments_are_refused_without_a_gpu():
     s.table = 16
     good = dict(q=16, ldq=128, k=16, ldk=64, v=16, ldv=64, o=16, ldo=128, Hq=2, Hkv=1, dh=64, dtype=0, scale=0.1, rows=3)
     for change in (dict(Hq=3, Hkv=2), dict(Hkv=0), dict(dh=32), dict(dtype=1), dict(scale=0.0), dict(scale=-1.0),
-                   dict(scale=math.inf), dict(q=None), dict(k=8), dict(ldq=126), dict(ldk=65), dict(ldo=64), dict(rows=2)):
+                   dict(scale=math.inf), dict(scale=1e-30), dict(q=None), dict(k=8), dict(ldq=126), dict(ldk=65), dict(ldo=64), dict(rows=2)):
         a = dict(good, **change)
         assert lib.capdec_attn_packed_fwd(C.byref(s), a["q"], a["ldq"], a["k"], a["ldk"], a["v"], a["ldv"], a["o"], a["ldo"], 16,
                                           a["rows"], a["Hq"], a["Hkv"], a["dh"], a["dtype"], a["scale"], None) == -1, change

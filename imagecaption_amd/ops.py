@@ -931,7 +931,8 @@ class PackedSeqs:
     """Lengths of the sequences that lie back to back in the rows of packed matrices, and the tile table that the packed
     attention kernels walk on the device: made once for a set of lengths, used by every layer and both directions.
     ``lengths_k`` None: keys / values have the queries' lengths.  ``causal``: row i of nq sees the rows j <= i + nk - nq
-    of its sequence.  Makes a blocking copy to ``device``: not under graph capture."""
+    of its sequence.  Makes a blocking copy to ``device`` (not under graph capture).  A graph that captured calls with it reads
+    its table at every replay: keep it as long as the graph."""
 
     def __init__(self, lengths_q, lengths_k=None, causal=True, device="cuda"):
         lq = [int(v) for v in lengths_q]
@@ -947,10 +948,15 @@ class PackedSeqs:
         n = len(lq)
         cq, ck = (C.c_int * n)(*lq), (C.c_int * n)(*lk)
         l = lib()
+        if torch.cuda.is_current_stream_capturing():
+            raise _capi.CapdecError("PackedSeqs: the blocking copy of its table cannot be captured; make it before the capture")
         self.table = torch.empty(l.capdec_packed_table_bytes(cq, ck, n), dtype=torch.uint8, device=device)
         self.c = _capi.PackedSeqs()
         self.cref = C.byref(self.c)
         with torch.cuda.device(self.table.device):
+            self.stream = stream()
+            # the block may have belonged to a tensor that work queued on this stream still writes
+            torch.cuda.current_stream().synchronize()
             check(l.capdec_packed_plan(cq, ck, n, int(self.causal), ptr(self.table), self.table.numel(), C.byref(self.c)),
                   "capdec_packed_plan")
 
@@ -994,6 +1000,14 @@ def _vector(t, name, dtype, n, cur):
     raise _capi.CapdecError(f"{name}: need a dense {dtype} vector of {n}, got {t.dtype} {tuple(t.shape)} / {t.stride()}")
 
 
+def _table_stream(seqs):
+    """The current stream; the allocator learns of a use of the plan's table on a stream other than its own."""
+    st = stream()
+    if st != seqs.stream:
+        seqs.table.record_stream(torch.cuda.current_stream())
+    return st
+
+
 def _packed_args(name, q, k, v, Hq, Hkv, seqs, scale):
     if q.dtype not in _ES:
         raise _capi.CapdecError(f"{name}: q is {q.dtype}: fp32 or bf16 matrices")
@@ -1024,7 +1038,7 @@ def attn_packed_fwd(q, k, v, Hq, Hkv, seqs, out=None, save_lse=True, scale=None)
         if rows > n:
             lse[:, n:].zero_()
     check(lib().capdec_attn_packed_fwd(seqs.cref, pq, lq, pk, lk, pv, lv, po, lo, None if lse is None else lse.data_ptr(), rows, Hq, Hkv,
-                                       dh, dtype, scale, stream()), "capdec_attn_packed_fwd")
+                                       dh, dtype, scale, _table_stream(seqs)), "capdec_attn_packed_fwd")
     return out, lse
 
 
@@ -1058,7 +1072,7 @@ def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=Non
     # scratch: rowsum(do * o), with bf16 matrices 16 bytes for each (head, row)
     delta = lse.new_empty(lse.numel() * (1 if dtype == F32 else 4))
     check(lib().capdec_attn_packed_bwd(seqs.cref, pq, lq, pk, lk, pv, lv, po, lo, pdo, ldo, lse.data_ptr(), delta.data_ptr(),
-                                       lse.shape[1], pdq, ldq, pdk, ldk, pdv, ldv, Hq, Hkv, dh, dtype, scale, stream()),
+                                       lse.shape[1], pdq, ldq, pdk, ldk, pdv, ldv, Hq, Hkv, dh, dtype, scale, _table_stream(seqs)),
           "capdec_attn_packed_bwd")
     return dq, dk, dv
 

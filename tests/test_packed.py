@@ -289,6 +289,55 @@ def test_captured_calls_and_other_streams():
     assert torch.equal(o, o2) and all(torch.equal(a, b) for a, b in zip(eager, got))
 
 
+@pytest.mark.gpu
+def test_a_plan_made_while_its_memory_is_still_written():
+    """The allocator hands out blocks that work queued on the same stream may still write."""
+    from imagecaption_amd._capi import CapdecError
+    ops = _ops()
+    lengths = [300 + i for i in range(200)]
+    want = ops.PackedSeqs(lengths, device=DEV)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        block = torch.empty_like(want.table)
+        at = block.data_ptr()
+        torch.cuda._sleep(20_000_000)
+        block.fill_(255)
+        del block
+        got = ops.PackedSeqs(lengths, device=DEV)
+    side.synchronize()
+    assert got.table.data_ptr() == at  # the test means something
+    assert torch.equal(got.table, want.table)
+    graph = torch.cuda.CUDAGraph()
+    x = torch.zeros(4, device=DEV)
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(CapdecError, match="before the capture"):
+            ops.PackedSeqs([3], device=DEV)
+    graph.replay()
+    assert x.tolist() == [1.0] * 4
+
+
+@pytest.mark.gpu
+def test_a_plan_freed_while_another_stream_reads_it():
+    ops = _ops()
+    lq, Hq, Hkv, dh = [700] * 40, 4, 4, 64
+    q, k, v, _ = _inputs(lq, lq, Hq, Hkv, dh, torch.bfloat16, 81)
+    seqs = ops.PackedSeqs(lq, device=DEV)
+    want, _ = ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    seqs = ops.PackedSeqs(lq, device=DEV)
+    at, size = seqs.table.data_ptr(), seqs.table.numel()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got, _ = ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs)
+    del seqs
+    later = torch.empty(size, dtype=torch.uint8, device=DEV)  # on the table's own stream: must not be its block yet
+    assert later.data_ptr() != at
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
 def test_plans_and_arguments_are_refused_without_a_gpu():
     from imagecaption_amd import _capi
     from imagecaption_amd._capi import CapdecError

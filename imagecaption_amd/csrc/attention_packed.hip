@@ -803,7 +803,7 @@ static bool lengths_ok(const int* lens, int n) {
         if (lens[i] < 0) return false;
         sum += lens[i];
     }
-    return sum < (1ll << 31);
+    return sum < (1ll << 31) - 1024;  // (a tile's first row plus its height stays an int)
 }
 
 }  // namespace capdec
@@ -822,7 +822,7 @@ extern "C" int capdec_packed_plan(const int* lens_q, const int* lens_k, int n, i
                                   capdec_packed_seqs* seqs) {
     CAPDEC_REQUIRE(lens_q && table_dev && seqs && n > 0, "capdec_packed_plan: bad arguments (n=%d)", n);
     const size_t need = capdec_packed_table_bytes(lens_q, lens_k, n);
-    CAPDEC_REQUIRE(need > 0, "capdec_packed_plan: a length is negative, or the rows pass 2^31");
+    CAPDEC_REQUIRE(need > 0, "capdec_packed_plan: a length is negative, or the rows pass 2^31 - 1024");
     CAPDEC_REQUIRE(aligned16(table_dev), "capdec_packed_plan: the table must be 16-byte aligned");
     if (table_bytes < need) {
         set_error("capdec_packed_plan: table of %zu bytes, %zu needed", table_bytes, need);

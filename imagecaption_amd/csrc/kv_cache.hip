@@ -213,7 +213,8 @@ extern "C" int capdec_kv_read(const capdec_kv_cache* cache, const int* slots, in
 extern "C" int capdec_kv_bad_pages(unsigned int* count, int reset) {
     CAPDEC_REQUIRE(count, "capdec_kv_bad_pages: null pointer");
     unsigned int slots = 0, pages = 0;
-    if (hipMemcpyFromSymbol(&slots, HIP_SYMBOL(g_bad_slots), sizeof(slots)) != hipSuccess || paged_bad_count(&pages, reset != 0) != 0) {
+    // (the copies alone would not wait for kernels on streams that do not block the default one)
+    if (hipDeviceSynchronize() != hipSuccess || hipMemcpyFromSymbol(&slots, HIP_SYMBOL(g_bad_slots), sizeof(slots)) != hipSuccess || paged_bad_count(&pages, reset != 0) != 0) {
         set_error("capdec_kv_bad_pages: reading the counters failed");
         return CAPDEC_ERR_LAUNCH;
     }

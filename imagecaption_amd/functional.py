@@ -178,11 +178,13 @@ class AttnPackedFn(torch.autograd.Function):
         return o
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse = ctx.saved_tensors
         Hq, Hkv, seqs, scale = ctx.meta
-        # the gradient may come in any layout: autograd promises values, not strides
-        do = do if do.stride(-1) == 1 and do.stride(0) == do.shape[1] and do.data_ptr() % 16 == 0 else do.contiguous()
+        # the gradient may come in any layout and at any address: autograd promises values, not strides
+        if not do.is_contiguous() or do.data_ptr() % 16:
+            do = do.clone(memory_format=torch.contiguous_format)
         dq, dk, dv = ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, scale=scale)
         return dq, dk, dv, None, None, None, None
 

@@ -937,8 +937,8 @@ class PackedSeqs:
     def __init__(self, lengths_q, lengths_k=None, causal=True, device="cuda"):
         lq = [int(v) for v in lengths_q]
         lk = lq if lengths_k is None else [int(v) for v in lengths_k]
-        if not lq or len(lq) != len(lk) or min(min(lq), min(lk)) < 0 or max(sum(lq), sum(lk)) >= 1 << 31:
-            raise _capi.CapdecError("PackedSeqs: one length >= 0 for every sequence, under 2^31 rows together, as many for the "
+        if not lq or len(lq) != len(lk) or min(min(lq), min(lk)) < 0 or max(sum(lq), sum(lk)) >= (1 << 31) - 1024:
+            raise _capi.CapdecError("PackedSeqs: one length >= 0 for every sequence, under 2^31 - 1024 rows together, as many for the "
                                     "keys as for the queries")
         device = torch.device(device)
         if device.type != "cuda":
@@ -983,7 +983,7 @@ def _rows(t, name, dtype, rows, width, cur):
     shape, strides, at = t.shape, t.stride(), t.data_ptr()
     if t.dtype is dtype and len(shape) == 2 and shape[1] == width and shape[0] >= rows and t.get_device() == cur:
         if shape[0] > 1:
-            if strides[1] == 1 and width <= strides[0] and not strides[0] * _ES[dtype] % 16 and not at % 16:
+            if strides[1] == 1 and width <= strides[0] < 1 << 31 and not strides[0] * _ES[dtype] % 16 and not at % 16:
                 return at, strides[0]
         elif shape[0] == 0 or (strides[1] == 1 and not at % 16):  # (the stride of a single row means nothing)
             return at, width
@@ -1024,7 +1024,7 @@ def _packed_args(name, q, k, v, Hq, Hkv, seqs, scale):
 def attn_packed_fwd(q, k, v, Hq, Hkv, seqs, out=None, save_lse=True, scale=None):
     """Attention over packed sequences: q [>= rows_q, Hq * dh], k / v [>= rows_k, Hkv * dh] (row-strided views, all fp32 or
     all bf16, dh 64 or 128), ``seqs`` a PackedSeqs.  Returns (o, lse [Hq, rows of q] or None).  Rows behind the last sequence
-    stay as they are in a given ``out`` and are zeros in a new one."""
+    stay as they are in a given ``out`` (which must not overlap q, k or v) and are zeros in a new one."""
     dh, cur, dtype, scale, (pq, lq), (pk, lk), (pv, lv) = _packed_args("attn_packed_fwd", q, k, v, Hq, Hkv, seqs, scale)
     rows, n = q.shape[0], seqs.rows_q
     if out is None:
@@ -1044,7 +1044,8 @@ def attn_packed_fwd(q, k, v, Hq, Hkv, seqs, out=None, save_lse=True, scale=None)
 
 def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=None, scale=None):
     """(dq, dk, dv) of attn_packed_fwd; ``o`` / ``lse`` are its results, ``do`` the gradient of o.  Given dq / dk / dv are
-    written in place, rows behind the last sequence stay as they are there and are zeros in new ones."""
+    written in place (they must not overlap the other matrices), rows behind the last sequence stay as they are there and are
+    zeros in new ones."""
     name = "attn_packed_bwd"
     dh, cur, dtype, scale, (pq, lq), (pk, lk), (pv, lv) = _packed_args(name, q, k, v, Hq, Hkv, seqs, scale)
     dt, n, nk, wide, narrow = q.dtype, seqs.rows_q, seqs.rows_k, Hq * dh, Hkv * dh
@@ -1113,9 +1114,16 @@ class PagedKVCache:
         return cls(k, v, *(torch.empty((pages, heads, page), dtype=torch.float32, device=device) for _ in range(2)))
 
     def slots(self, table, positions):
-        """int32 slots of ``positions`` (int tensor) in the sequence whose pages are ``table`` (a row of the page table)."""
-        positions = positions.long()
-        return (table[positions // self.page].long() * self.page + positions % self.page).to(torch.int32)
+        """int32 slots of ``positions`` (int tensor) in the sequence whose pages are ``table`` (a row of the page table).  A
+        position outside the table, or on a page outside the cache, gets the first slot past the cache: the kernels skip and
+        count it (``check_pages``)."""
+        positions, none = positions.long(), self.pages * self.page
+        if table.numel() == 0:
+            return torch.full_like(positions, none, dtype=torch.int32)
+        column = torch.div(positions, self.page, rounding_mode="floor")
+        page = table[column.clamp(0, table.numel() - 1)].long()
+        there = (column >= 0) & (column < table.numel()) & (page >= 0) & (page < self.pages)
+        return torch.where(there, page * self.page + positions % self.page, none).to(torch.int32)
 
 
 def _on_one(name, *tensors):
@@ -1168,7 +1176,7 @@ def attn_paged(q, cache, page_table, kv_lens, Hq, cu_q=None, max_q=1, out=None, 
     holds the new tokens of the n sequences back to back, sequence s those of rows cu_q[s] .. cu_q[s + 1] - 1 (int32 [n + 1];
     None: one each), at most ``max_q``; kv_lens int32 [n]: positions of each sequence with the new ones; page_table int32
     [n, columns].  Causal: new token i of nq sees the positions up to kv_lens - nq + i.  Returns o (rows of no sequence stay as
-    they are in a given ``out`` and are zeros in a new one), or (o, lse [Hq, rows])."""
+    they are in a given ``out`` and are zeros in a new one), or (o, lse [Hq, rows]).  ``out`` must not overlap q or the cache."""
     name = "attn_paged"
     n, cur, dh, heads = kv_lens.numel(), _here(name, q), cache.dh, cache.heads
     if Hq <= 0 or Hq % heads or max_q <= 0:
@@ -1181,9 +1189,9 @@ def attn_paged(q, cache, page_table, kv_lens, Hq, cu_q=None, max_q=1, out=None, 
     pc = None if cu_q is None else _vector(cu_q, name + ".cu_q", torch.int32, n + 1, cur)
     shape, strides = page_table.shape, page_table.stride()
     if page_table.dtype is not torch.int32 or len(shape) != 2 or shape[0] != n or shape[1] == 0 or strides[1] != 1 or n == 0 \
-            or (n > 1 and strides[0] < shape[1]) or page_table.get_device() != cur:
+            or (n > 1 and not shape[1] <= strides[0] < 1 << 31) or page_table.get_device() != cur:
         _elsewhere(name + ".page_table", page_table, cur)
-        raise _capi.CapdecError(f"{name}: page_table {page_table.dtype} {tuple(shape)} / {strides} must be int32 [{n}, columns] with unit "
+        raise _capi.CapdecError(f"{name}: page_table {page_table.dtype} {tuple(shape)} / {strides} must be int32 [{n}, columns] (at least one of each) with unit "
                                 "column stride")
     rows, cols = q.shape[0], shape[1]
     if out is None:
@@ -1227,10 +1235,10 @@ def draft_verify(target, draft, tokens, u_accept, u_sample, num_draft=None, pad=
         """(pointer, row stride) of an [n, d] matrix."""
         strides = t.stride()
         if t.dtype is not dtype or tuple(t.shape) != (n, d) or t.get_device() != cur or (
-                n and d and (d > 1 and strides[1] != 1 or n > 1 and strides[0] < d)):
+                n and d and (d > 1 and strides[1] != 1 or n > 1 and not d <= strides[0] < 1 << 31)):
             _elsewhere(name + what, t, cur)
             raise _capi.CapdecError(f"{name}{what}: need {dtype} {(n, d)} with unit column stride, got {t.dtype} {tuple(t.shape)} / {strides}")
-        return t.data_ptr(), max(strides[0], d)
+        return t.data_ptr(), strides[0] if n > 1 else d
 
     pt, ts, tr = block(target, ".target", d + 1)
     pd, ds, dr = (None, 0, 0) if draft is None else block(draft, ".draft", d)

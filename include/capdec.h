@@ -356,7 +356,7 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
  *   fwd.  delta: 16-byte aligned scratch that bwd fills, Hq * stat_rows * 4 bytes with CAPDEC_F32, Hq * stat_rows * 16
  *   bytes with CAPDEC_BF16S.
  *   bwd: dq, dk, dv from do; dk / dv sum over the query heads of their group.  No atomics: bitwise reproducible.
- *   scale between 2^-60 and 2^60.
+ *   scale between 2^-60 and 2^60.  Results must not overlap the matrices that are read; fewer than 2^31 - 1024 rows a side.
  * dtype CAPDEC_F32: every matrix fp32, exact fp32 products; CAPDEC_BF16S: every matrix bf16, fp32 accumulation, softmax and
  * statistics, probabilities and score gradients rounded to bf16 for the products that take them (the only roundings
  * besides the results').  dh in {64, 128}; 16-byte aligned matrices, row strides multiples of 16 bytes, at most 2^25 bytes.  Non-finite values:
@@ -402,7 +402,8 @@ int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ld
  *   reads key / value head h / (Hq / heads).  Products in bf16 with fp32 accumulation, softmax in fp32; weights are rounded
  *   to bf16 for the context product (after the value's scale is multiplied in), the result once.  A token that sees nothing
  *   gets o = 0, lse = -inf; lse (fp32 [Hq, rows]) may be NULL.  Rows behind the last sequence stay as they are.  scale between
- *   2^-60 and 2^60.
+ *   2^-60 and 2^60.  Positions past kv_lens are never read, whatever their slots hold; an infinity or NaN among the values of
+ *   a seen position reaches the new tokens of ITS sequence that do not see it yet as well (0 x inf), no other sequence.
  *   Everything that varies from step to step (cu_q, kv_lens, page_table) is read on the device, so a captured call can be
  *   replayed with new contents.  The keys are split over workgroups and joined in a second launch when there are few rows;
  *   the workspace (capdec_attn_paged_workspace_bytes, 16-byte aligned) needs no clearing and must not be shared by calls

@@ -236,6 +236,15 @@ def test_a_single_row_and_gradients_of_any_layout():
             else:
                 got.sum().backward()
             assert all(torch.equal(a.grad, b) for a, b in zip(leaves, want))
+            # a gradient that starts two bytes into its memory
+            leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+            joined = torch.cat([o.new_zeros(1), functional.attn_packed(*leaves, 2, 1, seqs).flatten()])
+            joined.backward(torch.cat([o.new_zeros(1), grad.flatten()]))
+            assert all(torch.equal(a.grad, b) for a, b in zip(leaves, want))
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+        first = torch.autograd.grad(functional.attn_packed(*leaves, 2, 1, seqs), leaves, do.clone().requires_grad_(True), create_graph=True)
+        with pytest.raises(RuntimeError):  # no second derivatives, and none that are silently zero
+            torch.autograd.grad(sum(g.float().sum() for g in first), leaves)
         if lq == [1]:  # one key: the softmax is 1 whatever the score
             assert bool((want[0] == 0).all()) and bool((want[1] == 0).all()) and torch.equal(o[:, :64], v)
             turned = q.reshape(-1, 1).contiguous().t()
@@ -342,7 +351,7 @@ def test_plans_and_arguments_are_refused_without_a_gpu():
     from imagecaption_amd import _capi
     from imagecaption_amd._capi import CapdecError
     ops = _ops()
-    for bad in ([], [-1], [3, -2], [1 << 30, 1 << 30]):
+    for bad in ([], [-1], [3, -2], [1 << 30, 1 << 30], [(1 << 31) - 1]):
         with pytest.raises(CapdecError):
             ops.PackedSeqs(bad, device=DEV)
     with pytest.raises(CapdecError):
@@ -352,6 +361,7 @@ def test_plans_and_arguments_are_refused_without_a_gpu():
     lib = _capi.lib()
     ints = lambda *v: (C.c_int * len(v))(*v)
     assert lib.capdec_packed_table_bytes(ints(3, -1), None, 2) == 0
+    assert lib.capdec_packed_table_bytes(ints((1 << 31) - 1), None, 1) == 0 and lib.capdec_packed_table_bytes(ints(1), ints((1 << 31) - 1024), 1) == 0
     assert lib.capdec_packed_table_bytes(ints(128, 0, 129), None, 3) == 32 * 2 * (1 + 2 + 2 + 3 + 4 + 5)
     s = _capi.PackedSeqs()
     assert lib.capdec_packed_plan(ints(3), None, 1, 1, 16, 1, C.byref(s)) == -4  # the table does not fit
@@ -391,5 +401,10 @@ def test_tensors_that_do_not_fit_are_refused():
             ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs, scale=bad)
     with pytest.raises(CapdecError):
         ops.attn_packed_bwd(q, k, v, o, do, lse.t(), Hq, Hkv, seqs)
+    wide = torch.empty((1 << 32) + 512, dtype=torch.bfloat16, device=DEV)
+    two = ops.PackedSeqs([2], device=DEV)
+    for far in ((1 << 32) + 256, 1 << 25):  # a row stride that 32 bits would cut to 256; one of more than 2^25 bytes
+        with pytest.raises(CapdecError):
+            ops.attn_packed_fwd(wide.as_strided((2, Hq * dh), (far, 1)), k, v, Hq, Hkv, two)
     with pytest.raises(CapdecError):
         ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dk=torch.zeros(14, 64, dtype=torch.bfloat16, device=DEV))

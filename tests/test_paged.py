@@ -260,6 +260,44 @@ def test_bad_pages_slots_and_lengths_are_skipped_and_counted(new):
 
 
 @pytest.mark.gpu
+def test_slots_of_positions_and_pages_that_do_not_exist():
+    ops = _ops()
+    ops.check_pages()
+    cache = ops.PagedKVCache.new(6, 2, 16, 64, BF16, DEV)
+    table = torch.tensor([3, -1, 6, 1 << 28, 5], dtype=torch.int32)
+    positions = torch.tensor([0, 15, 16, 40, 48, 63, 64, 79, 80, 1 << 40, -1], dtype=torch.int64)
+    none = cache.pages * cache.page
+    want = [48, 63, none, none, none, none, 80, 95, none, none, none]
+    for t in (table, table.to(DEV)):
+        got = cache.slots(t, positions.to(t.device))
+        assert got.dtype == torch.int32 and got.tolist() == want
+    assert cache.slots(table[:0], positions).tolist() == [none] * len(want)
+    rows = torch.ones(len(want), 2 * 64, dtype=BF16, device=DEV)
+    before = cache.k.clone()
+    ops.kv_cache_write(cache, rows, rows, got)
+    assert torch.equal(cache.k[[0, 1, 2, 4]].view(torch.int16), before[[0, 1, 2, 4]].view(torch.int16))
+    with pytest.raises(IndexError):
+        ops.check_pages()
+
+
+@pytest.mark.gpu
+def test_counts_wait_for_work_on_other_streams():
+    ops = _ops()
+    ops.check_pages()
+    cache = ops.PagedKVCache.new(6, 2, 16, 64, BF16, DEV)
+    rows = torch.ones(3, 2 * 64, dtype=BF16, device=DEV)
+    slots = torch.tensor([0, 6 * 16, 1], dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        ops.kv_cache_write(cache, rows, rows, slots)
+    with pytest.raises(IndexError):
+        ops.check_pages()
+    ops.check_pages()
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """Pages whose byte offsets pass 2^33, and packed rows 2^24 elements apart."""
     ops = _ops()

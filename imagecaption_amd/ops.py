@@ -980,21 +980,30 @@ _ES = {torch.float32: 4, torch.bfloat16: 2}
 
 def _rows(t, name, dtype, rows, width, cur):
     """(pointer, row stride) of a [>= rows, width] matrix of ``dtype`` on device ``cur``, rows in whole 16-byte pieces."""
-    shape, strides, at = t.shape, t.stride(), t.data_ptr()
-    if t.dtype is dtype and len(shape) == 2 and shape[1] == width and shape[0] >= rows and t.get_device() == cur:
-        if shape[0] > 1:
-            if strides[1] == 1 and width <= strides[0] < 1 << 31 and not strides[0] * _ES[dtype] % 16 and not at % 16:
-                return at, strides[0]
-        elif shape[0] == 0 or (strides[1] == 1 and not at % 16):  # (the stride of a single row means nothing)
+    at, shape = t.data_ptr(), t.shape
+    if t.dtype is dtype and not at & 15 and t.get_device() == cur and len(shape) == 2 and shape[1] == width and shape[0] >= rows:
+        if t.is_contiguous():  # (also of a single row, whatever its stride, and of none)
             return at, width
+        strides = t.stride()
+        if strides[1] == 1 and width <= strides[0] < 1 << 31 and not strides[0] * _ES[dtype] & 15:
+            return at, strides[0]
     _elsewhere(name, t, cur)
+    strides = t.stride()
     raise _capi.CapdecError(f"{name}: need a 16-byte aligned {dtype} [>= {rows}, {width}] matrix with unit column stride and a row "
                             f"stride in whole 16 bytes, got {t.dtype} {tuple(shape)} / {strides}")
 
 
+def _fresh(t, rows):
+    """(tensor, pointer, row stride): a new dense matrix like ``t``, with zeros behind the first ``rows``."""
+    new = torch.empty_like(t, memory_format=torch.contiguous_format)
+    if t.shape[0] > rows:
+        new[rows:].zero_()
+    return new, new.data_ptr(), t.shape[1]
+
+
 def _vector(t, name, dtype, n, cur):
     """Pointer of a dense vector of n entries on device ``cur``."""
-    if t.dtype is dtype and t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1) and t.get_device() == cur:
+    if t.dtype is dtype and t.is_contiguous() and t.get_device() == cur and t.dim() == 1 and t.numel() == n:
         return t.data_ptr()
     _elsewhere(name, t, cur)
     raise _capi.CapdecError(f"{name}: need a dense {dtype} vector of {n}, got {t.dtype} {tuple(t.shape)} / {t.stride()}")
@@ -1028,10 +1037,9 @@ def attn_packed_fwd(q, k, v, Hq, Hkv, seqs, out=None, save_lse=True, scale=None)
     dh, cur, dtype, scale, (pq, lq), (pk, lk), (pv, lv) = _packed_args("attn_packed_fwd", q, k, v, Hq, Hkv, seqs, scale)
     rows, n = q.shape[0], seqs.rows_q
     if out is None:
-        out = q.new_empty((rows, Hq * dh))
-        if rows > n:
-            out[n:].zero_()
-    po, lo = _rows(out, "attn_packed_fwd.out", q.dtype, n, Hq * dh, cur)
+        out, po, lo = _fresh(q, n)
+    else:
+        po, lo = _rows(out, "attn_packed_fwd.out", q.dtype, n, Hq * dh, cur)
     lse = None
     if save_lse:
         lse = q.new_empty((Hq, rows), dtype=torch.float32)
@@ -1056,20 +1064,17 @@ def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=Non
         _elsewhere(name + ".lse", lse, cur)
         raise _capi.CapdecError(f"{name}: lse {tuple(lse.shape)} must be the contiguous [Hq, rows] block that attn_packed_fwd returned")
     if dq is None:
-        dq = q.new_empty((q.shape[0], wide))
-        if q.shape[0] > n:
-            dq[n:].zero_()
+        dq, pdq, ldq = _fresh(q, n)
+    else:
+        pdq, ldq = _rows(dq, name + ".dq", dt, n, wide, cur)
     if dk is None:
-        dk = k.new_empty((k.shape[0], narrow))
-        if k.shape[0] > nk:
-            dk[nk:].zero_()
+        dk, pdk, ldk = _fresh(k, nk)
+    else:
+        pdk, ldk = _rows(dk, name + ".dk", dt, nk, narrow, cur)
     if dv is None:
-        dv = v.new_empty((v.shape[0], narrow))
-        if v.shape[0] > nk:
-            dv[nk:].zero_()
-    pdq, ldq = _rows(dq, name + ".dq", dt, n, wide, cur)
-    pdk, ldk = _rows(dk, name + ".dk", dt, nk, narrow, cur)
-    pdv, ldv = _rows(dv, name + ".dv", dt, nk, narrow, cur)
+        dv, pdv, ldv = _fresh(v, nk)
+    else:
+        pdv, ldv = _rows(dv, name + ".dv", dt, nk, narrow, cur)
     # scratch: rowsum(do * o), with bf16 matrices 16 bytes for each (head, row)
     delta = lse.new_empty(lse.numel() * (1 if dtype == F32 else 4))
     check(lib().capdec_attn_packed_bwd(seqs.cref, pq, lq, pk, lk, pv, lv, po, lo, pdo, ldo, lse.data_ptr(), delta.data_ptr(),
@@ -1153,10 +1158,11 @@ def kv_cache_write(cache, k, v, slots):
 
 def kv_cache_read(cache, slots, k=None, v=None, dtype=torch.bfloat16):
     """(k, v): the rows of ``slots`` (int32 [rows]; negative: zeros) as [rows, heads * dh] matrices of ``dtype`` (or into given
-    ones)."""
-    shape = (slots.numel(), cache.heads * cache.dh)
-    k = torch.empty(shape, dtype=dtype, device=cache.k.device) if k is None else k
-    v = torch.empty(shape, dtype=dtype, device=cache.k.device) if v is None else v
+    ones, both of one type)."""
+    if k is None:
+        shape = (slots.numel(), cache.heads * cache.dh)
+        k = cache.k.new_empty(shape, dtype=dtype if v is None else v.dtype)
+    v = torch.empty_like(k, memory_format=torch.contiguous_format) if v is None else v
     rows, dt, pk, lk, pv, lv, ps = _cache_rows("kv_cache_read", cache, k, v, slots)
     check(lib().capdec_kv_read(cache.cref, ps, rows, pk, lk, pv, lv, dt, stream()), "capdec_kv_read")
     return k, v
@@ -1198,11 +1204,11 @@ def attn_paged(q, cache, page_table, kv_lens, Hq, cu_q=None, max_q=1, out=None, 
         # (which rows belong to no sequence is known on the device only)
         out = q.new_empty((rows, Hq * dh)) if cu_q is None and rows == n else q.new_zeros((rows, Hq * dh))
     po, lo = _rows(out, name + ".out", torch.bfloat16, rows, Hq * dh, cur)
-    lse = torch.zeros((Hq, rows), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_zeros((Hq, rows), dtype=torch.float32) if return_lse else None
     l = lib()
     need = l.capdec_attn_paged_workspace_bytes(cache.cref, n, rows, int(max_q), Hq, cols)
     # a block of its own for every call: the allocator keeps it from calls on other streams and from other captured graphs
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     check(l.capdec_attn_paged(cache.cref, pq, lq, pc, pl, page_table.data_ptr(), strides[0] if n > 1 else cols, cols, n, rows,
                               int(max_q), Hq, scale, po, lo, ptr(lse), ptr(ws), need, stream()), "capdec_attn_paged")
     return (out, lse) if return_lse else out

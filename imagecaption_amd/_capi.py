@@ -47,7 +47,7 @@ class TrainGeom(C.Structure):
 
 class PackedSeqs(C.Structure):
     """capdec_packed_seqs of include/capdec.h."""
-    _fields_ = [(n, _i) for n in ("n", "causal", "rows_q", "rows_k")] + [("tiles", _i * 6), ("table", _vp)]
+    _fields_ = [(n, _i) for n in ("n", "causal", "rows_q", "rows_k")] + [("tiles", _i * 6), ("one_block", _i), ("table", _vp)]
 
 
 class KVCache(C.Structure):

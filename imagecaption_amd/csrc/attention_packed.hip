@@ -390,15 +390,17 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH
     const bool mine = row < w.nq;
     const size_t grow = (size_t)(w.q0 + row);
 
+    Staged<T, DH, NT, BN> ks, vs;
+    if (nt > 0) {
+        ks.load(kg, p.ldk, 0, w.nk, tid);
+        vs.load(vg, p.ldv, 0, w.nk, tid);
+    }
     typename L::frag qf[L::NF], df[L::NF];
     float dsum = row_delta<T, DH>(p, df, grow, head, mine, half);
     L::load_row(qf, (const T*)p.q + grow * p.ldq + head * DH, mine, half);
     const float lse2 = row_lse2(p, grow, head, mine);
     const bool one_block = wave_end <= 32;
-    Staged<T, DH, NT, BN> ks, vs;
     if (nt > 0) {
-        ks.load(kg, p.ldk, 0, w.nk, tid);
-        vs.load(vg, p.ldv, 0, w.nk, tid);
         ks.store(smem, tid);
         vs.store(smem + IMG, tid);
     }
@@ -543,6 +545,104 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
     }
 }
 
+// dq, dk, dv of sequences that fit one block of 32 rows on both sides, in one pass: a wave takes a (sequence, key / value head)
+// and walks the query heads of the group.  Everything is read once and o not at all (delta = sum p dp, see score_grads); the
+// scores are made in both orientations because the two sums run over different sides.  256 captions of up to 20 tokens,
+// 8 heads of 64, bf16: 9.8 us (dq, then dk and dv: 14.5).
+template <typename T, int DH>
+__global__ __launch_bounds__(64) void packed_bwd_block_kernel(PackedParams p) {
+    using L = AttTile<T, DH>;
+    constexpr int IMG = 32 * L::ROWB;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
+    __shared__ __attribute__((aligned(16))) float stat[2][32];  // [lse2 | delta][query]
+    const int lane = threadIdx.x, l31 = lane & 31, half = lane >> 5;
+    int hk, it;
+    packed_place(p.Hkv, hk, it);
+    const PackedItem w = p.items[it];
+    const int off = w.nk - w.nq;  // causal: query i sees the keys j <= i + off
+    const bool mine_q = l31 < w.nq, mine_k = l31 < w.nk;
+    unsigned char *Ks = smem, *Vs = smem + IMG, *Qs = smem + 2 * IMG, *Ds = smem + 3 * IMG;
+    Staged<T, DH, 64, 32> ks, vs, qst, dst;
+    float lse2;
+    auto fetch = [&](int head) {
+        qst.load((const T*)p.q + (size_t)w.q0 * p.ldq + head * DH, p.ldq, 0, w.nq, lane);
+        dst.load((const T*)p.dout + (size_t)w.q0 * p.lddo + head * DH, p.lddo, 0, w.nq, lane);
+        lse2 = row_lse2(p, (size_t)(w.q0 + l31), head, mine_q);
+    };
+    ks.load((const T*)p.k + (size_t)w.k0 * p.ldk + hk * DH, p.ldk, 0, w.nk, lane);
+    vs.load((const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, 0, w.nk, lane);
+    fetch(hk * p.group);
+    ks.store(Ks, lane);
+    vs.store(Vs, lane);
+    const typename L::lanes ln = L::make_lanes(lane);
+    const float c = p.scale * LOG2E;
+    const int see = p.causal ? min(w.nk, l31 + 1 + off) : w.nk;
+    f32x16 dk[L::NDT], dv[L::NDT];
+#pragma unroll
+    for (int dt = 0; dt < L::NDT; ++dt) {
+        zero16(dk[dt]);
+        zero16(dv[dt]);
+    }
+    for (int g = 0; g < p.group; ++g) {
+        const int head = hk * p.group + g;
+        qst.store(Qs, lane);
+        dst.store(Ds, lane);
+        if (half == 0) stat[0][l31] = lse2;
+        __syncthreads();
+        float x[16];
+        {
+            f32x16 s, dp, dq[L::NDT];
+            zero16(s);
+            zero16(dp);
+            L::mma_images(s, Ks, Qs, ln);   // S^T[key][query]
+            L::mma_images(dp, Vs, Ds, ln);  // dP^T[key][query]
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = row_of(r, half) < see ? s[r] : -INFINITY;
+            float dsum = 0.f;
+            score_grads(x, s, dp, c, lse2, true, dsum);
+            if (half == 0) stat[1][l31] = dsum;
+            typename L::weights dw;
+            L::pack(dw, x);
+#pragma unroll
+            for (int dt = 0; dt < L::NDT; ++dt) zero16(dq[dt]);
+            L::mma_cols(dq, Ks, ln, dw);  // dQ^T[dim][query] = K^T dS^T
+            if (mine_q) L::store_row((T*)p.dq + (size_t)(w.q0 + l31) * p.lddq + head * DH, dq, p.scale, half);
+        }
+        if (g + 1 < p.group) fetch(head + 1);
+        __syncthreads();
+        f32x16 s, dp;
+        zero16(s);
+        zero16(dp);
+        L::mma_images(s, Qs, Ks, ln);   // S[query][key]
+        L::mma_images(dp, Ds, Vs, ln);  // dP[query][key]
+        if (p.causal) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = l31 <= row_of(r, half) + off ? s[r] : -INFINITY;
+        }
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4t ls = *reinterpret_cast<const f32x4t*>(&stat[0][8 * i + 4 * half]);
+            const f32x4t de = *reinterpret_cast<const f32x4t*>(&stat[1][8 * i + 4 * half]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[4 * i + j] = exp2_fast(__fmaf_rn(s[4 * i + j], c, -ls[j]));
+                y[4 * i + j] = x[4 * i + j] * (dp[4 * i + j] - de[j]);
+            }
+        }
+        typename L::weights pw, dw;
+        L::pack(pw, x);
+        L::pack(dw, y);
+        L::mma_cols(dv, Ds, ln, pw);  // dV^T[dim][key] += dO^T P
+        L::mma_cols(dk, Qs, ln, dw);  // dK^T[dim][key] += Q^T dS
+        __syncthreads();
+    }
+    if (mine_k) {
+        L::store_row((T*)p.dk + (size_t)(w.k0 + l31) * p.lddk + hk * DH, dk, p.scale, half);
+        L::store_row((T*)p.dv + (size_t)(w.k0 + l31) * p.lddv + hk * DH, dv, 1.f, half);
+    }
+}
+
 // dk, dv: KB blocks of 32 key rows of one key / value head, every block walked by QS waves that take every QS-th query tile
 // of every query head of the group and add up at the end.  Runs after packed_bwd_dq_kernel (reads delta).
 template <typename T, int DH, int KB, int QS>
@@ -568,12 +668,10 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && (sizeof(T) == 2 || DH
     typename L::frag kf[OWN_LDS ? 1 : L::NF], vf[OWN_LDS ? 1 : L::NF];
     unsigned char* Ks = smem + 2 * IMG;
     unsigned char* Vs = Ks + KIMG;
+    Staged<T, DH, NT, OWN_LDS ? 32 * KB : 64> own_k, own_v;
     if constexpr (OWN_LDS) {
-        Staged<T, DH, NT, 32 * KB> own;
-        own.load((const T*)p.k + (size_t)w.k0 * p.ldk + hk * DH, p.ldk, w.t0, w.nk, tid);
-        own.store(Ks, tid);
-        own.load((const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, w.t0, w.nk, tid);
-        own.store(Vs, tid);
+        own_k.load((const T*)p.k + (size_t)w.k0 * p.ldk + hk * DH, p.ldk, w.t0, w.nk, tid);
+        own_v.load((const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, w.t0, w.nk, tid);
     } else {
         L::load_row(kf, (const T*)p.k + (size_t)(w.k0 + key) * p.ldk + hk * DH, mine, half);
         L::load_row(vf, (const T*)p.v + (size_t)(w.k0 + key) * p.ldv + hk * DH, mine, half);
@@ -598,6 +696,10 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && (sizeof(T) == 2 || DH
         }
     };
     if (nt > 0) fetch(0);
+    if constexpr (OWN_LDS) {
+        own_k.store(Ks, tid);
+        own_v.store(Vs, tid);
+    }
     typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
     f32x16 dk[L::NDT], dv[L::NDT];
@@ -863,6 +965,9 @@ extern "C" int capdec_packed_plan(const int* lens_q, const int* lens_k, int n, i
             seqs->rows_k += lk[i];
         }
         for (int part = 0; part < 6; ++part) seqs->tiles[part] = count[part];
+        seqs->one_block = 1;
+        for (int i = 0; i < n; ++i)
+            if (std::max(lens_q[i], lk[i]) > 32 || (lens_q[i] == 0) != (lk[i] == 0)) seqs->one_block = 0;
         seqs->table = table_dev;
     } catch (const std::exception& e) {
         set_error("capdec_packed_plan: %s", e.what());
@@ -923,6 +1028,10 @@ static void launch_fwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t
 
 template <typename T, int DH>
 static void launch_bwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t st) {
+    if (s->one_block) {
+        if (s->tiles[5] > 0) CAPDEC_PACKED((packed_bwd_block_kernel<T, DH>), 5, p.Hkv, 64);
+        return;
+    }
     const bool one = short_rows(s->tiles + 3);
     if (sizeof(T) == 2 && !one) p.stats = p.delta;
     if (s->tiles[0] > 0) {
@@ -981,7 +1090,7 @@ extern "C" int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void
                        packed_mat(dk, lddk, Hkv * dh, es, seqs->rows_k) && packed_mat(dv, lddv, Hkv * dh, es, seqs->rows_k),
                    "capdec_attn_packed_bwd: matrices must be non-null, 16-byte aligned, with row strides that are multiples of 16 "
                    "bytes, cover the heads and do not pass 2^25 bytes");
-    CAPDEC_REQUIRE(seqs->rows_q == 0 || (lse && delta && aligned16(delta) && stat_rows >= (size_t)seqs->rows_q),
+    CAPDEC_REQUIRE(seqs->rows_q == 0 || (lse && (delta || seqs->one_block) && aligned16(delta) && stat_rows >= (size_t)seqs->rows_q),
                    "capdec_attn_packed_bwd: lse / delta missing, delta not 16-byte aligned, or stat_rows=%zu below the %d query rows", stat_rows,
                    seqs->rows_q);
     PackedParams p;

@@ -353,7 +353,7 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
  *   nq sees the rows j <= i + nk - nq.  A row that sees nothing (lens_k = 0, or causal with nk < nq) gets o = 0 and
  *   lse = -inf, and gradients of zero.  Rows behind the last sequence are not touched.
  *   lse: fp32 [Hq, stat_rows], entry head * stat_rows + row, the natural log-sum-exp of the scaled scores; may be NULL in
- *   fwd.  delta: 16-byte aligned scratch that bwd fills, Hq * stat_rows * 4 bytes with CAPDEC_F32, Hq * stat_rows * 16
+ *   fwd.  delta: 16-byte aligned scratch that bwd fills (NULL if seqs->one_block), Hq * stat_rows * 4 bytes with CAPDEC_F32, Hq * stat_rows * 16
  *   bytes with CAPDEC_BF16S.
  *   bwd: dq, dk, dv from do; dk / dv sum over the query heads of their group.  No atomics: bitwise reproducible.
  *   scale between 2^-60 and 2^60.  Results must not overlap the matrices that are read; fewer than 2^31 - 1024 rows a side.
@@ -370,6 +370,7 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
 typedef struct capdec_packed_seqs {
     int n, causal, rows_q, rows_k;
     int tiles[6]; /* query tiles of 128 / 64 / 32 rows, key tiles of 128 / 64 / 32 rows */
+    int one_block; /* every sequence has 1 to 32 rows on both sides, or none on either */
     const void* table;
 } capdec_packed_seqs;
 size_t capdec_packed_table_bytes(const int* lens_q, const int* lens_k, int n); /* 0: bad lengths */

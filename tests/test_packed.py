@@ -106,6 +106,34 @@ def _inputs(lq, lk, Hq, Hkv, dh, dtype, seed, extra=0):
     return q, kv[:rk, :Hkv * dh], kv[:rk, 8 + Hkv * dh:], do
 
 
+# every sequence within one block of 32 rows on both sides (or with no rows at all)
+SHORT = [
+    ([1, 32, 20, 0, 7], None, True, 8, 2, 64),
+    ([20, 32, 3], [32, 5, 30], True, 4, 1, 128),   # fewer keys than queries, and more
+    ([31, 2, 17], [9, 32, 1], False, 6, 6, 128),
+    ([18], [25], False, 16, 2, 64),
+    ([0, 0], None, True, 2, 1, 64),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("case", range(len(SHORT)))
+def test_short_sequences_match_float64(case, dtype):
+    ops = _ops()
+    lq, lk, causal, Hq, Hkv, dh = SHORT[case]
+    q, k, v, do = _inputs(lq, lk or lq, Hq, Hkv, dh, dtype, 300 + case, extra=2)
+    scale = 1 / math.sqrt(dh)
+    ref = reference(q, k, v, do, lq, lk or lq, Hq, Hkv, causal, scale, E16 if dtype == torch.bfloat16 else 0.0)
+    seqs = ops.PackedSeqs(lq, lk, causal=causal, device=DEV)
+    assert seqs.c.one_block == 1
+    o, lse = ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs)
+    grads = ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        within(name, t, ref)
+    assert all(torch.equal(a, b) for a, b in zip(grads, ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs)))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("case", range(len(CASES)))

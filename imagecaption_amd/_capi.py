@@ -123,7 +123,7 @@ SIGNATURES = {
     "capdec_kv_write": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _i, _i, _vp, _i, _vp]),
     "capdec_kv_read": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _i, _vp, _i, _i, _vp]),
     "capdec_attn_paged_workspace_bytes": (_sz, [C.POINTER(KVCache), _i, _i, _i, _i, _i]),
-    "capdec_attn_paged": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _vp, _vp, _sz, _vp]),
+    "capdec_attn_paged": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _i, _vp, _vp, _sz, _vp]),
     "capdec_kv_bad_pages": (_i, [C.POINTER(C.c_uint), _i]),
     "capdec_draft_verify": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i64, _vp, _vp, _vp]),
     "capdec_softmax_ce": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _f, _f, _vp]),

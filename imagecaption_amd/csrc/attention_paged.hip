@@ -23,7 +23,7 @@ static __device__ uint4 g_zero_row[16];  // stands in for the rows of positions 
 constexpr int SPLIT_PAGES = 512;  // most pages of a split: their offsets fit LDS
 constexpr int SPLIT_IDS = SPLIT_PAGES + 2;
 constexpr int SPLIT_MIN = 512;    // fewest keys worth a split of their own (and a second launch)
-constexpr int SPLIT_WANT = 384;   // splits in all to aim at: three for every two of the 256 CUs, which hold two workgroups each
+constexpr int SPLIT_WANT = 512;   // workgroups to aim at: two for each of the 256 CUs, which is what they hold
 
 struct PagedParams {
     const void* k; const void* v; const float* ks; const float* vs;
@@ -31,77 +31,160 @@ struct PagedParams {
     const int* cu; const int* lens; const int* table;
     float* part_o; float2* part_ml; int* part_n;
     int ldq, ldo, ld_table, cols, n, rows, Hq, Hkv, group, page_log2, pages;
-    int splits, tiles;
+    int splits, tiles, clear;
     float scale;
 };
 
 // what a workgroup works on
 struct PagedItem {
-    int seq, hk, split, tile;
+    int seq, hk, split, tile, step;  // tiles tile, tile + step, ..
     int a, nq, len, kbegin, kend, nsplit;  // rows a .. a + nq - 1; keys kbegin .. kend - 1 of len
     bool ok;
 };
 
-// Keys of a split: the batch's keys shared out evenly over SPLIT_WANT workgroups, so that the longest sequence gets the most
-// splits and all splits take the same time (8 contexts of 9 to 60 thousand tokens, 32 heads over 4, e4m3: 49 us; aiming at 512:
-// 62 us, at 256: 60 us); at least SPLIT_MIN, at least what the grid's splits need for this sequence, in whole runs
-// of 128.  Every workgroup sums the lengths for itself: a read of n integers.
-__device__ __forceinline__ int split_size(const PagedParams& p, int64_t total, int len) {
-    const int64_t share = (total * p.Hkv * p.tiles + SPLIT_WANT - 1) / SPLIT_WANT;
+// Keys of a split: the batch's work -- keys times tiles of rows -- shared out over SPLIT_WANT workgroups, less what the sequences'
+// shorter last splits are expected to add: all of them run at once and take about as long (a prompt chunk over four sequences:
+// 108 us; without that allowance 116, with a share of every chunk's tiles instead of those it has 126).  At least SPLIT_MIN keys, at least what
+// the longest possible sequence needs to have no more than `splits`, in whole runs of 128.
+__device__ __forceinline__ int split_size(const PagedParams& p, int64_t work, int64_t tiles, int len) {
+    const int64_t room = max((int64_t)SPLIT_WANT - tiles * p.Hkv / 2, (int64_t)SPLIT_WANT / 4);
+    const int64_t share = (work * p.Hkv + room - 1) / room;
     int c = max((int)min(share, (int64_t)(1 << 30)), (len + p.splits - 1) / p.splits);
     c = max(c, SPLIT_MIN);
     c = min(c, (SPLIT_PAGES << p.page_log2) - 128);
     return (c + 127) & ~127;
 }
 
-__device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
-    __shared__ int64_t sums[4];
-    const int cap = p.cols << p.page_log2;
-    if (p.splits > 1) {
-        int64_t total = 0;
-        for (int i = threadIdx.x; i < p.n; i += 256) total += min(max(p.lens[i], 0), cap);
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            total += (int64_t)(((uint64_t)(uint32_t)__shfl_xor((int)(total >> 32), o, 64) << 32) | (uint32_t)__shfl_xor((int)total, o, 64));
-        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = total;
-    }
-    // The row tiles of one (sequence, head, split) go round the XCDs (blockIdx % 8): kept on one XCD they would share its L2,
-    // but a few such groups of up to 16 tiles do not divide by eight (a prompt chunk over four sequences: 134 us against
-    // 123).  Splits are the slowest index, and every further split turns the (sequence, head) pairs by three places: sequences
-    // that end early leave gaps, and these would all be on the same XCDs otherwise.
+    for (int o = 32; o > 0; o >>= 1)
+        v += (int64_t)(((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o, 64) << 32) | (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+// Workgroup -> (sequence, split, tile of BLOCK rows), key / value head.  With splits, only as many workgroups are launched as
+// there can be in all, and which one a workgroup is follows from the lengths, by a scan over them.  (One workgroup for every
+// split that the longest possible sequence could have, most of them without work: 49 us instead of 46 for 8 contexts of 9 to 60
+// thousand tokens, 29 instead of 21 for chunks of 5 drafted tokens over 48 contexts.)  The row tiles of one
+// (sequence, head, split) go round the XCDs (blockIdx % 8): kept on one XCD they would share its L2, but a few such groups of up
+// to 16 tiles do not divide by eight (a prompt chunk over four sequences: 134 us against 123).
+template <int BLOCK>
+__device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
+    __shared__ int64_t sums[2][4];
+    __shared__ int ends[4], found[8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, cap = p.cols << p.page_log2;
     PagedItem w;
-    const int blk = blockIdx.x, pairs = p.n * p.Hkv;
-    w.tile = blk % p.tiles;
-    const int u = blk / p.tiles;
-    w.ok = u < pairs * p.splits;
-    w.split = u / pairs;
-    const int sh = (int)((u % pairs + 3u * (unsigned)w.split) % (unsigned)pairs);
-    w.hk = sh % p.Hkv;
-    w.seq = w.ok ? sh / p.Hkv : 0;
-    if (p.cu) {
-        w.a = min(max(p.cu[w.seq], 0), p.rows);
-        w.nq = min(max(p.cu[w.seq + 1], w.a), p.rows) - w.a;
-    } else {
-        w.a = w.seq;
-        w.nq = 1;
-    }
-    const int len = p.lens[w.seq];
-    w.len = min(max(len, 0), cap);
-    if (len > cap && w.split == 0 && w.tile == 0 && w.hk == 0 && threadIdx.x == 0 && w.ok) atomicAdd(&g_bad_pages, 1u);
+    w.split = 0;
     w.nsplit = 1;
     w.kbegin = 0;
-    w.kend = w.len;
-    if (p.splits > 1) {
+    w.ok = true;
+    int from, to, len;
+    if (p.splits == 1) {
+        const int pair = blockIdx.x / p.tiles;
+        w.tile = blockIdx.x % p.tiles;
+        w.step = p.tiles;
+        w.hk = pair % p.Hkv;
+        w.seq = pair / p.Hkv;
+        from = p.cu ? p.cu[w.seq] : w.seq;
+        to = p.cu ? p.cu[w.seq + 1] : w.seq + 1;
+        len = p.lens[w.seq];
+        w.len = w.kend = min(max(len, 0), cap);
+    } else {
+        w.hk = blockIdx.x % p.Hkv;
+        const int unit = blockIdx.x / p.Hkv;
+        // a thread's sequence: all three numbers are asked for at once
+        auto ask = [&](int i, int& f, int& t, int& l) {
+            f = i < p.n ? (p.cu ? p.cu[i] : i) : 0;
+            t = i < p.n ? (p.cu ? p.cu[i + 1] : i + 1) : 0;
+            l = i < p.n ? p.lens[i] : 0;
+        };
+        auto tiles_of = [&](int f, int t) {
+            f = min(max(f, 0), p.rows);
+            return max(1, ((min(max(t, f), p.rows) - f) * p.group + BLOCK - 1) / BLOCK);
+        };
+        int f, t, l;
+        ask(tid, f, t, l);
+        int64_t tiles = tid < p.n ? tiles_of(f, t) : 0, work = tiles * min(max(l, 0), cap);
+        for (int i = tid + 256; i < p.n; i += 256) {
+            int f2, t2, l2;
+            ask(i, f2, t2, l2);
+            const int64_t more = tiles_of(f2, t2);
+            tiles += more;
+            work += more * min(max(l2, 0), cap);
+        }
+        tiles = wave_sum64(tiles);
+        work = wave_sum64(work);
+        if (lane == 0) {
+            sums[0][wave] = tiles;
+            sums[1][wave] = work;
+        }
         __syncthreads();
-        int size = split_size(p, sums[0] + sums[1] + sums[2] + sums[3], w.len);
-        w.nsplit = max(1, (w.len + size - 1) / size);
-        size = ((w.len + w.nsplit - 1) / w.nsplit + 127) & ~127;  // all of them alike, not whole ones and a rest
-        w.nsplit = max(1, (w.len + size - 1) / size);
+        tiles = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+        work = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+        int before = 0;  // workgroups (of one head) of the sequences already passed
+        for (int i0 = 0; i0 < p.n && before <= unit; i0 += 256) {
+            if (i0) ask(i0 + tid, f, t, l);
+            const int kept = min(max(l, 0), cap), height = tiles_of(f, t);
+            int size = split_size(p, work, tiles, kept), n = max(1, (kept + size - 1) / size);
+            size = max(((kept + n - 1) / n + 127) & ~127, 128);  // all of them alike, not whole ones and a rest
+            n = max(1, (kept + size - 1) / size);
+            const int mine = i0 + tid < p.n ? n * height : 0;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(upto, o, 64);
+                if (lane >= o) upto += x;
+            }
+            if (lane == 63) ends[wave] = upto;
+            __syncthreads();
+            int start = before + upto - mine;
+            for (int i = 0; i < wave; ++i) start += ends[i];
+            const unsigned at = (unsigned)(unit - start);
+            if (at < (unsigned)mine) {
+                found[0] = i0 + tid;
+                found[1] = min((int)(at / (unsigned)height), n - 1);
+                found[2] = n;
+                found[3] = size;
+                found[4] = f;
+                found[5] = t;
+                found[6] = l;
+                found[7] = at % (unsigned)height;
+            }
+            before += ends[0] + ends[1] + ends[2] + ends[3];
+            __syncthreads();
+        }
+        w.ok = unit < before;
+        if (!w.ok) return w;
+        auto take = [&](int i) { return __builtin_amdgcn_readfirstlane(found[i]); };  // (the same for all: scalar registers)
+        const int size = take(3);
+        w.seq = take(0);
+        w.split = take(1);
+        w.nsplit = take(2);
+        from = take(4);
+        to = take(5);
+        len = take(6);
+        w.tile = take(7);
+        w.step = tiles_of(from, to);
+        w.len = min(max(len, 0), cap);
         w.kbegin = w.split * size;
         w.kend = min(w.len, w.kbegin + size);
     }
-    w.ok = w.ok && w.split < w.nsplit;
+    w.a = min(max(from, 0), p.rows);
+    w.nq = min(max(to, w.a), p.rows) - w.a;
+    if (len > cap && w.split == 0 && w.tile == 0 && w.hk == 0 && tid == 0) atomicAdd(&g_bad_pages, 1u);
     return w;
+}
+
+// rows that belong to no sequence, behind the last and before the first: zeros, if the caller wants them
+template <int DH>
+__device__ __forceinline__ void clear_rest(const PagedParams& p, int tid) {
+    if (!p.clear) return;
+    const int begin = p.cu ? min(max(p.cu[0], 0), p.rows) : 0, end = p.cu ? min(max(p.cu[p.n], begin), p.rows) : p.n;
+    auto zero = [&](int row) {
+        for (int i = tid; i < p.Hq * DH / 8; i += 256) reinterpret_cast<uint4*>(p.o + (size_t)row * p.ldo)[i] = uint4{0, 0, 0, 0};
+    };
+    for (int64_t row = blockIdx.x; row < begin; row += gridDim.x) zero((int)row);
+    for (int64_t row = (int64_t)end + blockIdx.x; row < p.rows; row += gridDim.x) zero((int)row);
 }
 
 // the split's pages into LDS, as byte offsets of this head's first row there; pages outside the cache become -1
@@ -252,9 +335,22 @@ __global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2
     __shared__ __attribute__((aligned(16))) float sc[4][2][32];
     __shared__ float ml[4][2][32];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
-    const PagedItem w = paged_place(p);
+    const PagedItem w = paged_place<32 * R>(p);
+    clear_rest<DH>(p, tid);
     if (!w.ok) return;
     const int nrows = w.nq * p.group;
+    constexpr int NQ = 32 * R * L::PPR / 256;
+    uint4 rows[NQ];
+    auto load_rows = [&](int tile) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            const int rl = (j * 256 + tid) / L::PPR, piece = (j * 256 + tid) % L::PPR, r = tile * 32 * R + rl;
+            rows[j] = uint4{0, 0, 0, 0};
+            if (r < nrows)
+                rows[j] = *reinterpret_cast<const uint4*>(p.q + (size_t)(w.a + r / p.group) * p.ldq + (w.hk * p.group + r % p.group) * DH + piece * 8);
+        }
+    };
+    load_rows(w.tile);  // (on their way while the page table is read)
     load_pages(pages, &s_bad, p, w, E4M3 ? DH : 2 * DH, tid, 256);
     const int first_page = w.kbegin >> p.page_log2;
     const typename L::lanes ln = L::make_lanes(lane);
@@ -262,14 +358,12 @@ __global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2
     unsigned char* Vs = smem + wave * IMG;
     unsigned char* Qs = smem + 4 * IMG;
 
-    for (int tile = w.tile; tile * 32 * R < nrows; tile += p.tiles) {
+    for (int tile = w.tile; tile * 32 * R < nrows; tile += w.step) {
+        if (tile != w.tile) load_rows(tile);
 #pragma unroll
-        for (int j = 0; j < 32 * R * L::PPR / 256; ++j) {
-            const int rl = (j * 256 + tid) / L::PPR, piece = (j * 256 + tid) % L::PPR, r = tile * 32 * R + rl;
-            uint4 v = {0, 0, 0, 0};
-            if (r < nrows)
-                v = *reinterpret_cast<const uint4*>(p.q + (size_t)(w.a + r / p.group) * p.ldq + (w.hk * p.group + r % p.group) * DH + piece * 8);
-            *reinterpret_cast<uint4*>(Qs + rl * L::ROWB + ((piece ^ L::swz(rl & 31)) << 4)) = v;
+        for (int j = 0; j < NQ; ++j) {
+            const int rl = (j * 256 + tid) / L::PPR, piece = (j * 256 + tid) % L::PPR;
+            *reinterpret_cast<uint4*>(Qs + rl * L::ROWB + ((piece ^ L::swz(rl & 31)) << 4)) = rows[j];
         }
         int see[R];
 #pragma unroll
@@ -433,7 +527,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     __shared__ int s_bad;
     __shared__ __attribute__((aligned(16))) float sc[2][2][BN];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
-    const PagedItem w = paged_place(p);
+    const PagedItem w = paged_place<128>(p);
+    clear_rest<DH>(p, tid);
     if (!w.ok) return;
     const int nrows = w.nq * p.group;
     load_pages(pages, &s_bad, p, w, E4M3 ? DH : 2 * DH, tid, 256);
@@ -442,7 +537,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     const int first_page = w.kbegin >> p.page_log2;
     const typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
-    for (int tile = w.tile; tile * 128 < nrows; tile += p.tiles) {
+    for (int tile = w.tile; tile * 128 < nrows; tile += w.step) {
         const int r0 = tile * 128 + wave * 32, r = r0 + l31, token = r / p.group, head = w.hk * p.group + r % p.group;
         const int see = min(w.kend, w.len - w.nq + token + 1);
         const int all_see = min(w.kend, w.len - w.nq + r0 / p.group + 1);
@@ -665,22 +760,29 @@ int paged_bad_count(unsigned int* count, bool reset) {
 struct PagedShape {
     bool rows_kernel;
     int block, tiles, splits;  // rows of a tile, tiles of the longest chunk, splits of the longest sequence
+    int64_t blocks;            // workgroups
 };
 
-static PagedShape paged_shape(const capdec_kv_cache* c, int n, int max_q, int Hq, int table_cols) {
+static PagedShape paged_shape(const capdec_kv_cache* c, int n, int rows, int max_q, int Hq, int table_cols) {
     PagedShape s;
-    const int64_t rows = (int64_t)max_q * (Hq / c->heads);
-    s.rows_kernel = rows > 64;
-    s.block = s.rows_kernel ? 128 : (rows > 32 ? 64 : 32);
-    s.tiles = (int)((rows + s.block - 1) / s.block);
-    // the longest sequence of a ragged batch gets up to four times the even share of splits; workgroups without one end at once
-    const int64_t keys = (int64_t)table_cols * c->page, units = (int64_t)n * c->heads * s.tiles;
+    const int64_t group = Hq / c->heads, high = max_q * group;
+    s.rows_kernel = high > 64;
+    s.block = s.rows_kernel ? 128 : (high > 32 ? 64 : 32);
+    s.tiles = (int)((high + s.block - 1) / s.block);
+    // tiles of all chunks together, at most: by their rows, with one that is not full for each
+    const int64_t all = rows * group / s.block + n;
+    // the longest sequence of a ragged batch gets up to four times the even share of splits
+    const int64_t keys = (int64_t)table_cols * c->page, units = std::min((int64_t)n * s.tiles, all) * c->heads;
     int64_t splits = units >= SPLIT_WANT ? 1 : (4 * SPLIT_WANT + units - 1) / units;
     splits = std::min(splits, (keys + SPLIT_MIN - 1) / SPLIT_MIN);
     // (a split's keys are rounded up to whole runs of 128)
     const int64_t most = (int64_t)SPLIT_PAGES * c->page - 128;
     splits = std::max(splits, (keys + most - 1) / most);
     s.splits = (int)std::max<int64_t>(splits, 1);
+    // with s_i splits of at least min(share, most) keys for t_i tiles, sum s_i t_i <= sum t_i (keys_i / min(share, most) + 1),
+    // and share is at least sum keys_i t_i heads / SPLIT_WANT
+    const int64_t by_share = SPLIT_WANT / c->heads + 1, by_most = all * ((keys + most - 1) / most);
+    s.blocks = (s.splits == 1 ? (int64_t)n * s.tiles : std::min(all * s.splits, std::max(by_share, by_most) + all)) * c->heads;
     return s;
 }
 
@@ -690,8 +792,8 @@ static int paged_check(const char* what, const capdec_kv_cache* c, int n, int ro
     CAPDEC_REQUIRE(Hq > 0 && Hq % c->heads == 0 && (int64_t)Hq * c->dh < (1 << 24), "%s: Hq=%d must be a multiple of the cache's %d heads", what, Hq, c->heads);
     CAPDEC_REQUIRE((int64_t)table_cols * c->page < (1ll << 31) - (1 << 20), "%s: a page table of %d columns passes 2^31 positions", what, table_cols);
     CAPDEC_REQUIRE((int64_t)rows * (Hq / c->heads) < (1ll << 30) && (int64_t)max_q * (Hq / c->heads) < (1ll << 30), "%s: too many rows", what);
-    const PagedShape s = paged_shape(c, n, max_q, Hq, table_cols);
-    CAPDEC_REQUIRE((int64_t)n * c->heads * s.splits * s.tiles < (1ll << 31) && (int64_t)rows * Hq < (1ll << 31),
+    const PagedShape s = paged_shape(c, n, rows, max_q, Hq, table_cols);
+    CAPDEC_REQUIRE(s.blocks < (1ll << 31) && (int64_t)rows * Hq < (1ll << 31),
                    "%s: too much work for one launch", what);
     return 0;
 }
@@ -710,14 +812,14 @@ using namespace capdec;
 
 extern "C" size_t capdec_attn_paged_workspace_bytes(const capdec_kv_cache* cache, int n, int rows, int max_q, int Hq, int table_cols) {
     if (paged_check("capdec_attn_paged_workspace_bytes", cache, n, rows, max_q, Hq, table_cols)) return 0;
-    const PagedShape s = paged_shape(cache, n, max_q, Hq, table_cols);
+    const PagedShape s = paged_shape(cache, n, rows, max_q, Hq, table_cols);
     size_t a, b;
     return s.splits == 1 ? 0 : paged_bytes(s.splits, rows, Hq, cache->dh, &a, &b);
 }
 
 extern "C" int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, int ldq, const int* cu_q, const int* kv_lens,
                                  const int* page_table, int ld_table, int table_cols, int n, int rows, int max_q, int Hq, float scale,
-                                 void* o, int ldo, void* lse, void* workspace, size_t workspace_bytes, capdec_stream_t stream) {
+                                 void* o, int ldo, int clear, void* lse, void* workspace, size_t workspace_bytes, capdec_stream_t stream) {
     if (int rc = paged_check("capdec_attn_paged", cache, n, rows, max_q, Hq, table_cols)) return rc;
     CAPDEC_REQUIRE(kv_lens && page_table && ld_table >= table_cols, "capdec_attn_paged: lengths / page table missing, or ld_table=%d below %d columns",
                    ld_table, table_cols);
@@ -727,7 +829,7 @@ extern "C" int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, in
     CAPDEC_REQUIRE(q && o && aligned16(q) && aligned16(o) && ldq % 8 == 0 && ldo % 8 == 0 && ldq >= Hq * cache->dh && ldo >= Hq * cache->dh,
                    "capdec_attn_paged: q / o must be non-null, 16-byte aligned bf16 matrices with row strides that are multiples of 8 and cover "
                    "the heads");
-    const PagedShape s = paged_shape(cache, n, max_q, Hq, table_cols);
+    const PagedShape s = paged_shape(cache, n, rows, max_q, Hq, table_cols);
     PagedParams p;
     memset(&p, 0, sizeof(p));
     if (s.splits > 1) {
@@ -747,8 +849,8 @@ extern "C" int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, in
     p.cu = cu_q; p.lens = kv_lens; p.table = page_table;
     p.ldq = ldq; p.ldo = ldo; p.ld_table = ld_table; p.cols = table_cols; p.n = n; p.rows = rows;
     p.Hq = Hq; p.Hkv = cache->heads; p.group = Hq / cache->heads; p.page_log2 = log2_of(cache->page); p.pages = cache->pages;
-    p.splits = s.splits; p.tiles = s.tiles; p.scale = scale;
-    const unsigned blocks = (unsigned)((int64_t)n * cache->heads * s.splits * s.tiles);
+    p.splits = s.splits; p.tiles = s.tiles; p.clear = clear != 0; p.scale = scale;
+    const unsigned blocks = (unsigned)s.blocks;
     const bool e = cache->dtype == CAPDEC_E4M3, wide = cache->dh == 128;
     hipStream_t st = (hipStream_t)stream;
 #define CAPDEC_PAGED(E, D)                                                                                       \

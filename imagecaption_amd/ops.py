@@ -1200,17 +1200,18 @@ def attn_paged(q, cache, page_table, kv_lens, Hq, cu_q=None, max_q=1, out=None, 
         raise _capi.CapdecError(f"{name}: page_table {page_table.dtype} {tuple(shape)} / {strides} must be int32 [{n}, columns] (at least one of each) with unit "
                                 "column stride")
     rows, cols = q.shape[0], shape[1]
-    if out is None:
-        # (which rows belong to no sequence is known on the device only)
-        out = q.new_empty((rows, Hq * dh)) if cu_q is None and rows == n else q.new_zeros((rows, Hq * dh))
-    po, lo = _rows(out, name + ".out", torch.bfloat16, rows, Hq * dh, cur)
+    clear = out is None  # (which rows belong to no sequence is known on the device only: the kernel clears them)
+    if clear:
+        out, po, lo = _fresh(q, rows)
+    else:
+        po, lo = _rows(out, name + ".out", torch.bfloat16, rows, Hq * dh, cur)
     lse = q.new_zeros((Hq, rows), dtype=torch.float32) if return_lse else None
     l = lib()
     need = l.capdec_attn_paged_workspace_bytes(cache.cref, n, rows, int(max_q), Hq, cols)
     # a block of its own for every call: the allocator keeps it from calls on other streams and from other captured graphs
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     check(l.capdec_attn_paged(cache.cref, pq, lq, pc, pl, page_table.data_ptr(), strides[0] if n > 1 else cols, cols, n, rows,
-                              int(max_q), Hq, scale, po, lo, ptr(lse), ptr(ws), need, stream()), "capdec_attn_paged")
+                              int(max_q), Hq, scale, po, lo, clear, ptr(lse), ptr(ws), need, stream()), "capdec_attn_paged")
     return (out, lse) if return_lse else out
 
 

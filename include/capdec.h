@@ -402,8 +402,8 @@ int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ld
  *   NULL: one token each, row s).  max_q is the largest nq (a hint: more rows are still computed, more slowly).  Query head h
  *   reads key / value head h / (Hq / heads).  Products in bf16 with fp32 accumulation, softmax in fp32; weights are rounded
  *   to bf16 for the context product (after the value's scale is multiplied in), the result once.  A token that sees nothing
- *   gets o = 0, lse = -inf; lse (fp32 [Hq, rows]) may be NULL.  Rows behind the last sequence stay as they are.  scale between
- *   2^-60 and 2^60.  Positions past kv_lens are never read, whatever their slots hold; an infinity or NaN among the values of
+ *   gets o = 0, lse = -inf; lse (fp32 [Hq, rows]) may be NULL.  Rows of no sequence stay as they are in lse,
+ *   and in o too unless `clear` is set: then they get zeros.  scale between 2^-60 and 2^60.  Positions past kv_lens are never read, whatever their slots hold; an infinity or NaN among the values of
  *   a seen position reaches the new tokens of ITS sequence that do not see it yet as well (0 x inf), no other sequence.
  *   Everything that varies from step to step (cu_q, kv_lens, page_table) is read on the device, so a captured call can be
  *   replayed with new contents.  The keys are split over workgroups and joined in a second launch when there are few rows;
@@ -425,7 +425,7 @@ int capdec_kv_read(const capdec_kv_cache* cache, const int* slots, int rows, voi
 size_t capdec_attn_paged_workspace_bytes(const capdec_kv_cache* cache, int n, int rows, int max_q, int Hq, int table_cols);
 int capdec_attn_paged(const capdec_kv_cache* cache, const void* q, int ldq, const int* cu_q, const int* kv_lens,
                       const int* page_table, int ld_table, int table_cols, int n, int rows, int max_q, int Hq, float scale, void* o,
-                      int ldo, void* lse, void* workspace, size_t workspace_bytes, capdec_stream_t stream);
+                      int ldo, int clear, void* lse, void* workspace, size_t workspace_bytes, capdec_stream_t stream);
 int capdec_kv_bad_pages(unsigned int* count, int reset);
 
 /* ---- verification of drafted tokens -------------------------------------------------------------------------------

@@ -148,6 +148,8 @@ PAGED = [
     ([9, 5, 7], [640, 9, 333], 40, 8, 128, 64),                # 45 rows a head: two blocks of 32
     ([33, 70, 1, 20], [300, 70, 64, 1025], 8, 2, 16, 128),     # many rows
     ([200, 131], [900, 131], 3, 3, 256, 64),
+    ([1] * 300, [37 * i % 1990 for i in range(300)], 2, 1, 16, 64),  # more sequences than threads, all sorts of splits
+    ([1, 0, 2] * 90, [1 + 997 * i % 1500 for i in range(270)], 3, 1, 8, 128),
 ]
 
 
@@ -201,6 +203,13 @@ def test_rows_of_no_sequence_and_columns_beside_stay(new):
     assert bool((rest == 7).all())
     fresh = ops.attn_paged(q, cache, table, lens, Hq, cu_q=cu, max_q=max(new))
     assert torch.equal(fresh[2:-3], out[2:-3]) and bool((fresh[:2] == 0).all()) and bool((fresh[-3:] == 0).all())
+    for tokens in (cu, None):  # memory that held something else, one token each as well
+        torch.full((rows, Hq * dh), 9.0, dtype=BF16, device=DEV)
+        fresh = ops.attn_paged(q, cache, table, lens, Hq, cu_q=tokens, max_q=max(new))
+        mine = slice(2, -3) if tokens is not None else slice(0, 3)
+        rest = fresh.clone()
+        rest[mine] = 0
+        assert bool((rest == 0).all()) and not bool((fresh[mine] == 9).any())
 
 
 @pytest.mark.gpu
@@ -523,14 +532,14 @@ def test_arguments_are_refused_without_a_gpu():
     for change in bad:
         assert lib.capdec_kv_write(cache(**change), 16, 128, 16, 128, 0, 16, 3, None) == -1, change
         assert lib.capdec_kv_read(cache(**change), 16, 3, 16, 128, 16, 128, 0, None) == -1, change
-        assert lib.capdec_attn_paged(cache(**change), 16, 128, None, 16, 16, 4, 4, 3, 3, 1, 2, 0.1, 16, 128, None, None, 0, None) == -1, change
+        assert lib.capdec_attn_paged(cache(**change), 16, 128, None, 16, 16, 4, 4, 3, 3, 1, 2, 0.1, 16, 128, 0, None, None, 0, None) == -1, change
         assert lib.capdec_attn_paged_workspace_bytes(cache(**change), 3, 3, 1, 2, 4) == 0
     for k, ldk, v, ldv, dtype, slots, rows in ((None, 128, 16, 128, 0, 16, 3), (16, 64, 16, 128, 0, 16, 3), (16, 130, 16, 128, 0, 16, 3),
                                                 (16, 128, 8, 128, 0, 16, 3), (16, 128, 16, 128, 1, 16, 3), (16, 128, 16, 128, 0, None, 3),
                                                 (16, 128, 16, 128, 0, 16, -1), (16, 132, 16, 128, 3, 16, 3)):
         assert lib.capdec_kv_write(cache(), k, ldk, v, ldv, dtype, slots, rows, None) == -1
     assert lib.capdec_kv_write(cache(), None, 0, None, 0, 0, None, 0, None) == 0  # no rows: nothing to do
-    args = dict(q=16, ldq=128, cu=None, lens=16, table=16, ld=4, cols=4, n=3, rows=3, max_q=1, Hq=2, scale=0.1, o=16, ldo=128, lse=None,
+    args = dict(q=16, ldq=128, cu=None, lens=16, table=16, ld=4, cols=4, n=3, rows=3, max_q=1, Hq=2, scale=0.1, o=16, ldo=128, clear=0, lse=None,
                 ws=None, wb=0, st=None)
     for change in (dict(q=None), dict(ldq=64), dict(ldq=130), dict(lens=None), dict(table=None), dict(ld=3), dict(cols=0), dict(n=0),
                    dict(rows=2), dict(rows=-1), dict(max_q=0), dict(Hq=3), dict(Hq=0), dict(scale=0.0), dict(scale=math.inf), dict(o=8),

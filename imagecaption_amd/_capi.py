@@ -47,7 +47,8 @@ class TrainGeom(C.Structure):
 
 class PackedSeqs(C.Structure):
     """capdec_packed_seqs of include/capdec.h."""
-    _fields_ = [(n, _i) for n in ("n", "causal", "rows_q", "rows_k")] + [("tiles", _i * 6), ("one_block", _i), ("table", _vp)]
+    _fields_ = [(n, _i) for n in ("n", "causal", "rows_q", "rows_k")] + [("tiles", _i * 6), ("one_block", _i), ("walk_max", _i), ("walk_levels", _i * 5),
+                                                                    ("walk_sum", C.c_int64), ("table", _vp)]
 
 
 class KVCache(C.Structure):
@@ -118,7 +119,8 @@ SIGNATURES = {
     "capdec_packed_table_bytes": (_sz, [C.POINTER(_i), C.POINTER(_i), _i]),
     "capdec_packed_plan": (_i, [C.POINTER(_i), C.POINTER(_i), _i, _i, _vp, _sz, C.POINTER(PackedSeqs)]),
     "capdec_attn_packed_fwd": (_i, [C.POINTER(PackedSeqs), _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _sz, _i, _i, _i, _i, _f, _vp]),
-    "capdec_attn_packed_bwd": (_i, [C.POINTER(PackedSeqs), _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _sz,
+    "capdec_attn_packed_scratch_bytes": (_sz, [C.POINTER(PackedSeqs), _sz, _i, _i, _i, _i]),
+    "capdec_attn_packed_bwd": (_i, [C.POINTER(PackedSeqs), _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _sz, _vp, _sz,
                                     _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _f, _vp]),
     "capdec_kv_write": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _i, _i, _vp, _i, _vp]),
     "capdec_kv_read": (_i, [C.POINTER(KVCache), _vp, _i, _vp, _i, _vp, _i, _i, _vp]),

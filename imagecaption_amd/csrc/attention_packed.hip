@@ -26,6 +26,8 @@ struct PackedItem {  // one tile of rows of one sequence
     int reserved[3];
 };
 
+constexpr int WALK_LEVELS = 5;
+
 struct PackedParams {
     const void* q; const void* k; const void* v; const void* o; const void* dout;
     void* out; void* dq; void* dk; void* dv;
@@ -36,6 +38,9 @@ struct PackedParams {
     int Hq, Hkv, group, causal;
     size_t stat_rows;  // rows of one head in lse / delta
     float scale;
+    int parts, slots;          // dk, dv: parts of the longest key tiles (1: no tile is split), partial sums of one head
+    int levels[WALK_LEVELS];   // tiles whose walk is longer than 1/2, 1/4, .. of the longest: parts, parts / 2, .. each
+    float* part;               // partial sums [Hkv, slots, dk | dv, 64 keys, dh]
 };
 
 // workgroup -> (head, item): with heads in eights every XCD (blockIdx % 8) serves its own run of neighbouring heads, so
@@ -50,6 +55,26 @@ __device__ __forceinline__ void packed_place(int heads, int& head, int& item) {
         head = blk % heads;
         item = blk / heads;
     }
+}
+
+// index in the list of key tiles with their parts -> tile, part of its walk, parts of it
+__device__ __forceinline__ void walk_part(const PackedParams& p, int at, int& item, int& part, int& parts) {
+    item = part = 0;
+    parts = 1;
+#pragma unroll
+    for (int l = 0; l < WALK_LEVELS; ++l) {
+        const int cut = p.parts >> l, n = p.levels[l];
+        if (cut <= 1) break;
+        if (at < n * cut) {
+            item += at / cut;
+            part = at % cut;
+            parts = cut;
+            return;
+        }
+        at -= n * cut;
+        item += n;
+    }
+    item += at;
 }
 
 // accumulators of a wave through LDS to another wave with the same lane layout
@@ -77,7 +102,7 @@ __device__ __forceinline__ void add_sums(const unsigned char* box, f32x16* acc, 
 template <typename T, int DH, int RB, int KS, int KB>
 __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd_kernel(PackedParams p) {
     using L = AttTile<T, DH>;
-    constexpr int NT = RB * KS * 64, BN = 32 * KB * KS, IMG = BN * L::ROWB, BOX = (DH / 4 * 16 + 8) * 64;
+    constexpr int NT = RB * KS * 64, BN = 32 * KB * KS, IMG = BN * L::ROWB, BOX = (DH / 8 * 16 + 8) * 64;
     constexpr int JOIN = RB * (KS - 1) * BOX;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG > JOIN ? 4 * IMG : JOIN];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
@@ -180,14 +205,14 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd
         if (ksp > 0) {
             unsigned char* box = smem + (rb * (KS - 1) + ksp - 1) * BOX;
             put_sums<L::NDT>(box, acc, lane);
-            reinterpret_cast<float2*>(box + DH / 4 * 16 * 64)[lane] = float2{run.m2, l};
+            reinterpret_cast<float2*>(box + DH / 8 * 16 * 64)[lane] = float2{run.m2, l};
         }
         __syncthreads();
         if (ksp > 0) return;
 #pragma unroll
         for (int o = 0; o < KS - 1; ++o) {
             const unsigned char* box = smem + (rb * (KS - 1) + o) * BOX;
-            const float2 ml = reinterpret_cast<const float2*>(box + DH / 4 * 16 * 64)[lane];
+            const float2 ml = reinterpret_cast<const float2*>(box + DH / 8 * 16 * 64)[lane];
             const float m = fmaxf(run.m2, ml.x);
             const float fa = run.m2 == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_fast(run.m2 - m);
             const float fb = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - m);
@@ -370,7 +395,7 @@ __device__ __forceinline__ void score_grads(float* x, const f32x16& s, const f32
 template <typename T, int DH, int RB, int KS, int KB>
 __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 && (sizeof(T) == 2 || DH == 64) ? 2 : 1) void packed_bwd_dq_kernel(PackedParams p) {
     using L = AttTile<T, DH>;
-    constexpr int NT = RB * KS * 64, BN = 32 * KB * KS, IMG = BN * L::ROWB, BOX = DH / 4 * 16 * 64;
+    constexpr int NT = RB * KS * 64, BN = 32 * KB * KS, IMG = BN * L::ROWB, BOX = DH / 8 * 16 * 64;
     constexpr int JOIN = RB * (KS - 1) * BOX;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG > JOIN ? 4 * IMG : JOIN];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
@@ -650,7 +675,7 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && (sizeof(T) == 2 || DH
     using L = AttTile<T, DH>;
     constexpr int NT = KB * QS * 64, BN = 32 * QS, IMG = BN * L::ROWB, KIMG = 32 * KB * L::ROWB;
     constexpr bool OWN_LDS = sizeof(T) == 4 && DH == 64 && NT > 64;  // the block's own rows stay in LDS: two waves a SIMD
-    constexpr int BOX = DH / 4 * 16 * 64, JOIN = KB * (QS - 1) * BOX, WALK = 2 * IMG + (OWN_LDS ? 2 * KIMG : 0);
+    constexpr int BOX = DH / 8 * 16 * 64, JOIN = KB * (QS - 1) * BOX, WALK = 2 * IMG + (OWN_LDS ? 2 * KIMG : 0);
     __shared__ __attribute__((aligned(1024))) unsigned char smem[WALK > JOIN ? WALK : JOIN];
     __shared__ float stat[2][BN];  // [lse2 | delta][query]
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
@@ -779,24 +804,27 @@ template <int DH, int KB, int QS>
 __global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd_dkv_kernel(PackedParams p) {
     using L = DmaTile<DH>;
     constexpr int BN = 32 * QS, IMG = BN * L::ROWB, KIMG = 32 * KB * L::ROWB;
-    constexpr int BOX = DH / 4 * 16 * 64, WALK = 4 * IMG + KIMG;
+    constexpr int BOX = DH / 8 * 16 * 64, WALK = 4 * IMG + KIMG;
     static_assert(KB * QS == 4 && KB * (QS - 1) * BOX <= WALK, "the sums of a block fit the images");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[WALK];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const int kb = wave % KB, qs = wave / KB;
-    int hk, it;
-    packed_place(p.Hkv, hk, it);
+    int hk, at, it, part, parts;
+    packed_place(p.Hkv, hk, at);
+    walk_part(p, at, it, part, parts);
     const PackedItem w = p.items[it];
     const int r0 = w.t0 + kb * 32;
     const int key = r0 + l31, off = w.nk - w.nq;
     const bool mine = key < w.nk;
     // causal: query i sees key j iff i >= j - off; the first tile that meets one of the workgroup's keys
     const int first = p.causal ? max(0, w.t0 - off) / BN : 0;
-    const int per = max(0, (w.nq + BN - 1) / BN - first), nt = per * p.group;
+    const int per = max(0, (w.nq + BN - 1) / BN - first), all = per * p.group;
+    const int begin = (int)((int64_t)all * part / parts), nt = (int)((int64_t)all * (part + 1) / parts) - begin;
     unsigned char* Vs = smem + 4 * IMG;
     const s16x4t* stats = reinterpret_cast<const s16x4t*>(p.stats);
     s16x4t st;
-    int fh = hk * p.group, fq = first;  // the next tile to fetch: head, tile
+    // the next tile to fetch: head, tile
+    int fh = hk * p.group + (per ? begin / per : 0), fq = first + (per ? begin % per : 0);
     typename L::template Fetch<BN, 4> fetch_q, fetch_do;
     fetch_q.init(p.ldq, lane);
     fetch_do.init(p.lddo, lane);
@@ -831,7 +859,7 @@ __global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd
         zero16(dv[dt]);
     }
     landed(kf);
-    int qt = first;
+    int qt = first + (per ? begin % per : 0);
     for (int t = 0; t < nt; ++t) {
         dma_sync();
         s16x4t now = st;
@@ -884,10 +912,50 @@ __global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd
             for (int o = 0; o < QS - 1; ++o) add_sums<L::NDT>(smem + (kb * (QS - 1) + o) * BOX, acc, lane, 1.f, 1.f);
         }
     }
-    if (qs == 0 && mine) {
+    if (qs == 0 && mine && parts > 1) {
+        float* to = p.part + ((((size_t)hk * p.slots + at) * 2) * 32 * KB + kb * 32 + l31) * DH;
+        AttTile<float, DH>::store_row(to, dk, 1.f, half);
+        AttTile<float, DH>::store_row(to + 32 * KB * DH, dv, 1.f, half);
+    } else if (qs == 0 && mine) {
         L::store_row((__bf16*)p.dk + (size_t)(w.k0 + key) * p.lddk + hk * DH, dk, p.scale, half);
         L::store_row((__bf16*)p.dv + (size_t)(w.k0 + key) * p.lddv + hk * DH, dv, 1.f, half);
     }
+}
+
+// the parts' sums of one key tile of 64 rows, in order
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
+    typedef T out4 __attribute__((ext_vector_type(4)));
+    constexpr int TILE = 64 * DH;
+    const int hk = blockIdx.x % p.Hkv, tid = threadIdx.x;
+    int it = blockIdx.x / p.Hkv, slot = 0, parts = 1, before = 0;
+#pragma unroll
+    for (int l = 0; l < WALK_LEVELS; ++l) {
+        const int cut = p.parts >> l, n = p.levels[l];
+        if (cut <= 1) break;
+        if (it < before + n) {
+            parts = cut;
+            slot += (it - before) * cut;
+            break;
+        }
+        before += n;
+        slot += n * cut;
+    }
+    const PackedItem w = p.items[it];
+    const float* from = p.part + ((size_t)hk * p.slots + slot) * 2 * TILE;
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+        for (int i = tid; i < TILE / 4; i += 256) {
+            const int row = i / (DH / 4), col = i % (DH / 4) * 4;
+            if (w.t0 + row >= w.nk) break;
+            f32x4t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int s = 0; s < parts; ++s) sum += *reinterpret_cast<const f32x4t*>(from + (size_t)(2 * s + side) * TILE + 4 * i);
+            const float mul = side ? 1.f : p.scale;
+            const out4 v = {(T)(sum[0] * mul), (T)(sum[1] * mul), (T)(sum[2] * mul), (T)(sum[3] * mul)};
+            T* to = side ? (T*)p.dv + (size_t)(w.k0 + w.t0 + row) * p.lddv : (T*)p.dk + (size_t)(w.k0 + w.t0 + row) * p.lddk;
+            *reinterpret_cast<out4*>(to + hk * DH + col) = v;
+        }
 }
 
 // rows of a workgroup's tile, as the plan's table lists them for queries and then for keys
@@ -946,12 +1014,27 @@ extern "C" int capdec_packed_plan(const int* lens_q, const int* lens_k, int n, i
                 q0 += nq;
                 k0 += nk;
             }
-            auto cost = [&](const PackedItem& a) {  // rows of the other side that the tile walks
-                if (keys) return causal ? a.nq - std::max(0, a.t0 - (a.nk - a.nq)) : a.nq;
+            auto cost = [&](const PackedItem& a) {  // tiles of 64 queries / rows of keys that the tile walks
+                if (keys) return std::max(0, (a.nq + 63) / 64 - (causal ? std::max(0, a.t0 - (a.nk - a.nq)) / 64 : 0));
                 return causal ? std::min(a.nk, a.t0 + rows + a.nk - a.nq) : a.nk;
             };
             std::stable_sort(all.begin() + begin, all.end(), [&](const PackedItem& a, const PackedItem& b) { return cost(a) > cost(b); });
             count[part] = (int)(all.size() - begin);
+            if (part == 4) {
+                const int64_t longest = count[part] ? cost(all[begin]) : 0;
+                seqs->walk_max = (int)longest;
+                seqs->walk_sum = 0;
+                for (int l = 0; l < WALK_LEVELS; ++l) seqs->walk_levels[l] = 0;
+                for (size_t i = begin; i < all.size(); ++i) {
+                    const int64_t c = cost(all[i]);
+                    seqs->walk_sum += c;
+                    for (int l = 0; l < WALK_LEVELS; ++l)
+                        if (c << (l + 1) > longest) {
+                            ++seqs->walk_levels[l];
+                            break;
+                        }
+                }
+            }
         }
         if (!all.empty() && hipMemcpy(table_dev, all.data(), all.size() * sizeof(PackedItem), hipMemcpyHostToDevice) != hipSuccess) {
             set_error("capdec_packed_plan: copying the table to the device failed");
@@ -1019,6 +1102,22 @@ static bool short_rows(const int* tiles) { return 2 * (int64_t)tiles[2] < 3 * (i
 template <typename T>
 static bool tall_rows(const int* tiles, int heads) { return sizeof(T) == 2 && (int64_t)tiles[0] * heads >= 512; }
 
+// dk, dv of key tiles whose walk over the queries is much longer than a workgroup's even share (512 run at once) are summed in
+// parts by several workgroups and joined: PARTS_FIGURES
+struct PackedParts {
+    int parts, items, slots;  // of the longest tiles; tiles that are split, their parts together
+};
+static PackedParts packed_parts(const capdec_packed_seqs* s, int Hkv, int group) {
+    PackedParts c = {1, 0, 0};
+    const int64_t longest = (int64_t)s->walk_max * group, all = s->walk_sum * group * Hkv;
+    while (c.parts < (1 << WALK_LEVELS) && 4 * longest * 512 > 5 * all * c.parts && longest >= 16 * c.parts) c.parts *= 2;
+    for (int l = 0; l < WALK_LEVELS && (c.parts >> l) > 1; ++l) {
+        c.items += s->walk_levels[l];
+        c.slots += s->walk_levels[l] * (c.parts >> l);
+    }
+    return c;
+}
+
 template <typename T, int DH>
 static void launch_fwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t st) {
     if (short_rows(s->tiles)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
@@ -1042,14 +1141,29 @@ static void launch_bwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t
     if (s->tiles[3] > 0) {
         if (one) CAPDEC_PACKED((packed_bwd_dkv_kernel<T, DH, 1, 1>), 5, p.Hkv, 64);
         else if constexpr (sizeof(T) == 4) CAPDEC_PACKED((packed_bwd_dkv_kernel<T, DH, 2, 2>), 4, p.Hkv, 256);
-        // 64 keys and two waves a block; 32 keys and four where 64 would leave CUs without a workgroup (one text of 2000 tokens,
-        // 16 heads over 2: backward 261 us against 399; 32 paragraphs of 8 heads of 128 the other way, 73 / 48)
-        else if ((int64_t)s->tiles[4] * p.Hkv < 256) CAPDEC_PACKED((packed16_bwd_dkv_kernel<DH, 1, 4>), 5, p.Hkv, 256);
-        else CAPDEC_PACKED((packed16_bwd_dkv_kernel<DH, 2, 2>), 4, p.Hkv, 256);
+        else {
+            const PackedParts cut = packed_parts(s, p.Hkv, p.group);
+            p.parts = cut.parts;
+            p.slots = cut.slots;
+            for (int l = 0; l < WALK_LEVELS; ++l) p.levels[l] = s->walk_levels[l];
+            p.part = (float*)((char*)p.stats + (size_t)p.Hq * p.stat_rows * 16);
+            p.items = items_of(s, 4);
+            hipLaunchKernelGGL((packed16_bwd_dkv_kernel<DH, 2, 2>), dim3((unsigned)((s->tiles[4] - cut.items + cut.slots) * p.Hkv)), dim3(256), 0, st, p);
+            if (cut.parts > 1) hipLaunchKernelGGL((packed_join_kernel<T, DH>), dim3((unsigned)(cut.items * p.Hkv)), dim3(256), 0, st, p);
+        }
     }
 }
 
 }  // namespace capdec
+
+// [delta or statistics][partial sums]
+extern "C" size_t capdec_attn_packed_scratch_bytes(const capdec_packed_seqs* seqs, size_t stat_rows, int Hq, int Hkv, int dh, int dtype) {
+    if (packed_check("capdec_attn_packed_scratch_bytes", seqs, Hq, Hkv, dh, dtype, 1.f) || seqs->one_block) return 0;
+    if (dtype == CAPDEC_F32) return Hq * stat_rows * 4;
+    size_t bytes = Hq * stat_rows * 16;
+    if (!short_rows(seqs->tiles + 3)) bytes += (size_t)packed_parts(seqs, Hkv, Hq / Hkv).slots * Hkv * 2 * 64 * dh * 4;
+    return bytes;
+}
 
 extern "C" int capdec_attn_packed_fwd(const capdec_packed_seqs* seqs, const void* q, int ldq, const void* k, int ldk, const void* v,
                                       int ldv, void* o, int ldo, void* lse, size_t stat_rows, int Hq, int Hkv, int dh, int dtype,
@@ -1079,8 +1193,8 @@ extern "C" int capdec_attn_packed_fwd(const capdec_packed_seqs* seqs, const void
 }
 
 extern "C" int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ldq, const void* k, int ldk, const void* v,
-                                      int ldv, const void* o, int ldo, const void* dout, int lddo, const void* lse, void* delta,
-                                      size_t stat_rows, void* dq, int lddq, void* dk, int lddk, void* dv, int lddv, int Hq, int Hkv,
+                                      int ldv, const void* o, int ldo, const void* dout, int lddo, const void* lse,
+                                      size_t stat_rows, void* scratch, size_t scratch_bytes, void* dq, int lddq, void* dk, int lddk, void* dv, int lddv, int Hq, int Hkv,
                                       int dh, int dtype, float scale, capdec_stream_t stream) {
     if (int rc = packed_check("capdec_attn_packed_bwd", seqs, Hq, Hkv, dh, dtype, scale)) return rc;
     const int es = dtype == CAPDEC_F32 ? 4 : 2;
@@ -1090,12 +1204,17 @@ extern "C" int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void
                        packed_mat(dk, lddk, Hkv * dh, es, seqs->rows_k) && packed_mat(dv, lddv, Hkv * dh, es, seqs->rows_k),
                    "capdec_attn_packed_bwd: matrices must be non-null, 16-byte aligned, with row strides that are multiples of 16 "
                    "bytes, cover the heads and do not pass 2^25 bytes");
-    CAPDEC_REQUIRE(seqs->rows_q == 0 || (lse && (delta || seqs->one_block) && aligned16(delta) && stat_rows >= (size_t)seqs->rows_q),
-                   "capdec_attn_packed_bwd: lse / delta missing, delta not 16-byte aligned, or stat_rows=%zu below the %d query rows", stat_rows,
-                   seqs->rows_q);
+    CAPDEC_REQUIRE(seqs->rows_q == 0 || (lse && stat_rows >= (size_t)seqs->rows_q),
+                   "capdec_attn_packed_bwd: lse missing, or stat_rows=%zu below the %d query rows", stat_rows, seqs->rows_q);
+    const size_t need = capdec_attn_packed_scratch_bytes(seqs, stat_rows, Hq, Hkv, dh, dtype);
+    CAPDEC_REQUIRE(need == 0 || (scratch && aligned16(scratch)), "capdec_attn_packed_bwd: scratch missing or not 16-byte aligned");
+    if (scratch_bytes < need) {
+        set_error("capdec_attn_packed_bwd: scratch of %zu bytes, %zu needed", scratch_bytes, need);
+        return CAPDEC_ERR_WORKSPACE;
+    }
     PackedParams p;
     memset(&p, 0, sizeof(p));
-    p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.lse = (float*)lse; p.delta = (float*)delta;
+    p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.lse = (float*)lse; p.delta = (float*)scratch;
     p.dq = dq; p.dk = dk; p.dv = dv;
     p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo; p.lddo = lddo; p.lddq = lddq; p.lddk = lddk; p.lddv = lddv;
     p.Hq = Hq; p.Hkv = Hkv; p.group = Hq / Hkv; p.causal = seqs->causal; p.stat_rows = stat_rows; p.scale = scale;

@@ -1075,10 +1075,11 @@ def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=Non
         dv, pdv, ldv = _fresh(v, nk)
     else:
         pdv, ldv = _rows(dv, name + ".dv", dt, nk, narrow, cur)
-    # scratch: rowsum(do * o), with bf16 matrices 16 bytes for each (head, row)
-    delta = None if seqs.c.one_block else lse.new_empty(lse.numel() * (1 if dtype == F32 else 4))
-    check(lib().capdec_attn_packed_bwd(seqs.cref, pq, lq, pk, lk, pv, lv, po, lo, pdo, ldo, lse.data_ptr(), ptr(delta),
-                                       lse.shape[1], pdq, ldq, pdk, ldk, pdv, ldv, Hq, Hkv, dh, dtype, scale, _table_stream(seqs)),
+    l = lib()
+    need = 0 if seqs.c.one_block else l.capdec_attn_packed_scratch_bytes(seqs.cref, lse.shape[1], Hq, Hkv, dh, dtype)
+    ws = lse.new_empty(need, dtype=torch.uint8) if need else None
+    check(l.capdec_attn_packed_bwd(seqs.cref, pq, lq, pk, lk, pv, lv, po, lo, pdo, ldo, lse.data_ptr(), lse.shape[1], ptr(ws), need,
+                                   pdq, ldq, pdk, ldk, pdv, ldv, Hq, Hkv, dh, dtype, scale, _table_stream(seqs)),
           "capdec_attn_packed_bwd")
     return dq, dk, dv
 

@@ -353,8 +353,8 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
  *   nq sees the rows j <= i + nk - nq.  A row that sees nothing (lens_k = 0, or causal with nk < nq) gets o = 0 and
  *   lse = -inf, and gradients of zero.  Rows behind the last sequence are not touched.
  *   lse: fp32 [Hq, stat_rows], entry head * stat_rows + row, the natural log-sum-exp of the scaled scores; may be NULL in
- *   fwd.  delta: 16-byte aligned scratch that bwd fills (NULL if seqs->one_block), Hq * stat_rows * 4 bytes with CAPDEC_F32, Hq * stat_rows * 16
- *   bytes with CAPDEC_BF16S.
+ *   fwd.  scratch: capdec_attn_packed_scratch_bytes bytes (NULL if that is 0), 16-byte aligned, needs no clearing, not to be
+ *   shared by calls that may overlap in time.
  *   bwd: dq, dk, dv from do; dk / dv sum over the query heads of their group.  No atomics: bitwise reproducible.
  *   scale between 2^-60 and 2^60.  Results must not overlap the matrices that are read; fewer than 2^31 - 1024 rows a side.
  * dtype CAPDEC_F32: every matrix fp32, exact fp32 products; CAPDEC_BF16S: every matrix bf16, fp32 accumulation, softmax and
@@ -371,17 +371,20 @@ typedef struct capdec_packed_seqs {
     int n, causal, rows_q, rows_k;
     int tiles[6]; /* query tiles of 128 / 64 / 32 rows, key tiles of 128 / 64 / 32 rows */
     int one_block; /* every sequence has 1 to 32 rows on both sides, or none on either */
+    int walk_max, walk_levels[5]; /* key tiles of 64 rows: the most tiles of 64 queries that one of them meets, and how many meet */
+    int64_t walk_sum;             /* more than 1/2, 1/4, .. 1/32 of that; all of them together */
     const void* table;
 } capdec_packed_seqs;
 size_t capdec_packed_table_bytes(const int* lens_q, const int* lens_k, int n); /* 0: bad lengths */
 int capdec_packed_plan(const int* lens_q, const int* lens_k, int n, int causal, void* table_dev, size_t table_bytes,
                        capdec_packed_seqs* seqs);
+size_t capdec_attn_packed_scratch_bytes(const capdec_packed_seqs* seqs, size_t stat_rows, int Hq, int Hkv, int dh, int dtype);
 int capdec_attn_packed_fwd(const capdec_packed_seqs* seqs, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
                            void* o, int ldo, void* lse, size_t stat_rows, int Hq, int Hkv, int dh, int dtype, float scale,
                            capdec_stream_t stream);
 int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv,
-                           const void* o, int ldo, const void* dout, int lddo, const void* lse, void* delta, size_t stat_rows,
-                           void* dq, int lddq, void* dk, int lddk, void* dv, int lddv, int Hq, int Hkv, int dh, int dtype,
+                           const void* o, int ldo, const void* dout, int lddo, const void* lse, size_t stat_rows, void* scratch,
+                           size_t scratch_bytes, void* dq, int lddq, void* dk, int lddk, void* dv, int lddv, int Hq, int Hkv, int dh, int dtype,
                            float scale, capdec_stream_t stream);
 
 /* ---- paged key / value cache: write, read back, attention of new tokens over it ----------------------------------

@@ -106,6 +106,26 @@ def _inputs(lq, lk, Hq, Hkv, dh, dtype, seed, extra=0):
     return q, kv[:rk, :Hkv * dh], kv[:rk, 8 + Hkv * dh:], do
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq, lk, causal, Hq, Hkv, dh", [([1500, 70], None, True, 8, 1, 64), ([900, 40, 1], [300, 7, 1000], False, 6, 2, 128),
+                                                         ([1100] + [65] * 30, None, True, 4, 4, 128)])
+def test_long_walks_in_parts_match_float64(lq, lk, causal, Hq, Hkv, dh):
+    """Key tiles whose sums over the queries are cut into parts."""
+    from imagecaption_amd import _capi
+    ops = _ops()
+    q, k, v, do = _inputs(lq, lk or lq, Hq, Hkv, dh, torch.bfloat16, 500 + dh)
+    scale = 1 / math.sqrt(dh)
+    ref = reference(q, k, v, do, lq, lk or lq, Hq, Hkv, causal, scale, E16)
+    seqs = ops.PackedSeqs(lq, lk, causal=causal, device=DEV)
+    stats = 16 * Hq * sum(lq)
+    assert _capi.lib().capdec_attn_packed_scratch_bytes(seqs.cref, sum(lq), Hq, Hkv, dh, _capi.BF16S) > stats
+    o, lse = ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs)
+    grads = ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        within(name, t, ref)
+    assert all(torch.equal(a, b) for a, b in zip(grads, ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs)))
+
+
 # every sequence within one block of 32 rows on both sides (or with no rows at all)
 SHORT = [
     ([1, 32, 20, 0, 7], None, True, 8, 2, 64),
@@ -404,8 +424,13 @@ def test_plans_and_arguments_are_refused_without_a_gpu():
         assert lib.capdec_attn_packed_fwd(C.byref(s), a["q"], a["ldq"], a["k"], a["ldk"], a["v"], a["ldv"], a["o"], a["ldo"], 16,
                                           a["rows"], a["Hq"], a["Hkv"], a["dh"], a["dtype"], a["scale"], None) == -1, change
         assert lib.capdec_last_error()
-    assert lib.capdec_attn_packed_bwd(C.byref(s), 16, 128, 16, 64, 16, 64, 16, 128, 16, 128, None, 16, 3, 16, 128, 16, 64, 16, 64,
+    assert lib.capdec_attn_packed_bwd(C.byref(s), 16, 128, 16, 64, 16, 64, 16, 128, 16, 128, None, 3, 16, 1 << 20, 16, 128, 16, 64, 16, 64,
                                       2, 1, 64, 0, 0.1, None) == -1  # no lse
+    need = lib.capdec_attn_packed_scratch_bytes(C.byref(s), 3, 2, 1, 64, 3)
+    assert need >= 2 * 3 * 16
+    for scratch, size, rc in ((None, need, -1), (8, need, -1), (16, need - 1, -4)):
+        assert lib.capdec_attn_packed_bwd(C.byref(s), 16, 128, 16, 64, 16, 64, 16, 128, 16, 128, 16, 3, scratch, size, 16, 128, 16, 64,
+                                          16, 64, 2, 1, 64, 3, 0.1, None) == rc
 
 
 @pytest.mark.gpu

@@ -680,15 +680,17 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && (sizeof(T) == 2 || DH
     __shared__ float stat[2][BN];  // [lse2 | delta][query]
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const int kb = wave % KB, qs = wave / KB;
-    int hk, it;
-    packed_place(p.Hkv, hk, it);
+    int hk, at, it, part, parts;
+    packed_place(p.Hkv, hk, at);
+    walk_part(p, at, it, part, parts);
     const PackedItem w = p.items[it];
     const int r0 = w.t0 + kb * 32;
     const int key = r0 + l31, off = w.nk - w.nq;
     const bool mine = key < w.nk;
     // causal: query i sees key j iff i >= j - off; the first tile that meets one of the workgroup's keys
     const int first = p.causal ? max(0, w.t0 - off) / BN : 0;
-    const int per = max(0, (w.nq + BN - 1) / BN - first), nt = per * p.group;
+    const int per = max(0, (w.nq + BN - 1) / BN - first), all = per * p.group;
+    const int begin = (int)((int64_t)all * part / parts), nt = (int)((int64_t)all * (part + 1) / parts) - begin;
 
     typename L::frag kf[OWN_LDS ? 1 : L::NF], vf[OWN_LDS ? 1 : L::NF];
     unsigned char* Ks = smem + 2 * IMG;
@@ -705,8 +707,8 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && (sizeof(T) == 2 || DH
     }
     Staged<T, DH, NT, BN> qst, dst;
     float st = 0.f;  // threads 0 .. BN - 1: a row's lse2, the next BN: its delta
-    auto fetch = [&](int t) {
-        const int head = hk * p.group + t / per, q0 = (first + t % per) * BN;
+    auto fetch = [&](int i) {
+        const int t = begin + i, head = hk * p.group + t / per, q0 = (first + t % per) * BN;
         qst.load((const T*)p.q + (size_t)w.q0 * p.ldq + head * DH, p.ldq, q0, w.nq, tid);
         dst.load((const T*)p.dout + (size_t)w.q0 * p.lddo + head * DH, p.lddo, q0, w.nq, tid);
         if (tid < 2 * BN) {
@@ -741,7 +743,7 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && (sizeof(T) == 2 || DH
         if (t + 1 < nt) fetch(t + 1);
         __builtin_amdgcn_sched_barrier(0);
         renew<DH>(ln);
-        const int q0 = (first + t % per) * BN + 32 * qs;
+        const int q0 = (first + (begin + t) % per) * BN + 32 * qs;
         const unsigned char* Qs = smem + 32 * qs * L::ROWB;
         const unsigned char* Ds = Qs + IMG;
         if (r0 < w.nk && q0 < w.nq && (!p.causal || r0 <= q0 + 31 + off)) {
@@ -789,21 +791,25 @@ __global__ __launch_bounds__(KB * QS * 64, KB * QS == 4 && (sizeof(T) == 2 || DH
             __syncthreads();
         }
     }
-    if (qs == 0 && mine) {
+    if (qs == 0 && mine && parts > 1) {
+        float* to = p.part + ((((size_t)hk * p.slots + at) * 2) * 32 * KB + kb * 32 + l31) * DH;
+        AttTile<float, DH>::store_row(to, dk, 1.f, half);
+        AttTile<float, DH>::store_row(to + 32 * KB * DH, dv, 1.f, half);
+    } else if (qs == 0 && mine) {
         L::store_row((T*)p.dk + (size_t)(w.k0 + key) * p.lddk + hk * DH, dk, p.scale, half);
         L::store_row((T*)p.dv + (size_t)(w.k0 + key) * p.lddv + hk * DH, dv, 1.f, half);
     }
 }
 
-// The same for bf16 with four waves, KB QS = 4.  Q and dO tiles travel global -> LDS by DMA,
+// The same for bf16, two blocks of two waves.  Q and dO tiles travel global -> LDS by DMA,
 // one tile ahead: the rows come from beyond the L2 (every query head of the group is walked), and registers for them would
 // cost the second wave of a SIMD.  V fragments are read from LDS for the same reason.  Per-query statistics enter the
 // products as one more k-step: -lse / scale and -delta split into three bf16 terms each (24 bits, exact to fp32) times ones,
 // so a lane loads 8 bytes for its own query and no value has to be handed around in accumulator-row order.
-template <int DH, int KB, int QS>
-__global__ __launch_bounds__(256, KB == 2 || DH == 64 ? 2 : 1) void packed16_bwd_dkv_kernel(PackedParams p) {
+template <int DH>
+__global__ __launch_bounds__(256, 2) void packed16_bwd_dkv_kernel(PackedParams p) {
     using L = DmaTile<DH>;
-    constexpr int BN = 32 * QS, IMG = BN * L::ROWB, KIMG = 32 * KB * L::ROWB;
+    constexpr int KB = 2, QS = 2, BN = 32 * QS, IMG = BN * L::ROWB, KIMG = 32 * KB * L::ROWB;
     constexpr int BOX = DH / 8 * 16 * 64, WALK = 4 * IMG + KIMG;
     static_assert(KB * QS == 4 && KB * (QS - 1) * BOX <= WALK, "the sums of a block fit the images");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[WALK];
@@ -1102,6 +1108,12 @@ static bool short_rows(const int* tiles) { return 2 * (int64_t)tiles[2] < 3 * (i
 template <typename T>
 static bool tall_rows(const int* tiles, int heads) { return sizeof(T) == 2 && (int64_t)tiles[0] * heads >= 512; }
 
+// bytes of what dq leaves for dk / dv, whole 16-byte pieces
+template <typename T>
+static size_t stat_bytes(int Hq, size_t stat_rows) {
+    return sizeof(T) == 4 ? (Hq * stat_rows * 4 + 15) & ~(size_t)15 : Hq * stat_rows * 16;
+}
+
 // dk, dv of key tiles whose walk over the queries is much longer than a workgroup's even share (512 run at once) are summed in
 // parts by several workgroups and joined: PARTS_FIGURES
 struct PackedParts {
@@ -1140,15 +1152,16 @@ static void launch_bwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t
     }
     if (s->tiles[3] > 0) {
         if (one) CAPDEC_PACKED((packed_bwd_dkv_kernel<T, DH, 1, 1>), 5, p.Hkv, 64);
-        else if constexpr (sizeof(T) == 4) CAPDEC_PACKED((packed_bwd_dkv_kernel<T, DH, 2, 2>), 4, p.Hkv, 256);
         else {
             const PackedParts cut = packed_parts(s, p.Hkv, p.group);
             p.parts = cut.parts;
             p.slots = cut.slots;
             for (int l = 0; l < WALK_LEVELS; ++l) p.levels[l] = s->walk_levels[l];
-            p.part = (float*)((char*)p.stats + (size_t)p.Hq * p.stat_rows * 16);
+            p.part = (float*)((char*)p.delta + stat_bytes<T>(p.Hq, p.stat_rows));
             p.items = items_of(s, 4);
-            hipLaunchKernelGGL((packed16_bwd_dkv_kernel<DH, 2, 2>), dim3((unsigned)((s->tiles[4] - cut.items + cut.slots) * p.Hkv)), dim3(256), 0, st, p);
+            const dim3 grid((unsigned)((s->tiles[4] - cut.items + cut.slots) * p.Hkv));
+            if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((packed_bwd_dkv_kernel<T, DH, 2, 2>), grid, dim3(256), 0, st, p);
+            else hipLaunchKernelGGL((packed16_bwd_dkv_kernel<DH>), grid, dim3(256), 0, st, p);
             if (cut.parts > 1) hipLaunchKernelGGL((packed_join_kernel<T, DH>), dim3((unsigned)(cut.items * p.Hkv)), dim3(256), 0, st, p);
         }
     }
@@ -1159,8 +1172,7 @@ static void launch_bwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t
 // [delta or statistics][partial sums]
 extern "C" size_t capdec_attn_packed_scratch_bytes(const capdec_packed_seqs* seqs, size_t stat_rows, int Hq, int Hkv, int dh, int dtype) {
     if (packed_check("capdec_attn_packed_scratch_bytes", seqs, Hq, Hkv, dh, dtype, 1.f) || seqs->one_block) return 0;
-    if (dtype == CAPDEC_F32) return Hq * stat_rows * 4;
-    size_t bytes = Hq * stat_rows * 16;
+    size_t bytes = dtype == CAPDEC_F32 ? stat_bytes<float>(Hq, stat_rows) : stat_bytes<__bf16>(Hq, stat_rows);
     if (!short_rows(seqs->tiles + 3)) bytes += (size_t)packed_parts(seqs, Hkv, Hq / Hkv).slots * Hkv * 2 * 64 * dh * 4;
     return bytes;
 }

@@ -107,18 +107,19 @@ def _inputs(lq, lk, Hq, Hkv, dh, dtype, seed, extra=0):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lq, lk, causal, Hq, Hkv, dh", [([1500, 70], None, True, 8, 1, 64), ([900, 40, 1], [300, 7, 1000], False, 6, 2, 128),
                                                          ([1100] + [65] * 30, None, True, 4, 4, 128)])
-def test_long_walks_in_parts_match_float64(lq, lk, causal, Hq, Hkv, dh):
+def test_long_walks_in_parts_match_float64(dtype, lq, lk, causal, Hq, Hkv, dh):
     """Key tiles whose sums over the queries are cut into parts."""
     from imagecaption_amd import _capi
     ops = _ops()
-    q, k, v, do = _inputs(lq, lk or lq, Hq, Hkv, dh, torch.bfloat16, 500 + dh)
+    q, k, v, do = _inputs(lq, lk or lq, Hq, Hkv, dh, dtype, 500 + dh)
     scale = 1 / math.sqrt(dh)
-    ref = reference(q, k, v, do, lq, lk or lq, Hq, Hkv, causal, scale, E16)
+    ref = reference(q, k, v, do, lq, lk or lq, Hq, Hkv, causal, scale, E16 if dtype == torch.bfloat16 else 0.0)
     seqs = ops.PackedSeqs(lq, lk, causal=causal, device=DEV)
-    stats = 16 * Hq * sum(lq)
-    assert _capi.lib().capdec_attn_packed_scratch_bytes(seqs.cref, sum(lq), Hq, Hkv, dh, _capi.BF16S) > stats
+    stats = (16 if dtype == torch.bfloat16 else 4) * Hq * sum(lq) + 15
+    assert _capi.lib().capdec_attn_packed_scratch_bytes(seqs.cref, sum(lq), Hq, Hkv, dh, _capi.BF16S if dtype == torch.bfloat16 else 0) > stats
     o, lse = ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs)
     grads = ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs)
     for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):

@@ -8,8 +8,8 @@
 // A workgroup of NW waves owns NW x 32 rows of one head (a wave owns 32: one row on a lane and its partner lane ^ 32) and
 // walks the other side's rows in tiles that all its waves read from LDS; the next tile travels global -> registers while
 // the current one is multiplied.  Tiles come from a table made once per set of lengths on the host, longest first, so no
-// workgroup searches for its sequence and the tail of a launch is made of its shortest tiles.  Everything a row sums up
-// stays inside one workgroup: no atomics, bitwise reproducible.  The backward runs twice over the scores (dq by query
+// workgroup searches for its sequence and the tail of a launch is made of its shortest tiles.  What a row sums up
+// stays inside one workgroup, or is joined in a fixed order: no atomics, bitwise reproducible.  The backward runs twice over the scores (dq by query
 // tiles, dk / dv by key tiles and all heads of the group): 7 products instead of 5, in exchange for no fp32 gradient
 // block in memory and no order that depends on the launch.
 #include <algorithm>
@@ -1098,15 +1098,17 @@ static const PackedItem* items_of(const capdec_packed_seqs* s, int part) {
     } while (0)
 
 // One wave a tile where most sequences fit 32 rows: a taller tile would be half empty, and its waves would wait for each
-// other (256 captions of up to 20 tokens, bf16: forward 5.8 us against 9.9, dq 6.9 / 11.7, dk and dv 7.7 / 15.7; sequences
-// of 33 to 64 the other way, backward 46 / 34).
+// other (200 captions of 8 to 40 tokens, 8 heads of 64, bf16: forward 6.1 us against 8.8, backward 16 / 27, fp32 50 / 84; 64
+// sequences of 33 to 64, 16 heads of 128 over 4, the other way: 13 / 15, 32 / 51).
 static bool short_rows(const int* tiles) { return 2 * (int64_t)tiles[2] < 3 * (int64_t)tiles[1]; }
 
-// 128 rows a workgroup where that makes two for each of the 256 CUs (6 prompts, 16 heads of 128: 196 us against 265 with
-// 64 rows); 64 rows and two waves a block where it does not (one prompt of 2000: 46 / 55).  fp32: always the latter: 32
-// keys of fp32 already fill the LDS of a 64-key tile, and at 128 dims 128 rows spill (32 paragraphs 26 / 39, 8 texts 152 / 300).
+// 128 rows a workgroup where that makes five for every four of the 256 CUs (6 prompts, 16 heads of 128: forward 157 us
+// against 210 with 64 rows; 32 paragraphs, 8 heads of 128: 11.6 / 15.3, backward 37 / 43); 64 rows and two waves a block where it
+// does not (10 texts of 300 to 500 tokens, 8 heads of 64, 280 tall tiles: backward 25 / 27; one text of 2000, 256: 141 / 145).
+// fp32: always the latter: 32 keys of fp32 already fill the LDS of a 64-key tile, and at 128 dims 128 rows spill (32
+// paragraphs 26 / 39, 8 texts 152 / 300).
 template <typename T>
-static bool tall_rows(const int* tiles, int heads) { return sizeof(T) == 2 && (int64_t)tiles[0] * heads >= 512; }
+static bool tall_rows(const int* tiles, int heads) { return sizeof(T) == 2 && (int64_t)tiles[0] * heads >= 320; }
 
 // bytes of what dq leaves for dk / dv, whole 16-byte pieces
 template <typename T>
@@ -1114,8 +1116,10 @@ static size_t stat_bytes(int Hq, size_t stat_rows) {
     return sizeof(T) == 4 ? (Hq * stat_rows * 4 + 15) & ~(size_t)15 : Hq * stat_rows * 16;
 }
 
-// dk, dv of key tiles whose walk over the queries is much longer than a workgroup's even share (512 run at once) are summed in
-// parts by several workgroups and joined: PARTS_FIGURES
+// dk, dv of key tiles whose walk over the queries is longer than 5/4 of a workgroup's even share (512 run at once) are summed in
+// parts by several workgroups and joined in a second launch: such a walk would be running alone at the end (8 texts of 300 to
+// 4096 tokens, 16 heads of 128 over 4: 340 us in one piece, 242 and 13 for the join in parts; one text of 2000 over 2 heads,
+// the whole backward: 333 / 141).  With 3/4, 1/2, 1/4 of a share: 4, 8 and 23 % more for the first one's backward.  A part is at least 8 tiles.
 struct PackedParts {
     int parts, items, slots;  // of the longest tiles; tiles that are split, their parts together
 };

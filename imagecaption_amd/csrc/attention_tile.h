@@ -97,6 +97,29 @@ struct AttTile<__bf16, DH> {
 #pragma unroll
             for (int e = 0; e < 8; ++e) w.f[m][e] = (__bf16)x[8 * m + e];
     }
+    // weights that keep 16 bits: the rounded ones and what the rounding left, added by products of their own
+    struct weights2 { weights hi, lo; };
+    __device__ static __forceinline__ void pack(weights2& w, const float* x) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w.hi.f[m][e] = (__bf16)x[8 * m + e];
+                w.lo.f[m][e] = (__bf16)(x[8 * m + e] - (float)w.hi.f[m][e]);
+            }
+    }
+    __device__ static __forceinline__ void mma_cols(f32x16* out, const unsigned char* img, const lanes& l, const weights2& w) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+                const bf16x4t lo = read_tr(img + m * 16 * ROWB + (l.col[0] ^ (dt << 6)));
+                const bf16x4t hi = read_tr(img + m * 16 * ROWB + (l.col[1] ^ (dt << 6)));
+                const bf16x8t a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.lo.f[m], out[dt], 0, 0, 0);
+                out[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.hi.f[m], out[dt], 0, 0, 0);
+            }
+    }
     __device__ static __forceinline__ bf16x4t read_tr(const unsigned char* p) {
         typedef __attribute__((address_space(3))) bf16x4t lds4;
         return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)p);
@@ -152,6 +175,7 @@ struct AttTile<float, DH> {
     static constexpr int ES = 4, ROWB = DH * ES, PPR = ROWB / 16, EPP = 4, NF = DH / 8, NDT = DH / 32;
     typedef f32x4t frag;  // elements 8 i + 4 half + 0..3: four 2-deep products take one element of each half-wave
     struct weights { float f[16]; };
+    typedef weights weights2;
     struct lanes { int l31, half; };
     __device__ static __forceinline__ int swz(int r) { return r & 15; }
     __device__ static __forceinline__ lanes make_lanes(int lane) { return lanes{lane & 31, lane >> 5}; }

@@ -358,8 +358,8 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
  *   bwd: dq, dk, dv from do; dk / dv sum over the query heads of their group.  No atomics: bitwise reproducible.
  *   scale between 2^-60 and 2^60.  Results must not overlap the matrices that are read; fewer than 2^31 - 1024 rows a side.
  * dtype CAPDEC_F32: every matrix fp32, exact fp32 products; CAPDEC_BF16S: every matrix bf16, fp32 accumulation, softmax and
- * statistics, probabilities and score gradients rounded to bf16 for the products that take them (the only roundings
- * besides the results').  dh in {64, 128}; 16-byte aligned matrices, row strides multiples of 16 bytes, at most 2^25 bytes.  Non-finite values:
+ * statistics, probabilities and score gradients rounded to bf16 for the products that take them (to 16 bits, two bf16 terms,
+ * where most sequences fit 32 rows), the only roundings besides the results'.  dh in {64, 128}; 16-byte aligned matrices, row strides multiples of 16 bytes, at most 2^25 bytes.  Non-finite values:
  * the products are plain ones (0 x inf = NaN), so an infinity or NaN in v reaches the rows of ITS sequence that share a
  * tile with it even where they are masked; it never reaches another sequence.
  * The plan: capdec_packed_plan checks the lengths (host arrays; lens_k = NULL: the same as lens_q), writes the tile table to
@@ -404,7 +404,8 @@ int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ld
  *   bf16 matrices with the new tokens of all sequences back to back: sequence s owns the rows cu_q[s] .. cu_q[s + 1] - 1 (cu_q
  *   NULL: one token each, row s).  max_q is the largest nq (a hint: more rows are still computed, more slowly).  Query head h
  *   reads key / value head h / (Hq / heads).  Products in bf16 with fp32 accumulation, softmax in fp32; weights are rounded
- *   to bf16 for the context product (after the value's scale is multiplied in), the result once.  A token that sees nothing
+ *   to bf16 for the context product (after the value's scale is multiplied in; to 16 bits, two bf16 terms, up to 64 rows a key /
+ *   value head), the result once.  A token that sees nothing
  *   gets o = 0, lse = -inf; lse (fp32 [Hq, rows]) may be NULL.  Rows of no sequence stay as they are in lse,
  *   and in o too unless `clear` is set: then they get zeros.  scale between 2^-60 and 2^60.  Positions past kv_lens are never read, whatever their slots hold; an infinity or NaN among the values of
  *   a seen position reaches the new tokens of ITS sequence that do not see it yet as well (0 x inf), no other sequence.

@@ -162,10 +162,13 @@ SIGNATURES = {
 }
 
 _lib = None
+fast = None  # the direct calls of ops.py's packed / paged entry points (csrc/calls.cpp), where they are built
+_DIRECT = ("attn_packed_fwd", "attn_packed_scratch_bytes", "attn_packed_bwd", "kv_write", "kv_read", "attn_paged_workspace_bytes",
+           "attn_paged", "draft_verify")
 
 
 def lib():
-    global _lib
+    global _lib, fast
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(
@@ -176,6 +179,14 @@ def lib():
             fn = getattr(l, name)  # AttributeError if the .so does not export a declared symbol
             fn.restype, fn.argtypes = res, args
         _lib = l
+        if _raw_stream is not None:
+            try:
+                from . import _calls
+            except ImportError:  # not built, or built for another torch: the same calls through ctypes, at more host time
+                pass
+            else:
+                _calls.bind(*(C.cast(getattr(l, "capdec_" + n), C.c_void_p).value for n in _DIRECT))
+                fast = _calls
     return _lib
 
 

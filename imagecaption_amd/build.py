@@ -14,6 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "_build")
 LIB = os.path.join(HERE, "libcapdec.so")
+CALLS = os.path.join(HERE, "_calls.so")
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 -- some of their operand forms have given wrong results on this hardware now
 # and then, and -O3 makes them from ordinary float code.  (The host pass does not know the feature and says so: harmless.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Wall", "-Wno-unused-function",
@@ -86,7 +87,28 @@ def build(force=False, verbose=True):
             raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
         if verbose:
             print(f"[capdec build] linked {LIB}")
+    build_calls(force, verbose)
     return LIB
+
+
+def build_calls(force=False, verbose=True):
+    """csrc/calls.cpp -> _calls.so: host code only, built against the installed torch."""
+    import sysconfig
+    import torch
+    src = os.path.join(CSRC, "calls.cpp")
+    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), _deps_mtime()):
+        return
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += ["-isystem" + i for i in inc] + [src, "-o", CALLS, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stderr[-4000:]}")
+    if verbose:
+        if r.stderr.strip():
+            print(r.stderr[-2000:], file=sys.stderr)
+        print(f"[capdec build] linked {CALLS}")
 
 
 if __name__ == "__main__":

@@ -952,7 +952,7 @@ class PackedSeqs:
             raise _capi.CapdecError("PackedSeqs: the blocking copy of its table cannot be captured; make it before the capture")
         self.table = torch.empty(l.capdec_packed_table_bytes(cq, ck, n), dtype=torch.uint8, device=device)
         self.c = _capi.PackedSeqs()
-        self.cref = C.byref(self.c)
+        self.cref, self.at, self.index = C.byref(self.c), C.addressof(self.c), self.table.get_device()
         with torch.cuda.device(self.table.device):
             self.stream = stream()
             # the block may have belonged to a tensor that work queued on this stream still writes
@@ -1034,6 +1034,14 @@ def attn_packed_fwd(q, k, v, Hq, Hkv, seqs, out=None, save_lse=True, scale=None)
     """Attention over packed sequences: q [>= rows_q, Hq * dh], k / v [>= rows_k, Hkv * dh] (row-strided views, all fp32 or
     all bf16, dh 64 or 128), ``seqs`` a PackedSeqs.  Returns (o, lse [Hq, rows of q] or None).  Rows behind the last sequence
     stay as they are in a given ``out`` (which must not overlap q, k or v) and are zeros in a new one."""
+    fast = _capi.fast
+    if fast is not None and out is None:
+        cur = _capi._cur_device()
+        st = _capi._raw_stream(cur)
+        if cur == seqs.index and st == seqs.stream:
+            done = fast.attn_packed_fwd(seqs.at, q, k, v, Hq, Hkv, save_lse, scale, cur, st)
+            if done is not None:
+                return done
     dh, cur, dtype, scale, (pq, lq), (pk, lk), (pv, lv) = _packed_args("attn_packed_fwd", q, k, v, Hq, Hkv, seqs, scale)
     rows, n = q.shape[0], seqs.rows_q
     if out is None:
@@ -1054,6 +1062,14 @@ def attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dq=None, dk=None, dv=Non
     """(dq, dk, dv) of attn_packed_fwd; ``o`` / ``lse`` are its results, ``do`` the gradient of o.  Given dq / dk / dv are
     written in place (they must not overlap the other matrices), rows behind the last sequence stay as they are there and are
     zeros in new ones."""
+    fast = _capi.fast
+    if fast is not None and dq is None and dk is None and dv is None:
+        cur = _capi._cur_device()
+        st = _capi._raw_stream(cur)
+        if cur == seqs.index and st == seqs.stream:
+            done = fast.attn_packed_bwd(seqs.at, q, k, v, Hq, Hkv, o, do, lse, scale, cur, st)
+            if done is not None:
+                return done
     name = "attn_packed_bwd"
     dh, cur, dtype, scale, (pq, lq), (pk, lk), (pv, lv) = _packed_args(name, q, k, v, Hq, Hkv, seqs, scale)
     dt, n, nk, wide, narrow = q.dtype, seqs.rows_q, seqs.rows_k, Hq * dh, Hkv * dh
@@ -1109,7 +1125,7 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page, self.dh = pages, heads, page, dh
         self.c = _capi.KVCache(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, heads, page, dh, _capi.E4M3 if e4m3 else _capi.BF16S)
-        self.cref = C.byref(self.c)
+        self.cref, self.at, self.index = C.byref(self.c), C.addressof(self.c), k.get_device()
 
     @classmethod
     def new(cls, pages, heads, page, dh, dtype=torch.bfloat16, device="cuda"):
@@ -1153,6 +1169,11 @@ def kv_cache_write(cache, k, v, slots):
     """Row r of k / v ([>= rows, heads * dh], fp32 or bf16, row-strided views) into slot ``slots[r]`` (int32 [rows]; negative:
     skipped) of a PagedKVCache, rounded to e4m3 with a scale of its own for each head where the cache holds e4m3.  The slots of
     one call must differ."""
+    fast = _capi.fast
+    if fast is not None:
+        cur = _capi._cur_device()
+        if cur == cache.index and fast.kv_cache_write(cache.at, k, v, slots, cur, _capi._raw_stream(cur)):
+            return
     rows, dtype, pk, lk, pv, lv, ps = _cache_rows("kv_cache_write", cache, k, v, slots)
     check(lib().capdec_kv_write(cache.cref, pk, lk, pv, lv, dtype, ps, rows, stream()), "capdec_kv_write")
 
@@ -1160,6 +1181,13 @@ def kv_cache_write(cache, k, v, slots):
 def kv_cache_read(cache, slots, k=None, v=None, dtype=torch.bfloat16):
     """(k, v): the rows of ``slots`` (int32 [rows]; negative: zeros) as [rows, heads * dh] matrices of ``dtype`` (or into given
     ones, both of one type)."""
+    fast = _capi.fast
+    if fast is not None and k is None and v is None and dtype in _ES:
+        cur = _capi._cur_device()
+        if cur == cache.index:
+            done = fast.kv_cache_read(cache.at, slots, dtype is torch.bfloat16, cur, _capi._raw_stream(cur))
+            if done is not None:
+                return done
     if k is None:
         shape = (slots.numel(), cache.heads * cache.dh)
         k = cache.k.new_empty(shape, dtype=dtype if v is None else v.dtype)
@@ -1184,6 +1212,13 @@ def attn_paged(q, cache, page_table, kv_lens, Hq, cu_q=None, max_q=1, out=None, 
     None: one each), at most ``max_q``; kv_lens int32 [n]: positions of each sequence with the new ones; page_table int32
     [n, columns].  Causal: new token i of nq sees the positions up to kv_lens - nq + i.  Returns o (rows of no sequence stay as
     they are in a given ``out`` and are zeros in a new one), or (o, lse [Hq, rows]).  ``out`` must not overlap q or the cache."""
+    fast = _capi.fast
+    if fast is not None and out is None and not return_lse:
+        cur = _capi._cur_device()
+        if cur == cache.index:
+            done = fast.attn_paged(cache.at, q, page_table, kv_lens, Hq, cu_q, max_q, scale, cur, _capi._raw_stream(cur))
+            if done is not None:
+                return done
     name = "attn_paged"
     n, cur, dh, heads = kv_lens.numel(), _here(name, q), cache.dh, cache.heads
     if Hq <= 0 or Hq % heads or max_q <= 0:
@@ -1221,6 +1256,12 @@ def draft_verify(target, draft, tokens, u_accept, u_sample, num_draft=None, pad=
     (None: a drafter sure of its tokens), fp32 probabilities with unit stride along the vocabulary; tokens int64 [n, drafts];
     u_accept [n, drafts] / u_sample [n] uniforms in [0, 1); num_draft int32 [n] (None: all).  Returns (out int64
     [n, drafts + 1]: accepted tokens, the drawn one, then ``pad``; accepted int32 [n])."""
+    fast = _capi.fast
+    if fast is not None and target.is_cuda:
+        cur = _capi._cur_device()
+        done = fast.draft_verify(target, draft, tokens, u_accept, u_sample, num_draft, pad, cur, _capi._raw_stream(cur))
+        if done is not None:
+            return done
     name, f32 = "draft_verify", torch.float32
     cur = _here(name, target)
     if target.dim() != 3 or target.shape[1] == 0 or target.shape[2] == 0:

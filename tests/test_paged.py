@@ -513,6 +513,82 @@ def test_prompt_cache_drafts_and_verification_together(dtype):
 
 
 # ---- refusals -------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_direct_and_general_calls_agree(monkeypatch):
+    """The direct calls (csrc/calls.cpp) take the plain forms and do what the general way through ctypes does."""
+    from imagecaption_amd import _capi
+    ops = _ops()
+    _capi.lib()
+    assert _capi.fast is not None
+    g = torch.Generator().manual_seed(7)
+    rand = lambda *shape, dtype=BF16: torch.randn(*shape, generator=g).to(dtype).to(DEV)
+    taken = []
+
+    class Counted:
+        def __getattr__(self, name):
+            call = getattr(direct, name)
+
+            def counted(*args):
+                done = call(*args)
+                taken.append((name, done is not None))
+                return done
+            return counted
+
+    direct = _capi.fast
+    seqs = {n: ops.PackedSeqs(lens, device=DEV) for n, lens in (("long", [70, 200, 1]), ("short", [9, 20, 32]))}
+    wide = rand(271, 3 * 256)
+    probs = torch.rand(3, 4, 50, generator=g).to(DEV)
+    tokens, u, us = torch.randint(0, 50, (3, 3), generator=g).to(DEV), torch.rand(3, 3, generator=g).to(DEV), torch.rand(3, generator=g).to(DEV)
+    table = torch.arange(12, dtype=torch.int32).view(3, 4).to(DEV)
+    lens, cu = torch.tensor([60, 3, 17], dtype=torch.int32, device=DEV), torch.tensor([0, 2, 3, 6], dtype=torch.int32, device=DEV)
+
+    def everything():
+        out = []
+        for dtype in (BF16, torch.float32):
+            for name, rows in (("long", 271), ("short", 61)):
+                x = wide[:rows].to(dtype)
+                q, k, v = x[:, :256], x[:, 256:384], x[:, 384:512]
+                for scale in (None, 0.3):
+                    o, lse = ops.attn_packed_fwd(q, k, v, 4, 2, seqs[name], scale=scale)
+                    out += [o, lse, *ops.attn_packed_bwd(q, k, v, o, x[:, 512:], lse, 4, 2, seqs[name], scale=scale)]
+                o, lse = ops.attn_packed_fwd(q, k, v, 4, 2, seqs[name], save_lse=False)
+                assert lse is None
+                out.append(o)
+        for dtype in (BF16, E4M3):
+            cache = ops.PagedKVCache(*(torch.zeros(12, 2, 16, 64, dtype=torch.uint8 if dtype == E4M3 else dtype, device=DEV).view(dtype)
+                                       for _ in range(2)),
+                                     *((torch.zeros(12, 2, 16, device=DEV) for _ in range(2)) if dtype == E4M3 else ()))
+            slots = torch.arange(192, dtype=torch.int32, device=DEV)
+            ops.kv_cache_write(cache, wide[:192, :128], wide[:192, 128:256], slots)
+            ops.kv_cache_write(cache, wide[:5, :128].float(), wide[:5, 128:256].float(), slots[100:105])
+            out += [*ops.kv_cache_read(cache, slots), *ops.kv_cache_read(cache, slots[7:8], dtype=torch.float32)]
+            out += [ops.attn_paged(wide[:6, :256], cache, table, lens, 4, cu_q=cu, max_q=3),
+                    ops.attn_paged(wide[:5, :512], cache, table, lens, 8, scale=0.2)]
+        out += [*ops.draft_verify(probs, probs[:, 1:], tokens, u, us, pad=-1), *ops.draft_verify(probs, None, tokens, u, us, num_draft=lens)]
+        return out
+
+    monkeypatch.setattr(_capi, "fast", Counted())
+    with_direct = everything()
+    assert all(done for _, done in taken) and {n for n, _ in taken} == {"attn_packed_fwd", "attn_packed_bwd", "kv_cache_write", "kv_cache_read",
+                                                                        "attn_paged", "draft_verify"}
+    monkeypatch.setattr(_capi, "fast", None)
+    general = everything()
+    assert len(general) == len(with_direct) and all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(general, with_direct))
+
+
+def test_direct_calls_leave_what_they_do_not_know():
+    from imagecaption_amd import _capi
+    _capi.lib()
+    if _capi.fast is None:
+        pytest.skip("the direct calls are not built")
+    x, y = torch.zeros(3, 64), [None] * 12
+    assert _capi.fast.attn_packed_fwd(*y[:10]) is None and _capi.fast.attn_packed_bwd(*y) is None and _capi.fast.kv_cache_write(*y[:6]) is None
+    assert _capi.fast.kv_cache_read(*y[:5]) is None and _capi.fast.attn_paged(*y[:10]) is None and _capi.fast.draft_verify(*y[:9]) is None
+    assert _capi.fast.draft_verify(x, None, x, x, x, None, 0, 0, 0) is None and _capi.fast.kv_cache_write() is None
+    with pytest.raises(TypeError):
+        _capi.fast.bind(1, 2)
+
+
 def test_arguments_are_refused_without_a_gpu():
     from imagecaption_amd import _capi
     from imagecaption_amd._capi import CapdecError

@@ -20,8 +20,7 @@ namespace capdec {
 static __device__ unsigned int g_bad_pages;
 static __device__ uint4 g_zero_row[16];  // stands in for the rows of positions that do not exist
 
-constexpr int SPLIT_PAGES = 512;  // most pages of a split: their offsets fit LDS
-constexpr int SPLIT_IDS = SPLIT_PAGES + 2;
+constexpr int WINDOW = 512;       // pages whose offsets are in LDS at a time
 constexpr int SPLIT_MIN = 512;    // fewest keys worth a split of their own (and a second launch)
 constexpr int SPLIT_WANT = 512;   // workgroups to aim at: two for each of the 256 CUs, which is what they hold
 
@@ -51,7 +50,6 @@ __device__ __forceinline__ int split_size(const PagedParams& p, int64_t work, in
     const int64_t share = (work * p.Hkv + room - 1) / room;
     int c = max((int)min(share, (int64_t)(1 << 30)), (len + p.splits - 1) / p.splits);
     c = max(c, SPLIT_MIN);
-    c = min(c, (SPLIT_PAGES << p.page_log2) - 128);
     return (c + 127) & ~127;
 }
 
@@ -187,12 +185,20 @@ __device__ __forceinline__ void clear_rest(const PagedParams& p, int tid) {
     for (int64_t row = (int64_t)end + blockIdx.x; row < p.rows; row += gridDim.x) zero((int)row);
 }
 
-// the split's pages into LDS, as byte offsets of this head's first row there; pages outside the cache become -1
-// and are counted; *bad tells that there are some
-__device__ __forceinline__ void load_pages(int64_t* pages, int* bad, const PagedParams& p, const PagedItem& w, int row_bytes, int tid, int nt) {
+// end of the window of pages that begins at key k0: whole pages, and a multiple of 128 keys from k0 unless it is kend
+__device__ __forceinline__ int window_end(const PagedParams& p, int k0, int kend) {
+    const int64_t e = ((int64_t)(k0 >> p.page_log2) + WINDOW) << p.page_log2;
+    return (int)min(e, (int64_t)kend);
+}
+
+// the pages of the keys k0 .. kend - 1 (one window) into LDS, as byte offsets of this head's first row there; pages outside the
+// cache become -1 and are counted; *bad tells that there are some.  The caller waits for the workgroup before it uses them.
+__device__ __forceinline__ void load_pages(int64_t* pages, int* bad, const PagedParams& p, const PagedItem& w, int k0, int kend, int row_bytes, int tid,
+                                           int nt) {
+    __syncthreads();  // the window before is no longer read
     if (tid == 0) *bad = 0;
     __syncthreads();
-    const int first = w.kbegin >> p.page_log2, n = w.kend > w.kbegin ? ((w.kend - 1) >> p.page_log2) - first + 1 : 0;
+    const int first = k0 >> p.page_log2, n = kend > k0 ? ((kend - 1) >> p.page_log2) - first + 1 : 0;
     const int* row = p.table + (size_t)w.seq * p.ld_table + first;
     for (int i = tid; i < n; i += nt) {
         const int id = row[i];
@@ -332,7 +338,7 @@ __global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2
     using L = AttTile<__bf16, DH>;
     constexpr int IMG = 32 * L::ROWB;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[(4 + R) * IMG];
-    __shared__ int64_t pages[SPLIT_IDS];
+    __shared__ int64_t pages[WINDOW];
     __shared__ int s_bad;
     __shared__ __attribute__((aligned(16))) float sc[4][2][32];
     __shared__ float ml[4][2][32];
@@ -353,8 +359,6 @@ __global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2
         }
     };
     load_rows(w.tile);  // (on their way while the page table is read)
-    load_pages(pages, &s_bad, p, w, E4M3 ? DH : 2 * DH, tid, 256);
-    const int first_page = w.kbegin >> p.page_log2;
     const typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
     unsigned char* Vs = smem + wave * IMG;
@@ -379,73 +383,78 @@ __global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2
 #pragma unroll
             for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[b][dt]);
         }
-        __syncthreads();  // pages, rows
-        const bool good = s_bad == 0;
-        KeyFrags<E4M3, DH> kf;
-        PageStage<E4M3, DH, 64, 32, false> st;
-        int k0 = w.kbegin + wave * 32;
-        if (k0 < w.kend) {
-            kf.load(p, pages, first_page, k0 + l31, w.kend, half);
-            st.load(p, pages, first_page, k0, w.kend, lane);
-        }
-        for (; k0 < w.kend; k0 += 128) {
-            f32x16 s[R];
+        for (int win = w.kbegin, wend; win < w.kend; win = wend) {
+            wend = window_end(p, win, w.kend);
+            load_pages(pages, &s_bad, p, w, win, wend, E4M3 ? DH : 2 * DH, tid, 256);
+            __syncthreads();  // pages, rows
+            const bool good = s_bad == 0;
+            const int first_page = win >> p.page_log2;
+            KeyFrags<E4M3, DH> kf;
+            PageStage<E4M3, DH, 64, 32, false> st;
+            int k0 = win + wave * 32;
+            if (k0 < wend) {
+                kf.load(p, pages, first_page, k0 + l31, wend, half);
+                st.load(p, pages, first_page, k0, wend, lane);
+            }
+            for (; k0 < wend; k0 += 128) {
+                f32x16 s[R];
 #pragma unroll
-            for (int b = 0; b < R; ++b) {
-                zero16(s[b]);
-                kf.mma(s[b], Qs + b * IMG + l31 * L::ROWB, L::swz(l31), half);  // S^T[key][row]
-            }
-            // one wave's LDS operations execute in order: the previous run's reads are done before these writes land
-            if (E4M3 && half == 0) {
-                sc[wave][0][l31] = kf.sk;
-                sc[wave][1][l31] = kf.sv;
-            }
-            st.put(Vs, st.v, lane);
-            if (k0 + 128 < w.kend) {
-                kf.load(p, pages, first_page, k0 + 128 + l31, w.kend, half);
-                st.load(p, pages, first_page, k0 + 128, w.kend, lane);
-            }
-            wave_fence();
+                for (int b = 0; b < R; ++b) {
+                    zero16(s[b]);
+                    kf.mma(s[b], Qs + b * IMG + l31 * L::ROWB, L::swz(l31), half);  // S^T[key][row]
+                }
+                // one wave's LDS operations execute in order: the previous run's reads are done before these writes land
+                if (E4M3 && half == 0) {
+                    sc[wave][0][l31] = kf.sk;
+                    sc[wave][1][l31] = kf.sv;
+                }
+                st.put(Vs, st.v, lane);
+                if (k0 + 128 < wend) {
+                    kf.load(p, pages, first_page, k0 + 128 + l31, wend, half);
+                    st.load(p, pages, first_page, k0 + 128, wend, lane);
+                }
+                wave_fence();
 #pragma unroll
-            for (int b = 0; b < R; ++b) {
-                if constexpr (E4M3) {
+                for (int b = 0; b < R; ++b) {
+                    if constexpr (E4M3) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const f32x4t f = *reinterpret_cast<const f32x4t*>(&sc[wave][0][8 * i + 4 * half]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) s[b][4 * i + j] *= f[j];
+                        }
+                    }
+                    if (!good || k0 + 32 > all_see) hide(s[b], p, pages, first_page, k0, see[b], good, half);
+                    float top = s[b][0];
+#pragma unroll
+                    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[b][r]);
+                    bool raised;
+                    const float a = run[b].raise(top, c, &raised);
+                    if (raised) {
+#pragma unroll
+                        for (int dt = 0; dt < L::NDT; ++dt)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) acc[b][dt][r] *= a;
+                    }
+                    const float base = run[b].base();
+                    float x[16];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const f32x4t f = *reinterpret_cast<const f32x4t*>(&sc[wave][0][8 * i + 4 * half]);
+                        f32x4t f = {1.f, 1.f, 1.f, 1.f};
+                        if constexpr (E4M3) f = *reinterpret_cast<const f32x4t*>(&sc[wave][1][8 * i + 4 * half]);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) s[b][4 * i + j] *= f[j];
+                        for (int j = 0; j < 4; ++j) {
+                            const float e = exp2_fast(__fmaf_rn(s[b][4 * i + j], c, -base));
+                            run[b].l += e;
+                            x[4 * i + j] = E4M3 ? e * f[j] : e;
+                        }
                     }
+                    typename L::weights2 pw;
+                    L::pack(pw, x);
+                    L::mma_cols(acc[b], Vs, ln, pw);
                 }
-                if (!good || k0 + 32 > all_see) hide(s[b], p, pages, first_page, k0, see[b], good, half);
-                float top = s[b][0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[b][r]);
-                bool raised;
-                const float a = run[b].raise(top, c, &raised);
-                if (raised) {
-#pragma unroll
-                    for (int dt = 0; dt < L::NDT; ++dt)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[b][dt][r] *= a;
-                }
-                const float base = run[b].base();
-                float x[16];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    f32x4t f = {1.f, 1.f, 1.f, 1.f};
-                    if constexpr (E4M3) f = *reinterpret_cast<const f32x4t*>(&sc[wave][1][8 * i + 4 * half]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float e = exp2_fast(__fmaf_rn(s[b][4 * i + j], c, -base));
-                        run[b].l += e;
-                        x[4 * i + j] = E4M3 ? e * f[j] : e;
-                    }
-                }
-                typename L::weights2 pw;
-                L::pack(pw, x);
-                L::mma_cols(acc[b], Vs, ln, pw);
+                wave_fence();
             }
-            wave_fence();
         }
         // join the four waves: statistics first, then the contexts, half the dims at a time, through their (now free) images
 #pragma unroll
@@ -525,7 +534,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     using L = AttTile<__bf16, DH>;
     constexpr int KB = 2, BN = 32 * KB, IMG = BN * L::ROWB;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
-    __shared__ int64_t pages[SPLIT_IDS];
+    __shared__ int64_t pages[WINDOW];
     __shared__ int s_bad;
     __shared__ __attribute__((aligned(16))) float sc[2][2][BN];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
@@ -533,10 +542,6 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     clear_rest<DH>(p, tid);
     if (!w.ok) return;
     const int nrows = w.nq * p.group;
-    load_pages(pages, &s_bad, p, w, E4M3 ? DH : 2 * DH, tid, 256);
-    __syncthreads();
-    const bool good = s_bad == 0;
-    const int first_page = w.kbegin >> p.page_log2;
     const typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
     for (int tile = w.tile; tile * 128 < nrows; tile += w.step) {
@@ -545,7 +550,6 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
         const int all_see = min(w.kend, w.len - w.nq + r0 / p.group + 1);
         const int wave_end = r0 < nrows ? min(w.kend, w.len - w.nq + min(r0 + 31, nrows - 1) / p.group + 1) : 0;
         const int end = min(w.kend, w.len - w.nq + min(tile * 128 + 127, nrows - 1) / p.group + 1);
-        const int nt = end > w.kbegin ? (end - w.kbegin + BN - 1) / BN : 0;
         typename L::frag qf[L::NF];
         L::load_row(qf, p.q + (size_t)(w.a + token) * p.ldq + head * DH, r < nrows, half);
         f32x16 acc[L::NDT];
@@ -553,134 +557,138 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
         for (int dt = 0; dt < L::NDT; ++dt) zero16(acc[dt]);
         Running run;
         run.init();
-        PageStage<E4M3, DH, 256, BN, true> st;
-        float sk, sv;
-        // tile t into the images at img: by DMA at once, or into registers (put stores them)
-        auto fetch = [&](int t, unsigned char* img) {
-            const int k0 = w.kbegin + t * BN;
-            if constexpr (E4M3) {
-                st.load(p, pages, first_page, k0, w.kend, tid);
-                if (tid < BN) key_scales<DH>(p, pages, first_page, k0 + tid, w.kend, sk, sv);
-            } else {
-                constexpr int PER = 64 / L::PPR, N = BN / PER / 4;  // rows of a 1 KiB transfer, transfers of a wave
-                const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(
-                    (int)(unsigned)(size_t)(const __attribute__((address_space(3))) unsigned char*)(img + wave * N * 1024));
-                const int mask = (1 << p.page_log2) - 1;
-                int64_t at[N];
-                unsigned within[N];
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const int rl = (wave * N + j) * PER + lane / L::PPR, key = min(k0 + rl, w.kend - 1);
-                    at[j] = pages[(key >> p.page_log2) - first_page];
-                    within[j] = (unsigned)((key & mask) * L::ROWB) + (((unsigned)(lane % L::PPR)) ^ (unsigned)L::swz(rl & 31)) * 16u;
-                }
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const unsigned char* ka = (const unsigned char*)p.k + at[j] + within[j];
-                    const unsigned char* va = (const unsigned char*)p.v + at[j] + within[j];
-                    if (!good && at[j] < 0) ka = va = reinterpret_cast<const unsigned char*>(g_zero_row) + within[j] % L::ROWB;
-                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + j * 1024), "v"(ka) : "memory");
-                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + IMG + j * 1024), "v"(va) : "memory");
-                }
-            }
-        };
-        auto put = [&](int t, unsigned char* img) {
-            if constexpr (E4M3) {
-                st.put(img, st.k, tid);
-                st.put(img + IMG, st.v, tid);
-                if (tid < BN) {
-                    sc[t & 1][0][tid] = sk;
-                    sc[t & 1][1][tid] = sv;
-                }
-            }
-        };
-        auto turn = [&](int t, unsigned char* cur, unsigned char* nx) __attribute__((always_inline)) {
-            const unsigned char* Ks = cur;
-            const unsigned char* Vs = Ks + IMG;
-            const bool more = t + 1 < nt;
-            if constexpr (!E4M3) dma_sync();
-            if (more) fetch(t + 1, nx);
-            __builtin_amdgcn_sched_barrier(0);
-            const int k0 = w.kbegin + t * BN;
-            if (k0 < wave_end) {
-                f32x16 s[KB];
-                bf16x8t kf[KB][L::NF], vf[2 * L::NDT];
-#pragma unroll
-                for (int b = 0; b < KB; ++b) L::read_rows(kf[b], Ks + b * 32 * L::ROWB, ln);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int b = 0; b < KB; ++b) zero16(s[b]);
-#pragma unroll
-                for (int ks = 0; ks < L::NF; ++ks)
-#pragma unroll
-                    for (int b = 0; b < KB; ++b) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b][ks], qf[ks], s[b], 0, 0, 0);  // S^T[key][row]
-                L::read_cols(vf, Vs, ln);
-                __builtin_amdgcn_sched_barrier(0);
+        landed(qf);
+        for (int win = w.kbegin, wend; win < end; win = wend) {
+            wend = window_end(p, win, w.kend);
+            load_pages(pages, &s_bad, p, w, win, wend, E4M3 ? DH : 2 * DH, tid, 256);  // (the images are free from here on, too)
+            __syncthreads();
+            const bool good = s_bad == 0;
+            const int first_page = win >> p.page_log2, nt = (min(end, wend) - win + BN - 1) / BN;
+            PageStage<E4M3, DH, 256, BN, true> st;
+            float sk, sv;
+            // tile t into the images at img: by DMA at once, or into registers (put stores them)
+            auto fetch = [&](int t, unsigned char* img) {
+                const int k0 = win + t * BN;
                 if constexpr (E4M3) {
+                    st.load(p, pages, first_page, k0, wend, tid);
+                    if (tid < BN) key_scales<DH>(p, pages, first_page, k0 + tid, wend, sk, sv);
+                } else {
+                    constexpr int PER = 64 / L::PPR, N = BN / PER / 4;  // rows of a 1 KiB transfer, transfers of a wave
+                    const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane(
+                        (int)(unsigned)(size_t)(const __attribute__((address_space(3))) unsigned char*)(img + wave * N * 1024));
+                    const int mask = (1 << p.page_log2) - 1;
+                    int64_t at[N];
+                    unsigned within[N];
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const int rl = (wave * N + j) * PER + lane / L::PPR, key = min(k0 + rl, wend - 1);
+                        at[j] = pages[(key >> p.page_log2) - first_page];
+                        within[j] = (unsigned)((key & mask) * L::ROWB) + (((unsigned)(lane % L::PPR)) ^ (unsigned)L::swz(rl & 31)) * 16u;
+                    }
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const unsigned char* ka = (const unsigned char*)p.k + at[j] + within[j];
+                        const unsigned char* va = (const unsigned char*)p.v + at[j] + within[j];
+                        if (!good && at[j] < 0) ka = va = reinterpret_cast<const unsigned char*>(g_zero_row) + within[j] % L::ROWB;
+                        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + j * 1024), "v"(ka) : "memory");
+                        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to + IMG + j * 1024), "v"(va) : "memory");
+                    }
+                }
+            };
+            auto put = [&](int t, unsigned char* img) {
+                if constexpr (E4M3) {
+                    st.put(img, st.k, tid);
+                    st.put(img + IMG, st.v, tid);
+                    if (tid < BN) {
+                        sc[t & 1][0][tid] = sk;
+                        sc[t & 1][1][tid] = sv;
+                    }
+                }
+            };
+            auto turn = [&](int t, unsigned char* cur, unsigned char* nx) __attribute__((always_inline)) {
+                const unsigned char* Ks = cur;
+                const unsigned char* Vs = Ks + IMG;
+                const bool more = t + 1 < nt;
+                if constexpr (!E4M3) dma_sync();
+                if (more) fetch(t + 1, nx);
+                __builtin_amdgcn_sched_barrier(0);
+                const int k0 = win + t * BN;
+                if (k0 < wave_end) {
+                    f32x16 s[KB];
+                    bf16x8t kf[KB][L::NF], vf[2 * L::NDT];
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) L::read_rows(kf[b], Ks + b * 32 * L::ROWB, ln);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) zero16(s[b]);
+#pragma unroll
+                    for (int ks = 0; ks < L::NF; ++ks)
+#pragma unroll
+                        for (int b = 0; b < KB; ++b) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[b][ks], qf[ks], s[b], 0, 0, 0);  // S^T[key][row]
+                    L::read_cols(vf, Vs, ln);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (E4M3) {
+#pragma unroll
+                        for (int b = 0; b < KB; ++b)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const f32x4t f = *reinterpret_cast<const f32x4t*>(&sc[t & 1][0][32 * b + 8 * i + 4 * half]);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) s[b][4 * i + j] *= f[j];
+                            }
+                    }
+                    if (!good || k0 + BN > all_see) {
+#pragma unroll
+                        for (int b = 0; b < KB; ++b) hide(s[b], p, pages, first_page, k0 + 32 * b, see, good, half);
+                    }
+                    float top = s[0][0];
 #pragma unroll
                     for (int b = 0; b < KB; ++b)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const f32x4t f = *reinterpret_cast<const f32x4t*>(&sc[t & 1][0][32 * b + 8 * i + 4 * half]);
+                        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+                    bool raised;
+                    const float a = run.raise(top, c, &raised);
+                    if (raised) {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) s[b][4 * i + j] *= f[j];
-                        }
-                }
-                if (!good || k0 + BN > all_see) {
+                        for (int dt = 0; dt < L::NDT; ++dt)
 #pragma unroll
-                    for (int b = 0; b < KB; ++b) hide(s[b], p, pages, first_page, k0 + 32 * b, see, good, half);
-                }
-                float top = s[0][0];
-#pragma unroll
-                for (int b = 0; b < KB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-                bool raised;
-                const float a = run.raise(top, c, &raised);
-                if (raised) {
-#pragma unroll
-                    for (int dt = 0; dt < L::NDT; ++dt)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[dt][i] *= a;
-                }
-                const float base = run.base();
-#pragma unroll
-                for (int b = 0; b < KB; ++b) {
-                    float x[16];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        f32x4t f = {1.f, 1.f, 1.f, 1.f};
-                        if constexpr (E4M3) f = *reinterpret_cast<const f32x4t*>(&sc[t & 1][1][32 * b + 8 * i + 4 * half]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float e = exp2_fast(__fmaf_rn(s[b][4 * i + j], c, -base));
-                            run.l += e;
-                            x[4 * i + j] = E4M3 ? e * f[j] : e;
-                        }
+                            for (int i = 0; i < 16; ++i) acc[dt][i] *= a;
                     }
-                    typename L::weights pw;
-                    L::pack(pw, x);
-                    L::mma_read_cols(acc, vf, pw);  // O^T[dim][row] += V^T P^T
-                    if (b + 1 < KB) L::read_cols(vf, Vs + (b + 1) * 32 * L::ROWB, ln);
+                    const float base = run.base();
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) {
+                        float x[16];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            f32x4t f = {1.f, 1.f, 1.f, 1.f};
+                            if constexpr (E4M3) f = *reinterpret_cast<const f32x4t*>(&sc[t & 1][1][32 * b + 8 * i + 4 * half]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float e = exp2_fast(__fmaf_rn(s[b][4 * i + j], c, -base));
+                                run.l += e;
+                                x[4 * i + j] = E4M3 ? e * f[j] : e;
+                            }
+                        }
+                        typename L::weights pw;
+                        L::pack(pw, x);
+                        L::mma_read_cols(acc, vf, pw);  // O^T[dim][row] += V^T P^T
+                        if (b + 1 < KB) L::read_cols(vf, Vs + (b + 1) * 32 * L::ROWB, ln);
+                    }
                 }
-            }
-            if constexpr (E4M3) {
-                if (more) {
-                    put(t + 1, nx);
-                    __syncthreads();
+                if constexpr (E4M3) {
+                    if (more) {
+                        put(t + 1, nx);
+                        __syncthreads();
+                    }
                 }
-            }
-        };
-        landed(qf);
-        __syncthreads();  // the images of the previous tile of rows are free
-        if (nt > 0) {
+            };
             fetch(0, smem);
             put(0, smem);
-        }
-        if constexpr (E4M3) __syncthreads();
-        for (int t = 0; t < nt; t += 2) {
-            turn(t, smem, smem + 2 * IMG);
-            if (t + 1 < nt) turn(t + 1, smem + 2 * IMG, smem);
+            if constexpr (E4M3) __syncthreads();
+            for (int t = 0; t < nt; t += 2) {
+                turn(t, smem, smem + 2 * IMG);
+                if (t + 1 < nt) turn(t + 1, smem + 2 * IMG, smem);
+            }
         }
         const float l = run.l + __shfl_xor(run.l, 32, 64);
         if (r < nrows) {
@@ -777,14 +785,10 @@ static PagedShape paged_shape(const capdec_kv_cache* c, int n, int rows, int max
     const int64_t keys = (int64_t)table_cols * c->page, units = std::min((int64_t)n * s.tiles, all) * c->heads;
     int64_t splits = units >= SPLIT_WANT ? 1 : (4 * SPLIT_WANT + units - 1) / units;
     splits = std::min(splits, (keys + SPLIT_MIN - 1) / SPLIT_MIN);
-    // (a split's keys are rounded up to whole runs of 128)
-    const int64_t most = (int64_t)SPLIT_PAGES * c->page - 128;
-    splits = std::max(splits, (keys + most - 1) / most);
     s.splits = (int)std::max<int64_t>(splits, 1);
-    // with s_i splits of at least min(share, most) keys for t_i tiles, sum s_i t_i <= sum t_i (keys_i / min(share, most) + 1),
-    // and share is at least sum keys_i t_i heads / SPLIT_WANT
-    const int64_t by_share = SPLIT_WANT / c->heads + 1, by_most = all * ((keys + most - 1) / most);
-    s.blocks = (s.splits == 1 ? (int64_t)n * s.tiles : std::min(all * s.splits, std::max(by_share, by_most) + all)) * c->heads;
+    // s_i splits for t_i tiles, each of at least a share: sum s_i t_i <= sum t_i (keys_i / share + 1), and share is at least
+    // sum keys_i t_i heads / SPLIT_WANT
+    s.blocks = (s.splits == 1 ? (int64_t)n * s.tiles : std::min(all * s.splits, SPLIT_WANT / c->heads + 1 + all)) * c->heads;
     return s;
 }
 

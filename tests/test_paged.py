@@ -150,6 +150,9 @@ PAGED = [
     ([200, 131], [900, 131], 3, 3, 256, 64),
     ([1] * 300, [37 * i % 1990 for i in range(300)], 2, 1, 16, 64),  # more sequences than threads, all sorts of splits
     ([1, 0, 2] * 90, [1 + 997 * i % 1500 for i in range(270)], 3, 1, 8, 128),
+    # so many sequences that none is split, and one whose pages pass a window of 512
+    ([1] * 20 + [3] + [1] * 43, [2] * 20 + [9001] + [5] * 43, 8, 8, 8, 64),
+    ([1] * 60 + [40] + [1] * 3, [2] * 60 + [8500] + [5] * 3, 16, 8, 8, 128),
 ]
 
 

@@ -43,8 +43,8 @@ struct PagedItem {
 
 // Keys of a split: the batch's work -- keys times tiles of rows -- shared out over SPLIT_WANT workgroups, less what the sequences'
 // shorter last splits are expected to add: all of them run at once and take about as long (a prompt chunk over four sequences:
-// 108 us; without that allowance 116, with a share of every chunk's tiles instead of those it has 126).  At least SPLIT_MIN keys, at least what
-// the longest possible sequence needs to have no more than `splits`, in whole runs of 128.
+// 105 us; without that allowance 116, with the longest chunk's tiles for every chunk 126).  At least SPLIT_MIN keys, at least
+// what the longest possible sequence needs to have no more than `splits`, in whole runs of 128.
 __device__ __forceinline__ int split_size(const PagedParams& p, int64_t work, int64_t tiles, int len) {
     const int64_t room = max((int64_t)SPLIT_WANT - tiles * p.Hkv / 2, (int64_t)SPLIT_WANT / 4);
     const int64_t share = (work * p.Hkv + room - 1) / room;
@@ -123,9 +123,11 @@ __device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
         for (int i0 = 0; i0 < p.n && before <= unit; i0 += 256) {
             if (i0) ask(i0 + tid, f, t, l);
             const int kept = min(max(l, 0), cap), height = tiles_of(f, t);
-            int size = split_size(p, work, tiles, kept), n = max(1, (kept + size - 1) / size);
-            size = max(((kept + n - 1) / n + 127) & ~127, 128);  // all of them alike, not whole ones and a rest
-            n = max(1, (kept + size - 1) / size);
+            // (a length and a share together may pass 2^31)
+            auto cuts = [&](int of) { return max(1, (int)(((unsigned)kept + (unsigned)of - 1u) / (unsigned)of)); };
+            int size = split_size(p, work, tiles, kept), n = cuts(size);
+            size = max((int)(((unsigned)kept + (unsigned)n - 1u) / (unsigned)n + 127u) & ~127, 128);  // all alike, not whole ones and a rest
+            n = cuts(size);
             const int mine = i0 + tid < p.n ? n * height : 0;
             int upto = mine;
 #pragma unroll

@@ -348,6 +348,42 @@ def test_captured_calls_and_other_streams():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lq", [[20, 9, 32], [20, 150, 9]], ids=["short", "long"])
+def test_a_captured_step_through_autograd(lq):
+    """Forward and backward captured together and replayed with new contents.  No eager graph of the leaves is alive then."""
+    from imagecaption_amd import functional
+    ops = _ops()
+    q, k, v, do = (t.contiguous() for t in _inputs(lq, lq, 4, 2, 64, torch.bfloat16, 91))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    seqs = ops.PackedSeqs(lq, device=DEV)
+
+    def step():
+        for t in leaves:
+            t.grad = None
+        functional.attn_packed(*leaves, 4, 2, seqs).backward(do)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    for t in leaves:
+        t.grad = None
+    with torch.cuda.graph(graph):
+        functional.attn_packed(*leaves, 4, 2, seqs).backward(do)
+    for turn in range(4):
+        with torch.no_grad():
+            for i, t in enumerate(leaves):
+                t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(10 * turn + i)))
+        graph.replay()
+        o, lse = ops.attn_packed_fwd(*(t.detach() for t in leaves), 4, 2, seqs)
+        want = ops.attn_packed_bwd(*(t.detach() for t in leaves), o, do, lse, 4, 2, seqs)
+        torch.cuda.synchronize()
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+
+
+@pytest.mark.gpu
 def test_a_plan_made_while_its_memory_is_still_written():
     """The allocator hands out blocks that work queued on the same stream may still write."""
     from imagecaption_amd._capi import CapdecError

@@ -45,32 +45,40 @@ struct PagedItem {
 // shorter last splits are expected to add: all of them run at once and take about as long (a prompt chunk over four sequences:
 // 105 us; without that allowance 116, with the longest chunk's tiles for every chunk 126).  At least SPLIT_MIN keys, at least
 // what the longest possible sequence needs to have no more than `splits`, in whole runs of 128.
-__device__ __forceinline__ int split_size(const PagedParams& p, int64_t work, int64_t tiles, int len) {
-    const int64_t room = max((int64_t)SPLIT_WANT - tiles * p.Hkv / 2, (int64_t)SPLIT_WANT / 4);
-    const int64_t share = (work * p.Hkv + room - 1) / room;
-    int c = max((int)min(share, (int64_t)(1 << 30)), (len + p.splits - 1) / p.splits);
-    c = max(c, SPLIT_MIN);
-    return (c + 127) & ~127;
+// (In fp32: the share only has to be the same for all workgroups and, for the grid to hold all splits, no less than the work
+// of a SPLIT_WANT-th, which half a tile's allowance or 2^-18 makes sure of.)
+__device__ __forceinline__ int split_size(const PagedParams& p, float work, int tiles, int len) {
+    const float room = fmaxf((float)SPLIT_WANT - (float)tiles * (float)p.Hkv * 0.5f, (float)SPLIT_WANT / 4);
+    const float share = work * (float)p.Hkv * (1.f + 0x1p-18f) / room;
+    const int c = max((int)fminf(share, 0x1p30f) + 1, (len + p.splits - 1) / p.splits);
+    return (max(c, SPLIT_MIN) + 127) & ~127;
 }
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        v += (int64_t)(((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o, 64) << 32) | (uint32_t)__shfl_xor((int)v, o, 64));
+// sums of v over the lanes up to this one
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+#define CAPDEC_SCAN(ctrl, rows) v += __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, false))
+    CAPDEC_SCAN(0x111, 0xf);  // row_shr:1, 2, 4, 8: within rows of 16 lanes
+    CAPDEC_SCAN(0x112, 0xf);
+    CAPDEC_SCAN(0x114, 0xf);
+    CAPDEC_SCAN(0x118, 0xf);
+    CAPDEC_SCAN(0x142, 0xa);  // row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3
+    CAPDEC_SCAN(0x143, 0xc);
+#undef CAPDEC_SCAN
     return v;
 }
+__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
 // Workgroup -> (sequence, split, tile of BLOCK rows), key / value head.  With splits, only as many workgroups are launched as
-// there can be in all, and which one a workgroup is follows from the lengths, by a scan over them.  (One workgroup for every
+// there can be in all, and which one a workgroup is follows from the lengths, by a scan over them that every wave makes for
+// itself.  (One workgroup for every
 // split that the longest possible sequence could have, most of them without work: 49 us instead of 46 for 8 contexts of 9 to 60
 // thousand tokens, 29 instead of 21 for chunks of 5 drafted tokens over 48 contexts.)  The row tiles of one
 // (sequence, head, split) go round the XCDs (blockIdx % 8): kept on one XCD they would share its L2, but a few such groups of up
 // to 16 tiles do not divide by eight (a prompt chunk over four sequences: 134 us against 123).
 template <int BLOCK>
 __device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
-    __shared__ int64_t sums[2][4];
-    __shared__ int ends[4], found[8];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, cap = p.cols << p.page_log2;
+    const int tid = threadIdx.x, lane = tid & 63, cap = p.cols << p.page_log2;
     PagedItem w;
     w.split = 0;
     w.nsplit = 1;
@@ -90,7 +98,7 @@ __device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
     } else {
         w.hk = blockIdx.x % p.Hkv;
         const int unit = blockIdx.x / p.Hkv;
-        // a thread's sequence: all three numbers are asked for at once
+        // a lane's sequence: all three numbers are asked for at once
         auto ask = [&](int i, int& f, int& t, int& l) {
             f = i < p.n ? (p.cu ? p.cu[i] : i) : 0;
             t = i < p.n ? (p.cu ? p.cu[i + 1] : i + 1) : 0;
@@ -101,73 +109,52 @@ __device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
             return max(1, ((min(max(t, f), p.rows) - f) * p.group + BLOCK - 1) / BLOCK);
         };
         int f, t, l;
-        ask(tid, f, t, l);
-        int64_t tiles = tid < p.n ? tiles_of(f, t) : 0, work = tiles * min(max(l, 0), cap);
-        for (int i = tid + 256; i < p.n; i += 256) {
+        ask(lane, f, t, l);
+        int tiles = lane < p.n ? tiles_of(f, t) : 0;
+        float work = (float)tiles * (float)min(max(l, 0), cap);
+        for (int i = lane + 64; i < p.n; i += 64) {
             int f2, t2, l2;
             ask(i, f2, t2, l2);
-            const int64_t more = tiles_of(f2, t2);
+            const int more = tiles_of(f2, t2);
             tiles += more;
-            work += more * min(max(l2, 0), cap);
+            work += (float)more * (float)min(max(l2, 0), cap);
         }
-        tiles = wave_sum64(tiles);
-        work = wave_sum64(work);
-        if (lane == 0) {
-            sums[0][wave] = tiles;
-            sums[1][wave] = work;
-        }
-        __syncthreads();
-        tiles = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
-        work = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+        tiles = last_lane(wave_scan(tiles));
+        work = __int_as_float(last_lane(__float_as_int(wave_scan(work))));
+        w.ok = false;
         int before = 0;  // workgroups (of one head) of the sequences already passed
-        for (int i0 = 0; i0 < p.n && before <= unit; i0 += 256) {
-            if (i0) ask(i0 + tid, f, t, l);
+        for (int i0 = 0; i0 < p.n; i0 += 64) {
+            if (i0) ask(i0 + lane, f, t, l);
             const int kept = min(max(l, 0), cap), height = tiles_of(f, t);
             // (a length and a share together may pass 2^31)
             auto cuts = [&](int of) { return max(1, (int)(((unsigned)kept + (unsigned)of - 1u) / (unsigned)of)); };
             int size = split_size(p, work, tiles, kept), n = cuts(size);
             size = max((int)(((unsigned)kept + (unsigned)n - 1u) / (unsigned)n + 127u) & ~127, 128);  // all alike, not whole ones and a rest
             n = cuts(size);
-            const int mine = i0 + tid < p.n ? n * height : 0;
-            int upto = mine;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int x = __shfl_up(upto, o, 64);
-                if (lane >= o) upto += x;
+            const int mine = i0 + lane < p.n ? n * height : 0, upto = wave_scan(mine);
+            const unsigned at = (unsigned)(unit - (before + upto - mine));
+            const unsigned long long own = __ballot(at < (unsigned)mine);
+            if (own) {
+                const int src = __ffsll(own) - 1;
+                auto take = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
+                const int index = take((int)at), cut = take(size);
+                w.ok = true;
+                w.seq = i0 + src;
+                w.step = take(height);
+                w.nsplit = take(n);
+                w.split = min((int)((unsigned)index / (unsigned)w.step), w.nsplit - 1);
+                w.tile = (int)((unsigned)index % (unsigned)w.step);
+                from = take(f);
+                to = take(t);
+                len = take(l);
+                w.len = min(max(len, 0), cap);
+                w.kbegin = w.split * cut;
+                w.kend = min(w.len, w.kbegin + cut);
+                break;
             }
-            if (lane == 63) ends[wave] = upto;
-            __syncthreads();
-            int start = before + upto - mine;
-            for (int i = 0; i < wave; ++i) start += ends[i];
-            const unsigned at = (unsigned)(unit - start);
-            if (at < (unsigned)mine) {
-                found[0] = i0 + tid;
-                found[1] = min((int)(at / (unsigned)height), n - 1);
-                found[2] = n;
-                found[3] = size;
-                found[4] = f;
-                found[5] = t;
-                found[6] = l;
-                found[7] = at % (unsigned)height;
-            }
-            before += ends[0] + ends[1] + ends[2] + ends[3];
-            __syncthreads();
+            before += last_lane(upto);
         }
-        w.ok = unit < before;
         if (!w.ok) return w;
-        auto take = [&](int i) { return __builtin_amdgcn_readfirstlane(found[i]); };  // (the same for all: scalar registers)
-        const int size = take(3);
-        w.seq = take(0);
-        w.split = take(1);
-        w.nsplit = take(2);
-        from = take(4);
-        to = take(5);
-        len = take(6);
-        w.tile = take(7);
-        w.step = tiles_of(from, to);
-        w.len = min(max(len, 0), cap);
-        w.kbegin = w.split * size;
-        w.kend = min(w.len, w.kbegin + size);
     }
     w.a = min(max(from, 0), p.rows);
     w.nq = min(max(to, w.a), p.rows) - w.a;

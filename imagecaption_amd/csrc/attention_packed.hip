@@ -101,13 +101,15 @@ __device__ __forceinline__ void add_sums(const unsigned char* box, f32x16* acc, 
 
 // (One wave a workgroup: bound by the way from launch to store, so the weights can keep 16 bits.  bf16 weights alone would double
 // the error of the result, whose own rounding is as large; 256 captions, forward 6.1 -> 6.2 us, backward 9.8 -> 10.7.)
-// RB blocks of 32 rows; the KS waves of a block take every KS-th run of 32 KB keys of a tile and join at the end
-template <typename T, int DH, int RB, int KS, int KB>
+// RB blocks of 32 rows; the KS waves of a block take every KS-th run of 32 KB keys of a tile and join at the end.  ONE: no walk is
+// longer than one tile, so there is one pair of images (132 sequences of 2 tokens, 15 heads of 128, fp32: 38 us with two, 19 with
+// one)
+template <typename T, int DH, int RB, int KS, int KB, bool ONE = false>
 __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd_kernel(PackedParams p) {
     using L = AttTile<T, DH>;
     constexpr int NT = RB * KS * 64, BN = 32 * KB * KS, IMG = BN * L::ROWB, BOX = (DH / 8 * 16 + 8) * 64;
-    constexpr int JOIN = RB * (KS - 1) * BOX;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG > JOIN ? 4 * IMG : JOIN];
+    constexpr int JOIN = RB * (KS - 1) * BOX, IMAGES = ONE ? 2 : 4;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[IMAGES * IMG > JOIN ? IMAGES * IMG : JOIN];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     const int rb = wave % RB, ksp = wave / RB;
     int head, it;
@@ -146,7 +148,7 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd
     for (int t = 0; t < nt; ++t) {
         const unsigned char* Ks = smem + (t & 1) * 2 * IMG + ksp * 32 * KB * L::ROWB;
         const unsigned char* Vs = Ks + IMG;
-        const bool more = t + 1 < nt;
+        const bool more = !ONE && t + 1 < nt;
         if (more) {
             ks.load(kg, p.ldk, (t + 1) * BN, w.nk, tid);
             vs.load(vg, p.ldv, (t + 1) * BN, w.nk, tid);
@@ -192,7 +194,8 @@ __global__ __launch_bounds__(RB * KS * 64, RB * KS == 4 ? 2 : 1) void packed_fwd
                 }
                 std::conditional_t<RB * KS == 1, typename L::weights2, typename L::weights> pw;
                 L::pack(pw, x);
-                L::mma_cols(acc, Vs + b * 32 * L::ROWB, ln, pw);  // O^T[dim][query] += V^T P^T
+                if constexpr (ONE) L::mma_cols(acc, Vs, ln, pw, w.nk);
+                else L::mma_cols(acc, Vs + b * 32 * L::ROWB, ln, pw);  // O^T[dim][query] += V^T P^T
             }
         }
         if (more) {
@@ -573,35 +576,43 @@ __global__ __launch_bounds__(256, 2) void packed16_bwd_dq_kernel(PackedParams p)
     }
 }
 
-// dq, dk, dv of sequences that fit one block of 32 rows on both sides, in one pass: a wave takes a (sequence, key / value head)
-// and walks the query heads of the group.  Everything is read once and o not at all (delta = sum p dp, see score_grads); the
-// scores are made in both orientations because the two sums run over different sides.  256 captions of up to 20 tokens,
-// 8 heads of 64, bf16: 10.7 us (dq, then dk and dv: 14.5).  Weights keep 16 bits, as in the forward.
-template <typename T, int DH>
-__global__ __launch_bounds__(64) void packed_bwd_block_kernel(PackedParams p) {
+// dq, dk, dv of sequences that fit one block of 32 rows on both sides, in one pass: a workgroup takes a (sequence, key / value
+// head), its W waves every W-th query head of the group, and the first wave adds up their dk and dv in order.  Everything is
+// read once and o not at all (delta = sum p dp, see score_grads).  Scores are made once, keys x queries; dk and dv, which sum
+// over the queries, take the transposed weights through LDS.  Products over the rows of an image stop behind the last one.
+// Weights keep 16 bits, as in the forward.  256 captions of up to 20 tokens, 8 heads of 64: bf16 10.0 us (dq, then dk and dv: 14.5;
+// scores made in both orientations instead of weights transposed: 10.3), fp32 26 (29); 64 sequences of 10 to 30 tokens, 32 heads
+// of 128 over 4, bf16: 19, 40 with one wave for the group.
+template <typename T, int DH, int W>
+__global__ __launch_bounds__(64 * W, DH == 64 && sizeof(T) == 2 ? 2 : 1) void packed_bwd_block_kernel(PackedParams p) {
     using L = AttTile<T, DH>;
-    constexpr int IMG = 32 * L::ROWB;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * IMG];
-    __shared__ __attribute__((aligned(16))) float stat[2][32];  // [lse2 | delta][query]
-    const int lane = threadIdx.x, l31 = lane & 31, half = lane >> 5;
+    constexpr int IMG = 32 * L::ROWB, BOX = DH / 8 * 16 * 64, TURN = 33;
+    constexpr bool AHEAD = L::ROWB <= 256;  // a wider head's rows on their way would not fit the registers
+    static_assert(BOX <= 2 * IMG, "a wave's sums fit its images");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[(2 + 2 * W) * IMG];
+    __shared__ float turned[W > 1 ? W : 1][W > 1 ? 32 * TURN : 1];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l31 = lane & 31, half = lane >> 5;
     int hk, it;
     packed_place(p.Hkv, hk, it);
     const PackedItem w = p.items[it];
     const int off = w.nk - w.nq;  // causal: query i sees the keys j <= i + off
     const bool mine_q = l31 < w.nq, mine_k = l31 < w.nk;
-    unsigned char *Ks = smem, *Vs = smem + IMG, *Qs = smem + 2 * IMG, *Ds = smem + 3 * IMG;
-    Staged<T, DH, 64, 32> ks, vs, qst, dst;
-    float lse2;
-    auto fetch = [&](int head) {
+    unsigned char *Ks = smem, *Vs = smem + IMG, *Qs = smem + (2 + 2 * wave) * IMG, *Ds = Qs + IMG;
+    float* turn = W > 1 ? turned[wave] : reinterpret_cast<float*>(Ks);  // (one head: K and V are no longer needed then)
+    Staged<T, DH, 64 * W, 32> ks, vs;
+    Staged<T, DH, 64, 32> qst, dst;
+    float next;
+    auto fetch = [&](int g) {
+        const int head = hk * p.group + g;
         qst.load((const T*)p.q + (size_t)w.q0 * p.ldq + head * DH, p.ldq, 0, w.nq, lane);
         dst.load((const T*)p.dout + (size_t)w.q0 * p.lddo + head * DH, p.lddo, 0, w.nq, lane);
-        lse2 = row_lse2(p, (size_t)(w.q0 + l31), head, mine_q);
+        next = row_lse2(p, (size_t)(w.q0 + l31), head, mine_q);
     };
-    ks.load((const T*)p.k + (size_t)w.k0 * p.ldk + hk * DH, p.ldk, 0, w.nk, lane);
-    vs.load((const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, 0, w.nk, lane);
-    fetch(hk * p.group);
-    ks.store(Ks, lane);
-    vs.store(Vs, lane);
+    ks.load((const T*)p.k + (size_t)w.k0 * p.ldk + hk * DH, p.ldk, 0, w.nk, tid);
+    vs.load((const T*)p.v + (size_t)w.k0 * p.ldv + hk * DH, p.ldv, 0, w.nk, tid);
+    if (AHEAD && wave < p.group) fetch(wave);
+    ks.store(Ks, tid);
+    vs.store(Vs, tid);
     const typename L::lanes ln = L::make_lanes(lane);
     const float c = p.scale * LOG2E;
     const int see = p.causal ? min(w.nk, l31 + 1 + off) : w.nk;
@@ -611,59 +622,66 @@ __global__ __launch_bounds__(64) void packed_bwd_block_kernel(PackedParams p) {
         zero16(dk[dt]);
         zero16(dv[dt]);
     }
-    for (int g = 0; g < p.group; ++g) {
-        const int head = hk * p.group + g;
+    // weights [key][query] of a lane's query -> [query][key] of a lane's key
+    auto transpose = [&](float* x) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) turn[row_of(r, half) * TURN + l31] = x[r];
+        wave_fence();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = turn[l31 * TURN + row_of(r, half)];
+        wave_fence();
+    };
+    __syncthreads();
+    for (int g = wave; g < p.group; g += W) {
+        if (!AHEAD) fetch(g);
+        wave_fence();
         qst.store(Qs, lane);
         dst.store(Ds, lane);
-        if (half == 0) stat[0][l31] = lse2;
-        __syncthreads();
-        float x[16];
-        {
-            f32x16 s, dp, dq[L::NDT];
-            zero16(s);
-            zero16(dp);
-            L::mma_images(s, Ks, Qs, ln);   // S^T[key][query]
-            L::mma_images(dp, Vs, Ds, ln);  // dP^T[key][query]
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = row_of(r, half) < see ? s[r] : -INFINITY;
-            float dsum = 0.f;
-            score_grads(x, s, dp, c, lse2, true, dsum);
-            if (half == 0) stat[1][l31] = dsum;
-            typename L::weights2 dw;
-            L::pack(dw, x);
-#pragma unroll
-            for (int dt = 0; dt < L::NDT; ++dt) zero16(dq[dt]);
-            L::mma_cols(dq, Ks, ln, dw);  // dQ^T[dim][query] = K^T dS^T
-            if (mine_q) L::store_row((T*)p.dq + (size_t)(w.q0 + l31) * p.lddq + head * DH, dq, p.scale, half);
-        }
-        if (g + 1 < p.group) fetch(head + 1);
-        __syncthreads();
+        wave_fence();
+        const float lse2 = next;
+        if (AHEAD && g + W < p.group) fetch(g + W);
         f32x16 s, dp;
         zero16(s);
         zero16(dp);
-        L::mma_images(s, Qs, Ks, ln);   // S[query][key]
-        L::mma_images(dp, Ds, Vs, ln);  // dP[query][key]
-        if (p.causal) {
+        L::mma_images(s, Ks, Qs, ln);   // S^T[key][query]
+        L::mma_images(dp, Vs, Ds, ln);  // dP^T[key][query]
+        float x[16], y[16], dsum = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = l31 <= row_of(r, half) + off ? s[r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) {
+            x[r] = row_of(r, half) < see ? exp2_fast(__fmaf_rn(s[r], c, -lse2)) : 0.f;
+            dsum = __fmaf_rn(x[r], x[r] > 0.f ? dp[r] : 0.f, dsum);
         }
-        float y[16];
+        dsum += __shfl_xor(dsum, 32, 64);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4t ls = *reinterpret_cast<const f32x4t*>(&stat[0][8 * i + 4 * half]);
-            const f32x4t de = *reinterpret_cast<const f32x4t*>(&stat[1][8 * i + 4 * half]);
+        for (int r = 0; r < 16; ++r) y[r] = x[r] * (dp[r] - dsum);
+        typename L::weights2 pw, dw;
+        L::pack(dw, y);
+        f32x16 dq[L::NDT];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[4 * i + j] = exp2_fast(__fmaf_rn(s[4 * i + j], c, -ls[j]));
-                y[4 * i + j] = x[4 * i + j] * (dp[4 * i + j] - de[j]);
+        for (int dt = 0; dt < L::NDT; ++dt) zero16(dq[dt]);
+        L::mma_cols(dq, Ks, ln, dw, w.nk);  // dQ^T[dim][query] = K^T dS^T
+        if (mine_q) L::store_row((T*)p.dq + (size_t)(w.q0 + l31) * p.lddq + (hk * p.group + g) * DH, dq, p.scale, half);
+        wave_fence();
+        transpose(x);
+        L::pack(pw, x);
+        L::mma_cols(dv, Ds, ln, pw, w.nq);  // dV^T[dim][key] += dO^T P
+        transpose(y);
+        L::pack(dw, y);
+        L::mma_cols(dk, Qs, ln, dw, w.nq);  // dK^T[dim][key] += Q^T dS
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            f32x16* acc = side ? dk : dv;
+            __syncthreads();
+            if (wave > 0) put_sums<L::NDT>(Qs, acc, lane);
+            __syncthreads();
+            if (wave == 0) {
+#pragma unroll
+                for (int o = 1; o < W; ++o) add_sums<L::NDT>(smem + (2 + 2 * o) * IMG, acc, lane, 1.f, 1.f);
             }
         }
-        typename L::weights2 pw, dw;
-        L::pack(pw, x);
-        L::pack(dw, y);
-        L::mma_cols(dv, Ds, ln, pw);  // dV^T[dim][key] += dO^T P
-        L::mma_cols(dk, Qs, ln, dw);  // dK^T[dim][key] += Q^T dS
-        __syncthreads();
+        if (wave > 0) return;
     }
     if (mine_k) {
         L::store_row((T*)p.dk + (size_t)(w.k0 + l31) * p.lddk + hk * DH, dk, p.scale, half);
@@ -1139,7 +1157,8 @@ static PackedParts packed_parts(const capdec_packed_seqs* s, int Hkv, int group)
 
 template <typename T, int DH>
 static void launch_fwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t st) {
-    if (short_rows(s->tiles)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
+    if (s->one_block) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 1, 1, true>), 2, p.Hq, 64);
+    else if (short_rows(s->tiles)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
     else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
     else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed16_fwd_kernel<DH>), 0, p.Hq, 256);
 }
@@ -1147,7 +1166,10 @@ static void launch_fwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t
 template <typename T, int DH>
 static void launch_bwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t st) {
     if (s->one_block) {
-        if (s->tiles[5] > 0) CAPDEC_PACKED((packed_bwd_block_kernel<T, DH>), 5, p.Hkv, 64);
+        constexpr int W = sizeof(T) == 4 && DH == 128 ? 2 : 4;
+        if (s->tiles[5] == 0) return;
+        if (p.group == 1) CAPDEC_PACKED((packed_bwd_block_kernel<T, DH, 1>), 5, p.Hkv, 64);
+        else CAPDEC_PACKED((packed_bwd_block_kernel<T, DH, W>), 5, p.Hkv, 64 * W);
         return;
     }
     const bool one = short_rows(s->tiles + 3);

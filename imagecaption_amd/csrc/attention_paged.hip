@@ -309,13 +309,6 @@ __device__ __forceinline__ void hide(f32x16& s, const PagedParams& p, const int6
     }
 }
 
-// Orders a wave's LDS writes before other lanes' reads (and reads before the next writes) for the compiler; the hardware
-// executes one wave's LDS operations in order, so nothing is waited for.
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // (Weights keep 16 bits: bound by the cache's bytes, the kernel has room for the products of their second terms.  8 contexts of 9
 // to 60 thousand tokens: 46 us either way; 48 of 100 to 8000, five tokens each: 21 -> 22.7.)
 // R blocks of 32 rows; every wave walks its own runs of 32 keys, one run ahead in registers.  The rows are the same for all

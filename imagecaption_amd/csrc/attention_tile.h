@@ -6,7 +6,7 @@
 //              against the wave's own rows, which stay in registers as B fragments);
 //   mma_cols   out[head dim][lane's column] += image^T x weights, reduced over the image's rows (context and gradients):
 //              the 32 weights of a column are the accumulator of a mma_rows product, in the order in which the matrix
-//              instruction left them, so probabilities never move between lanes.
+//              instruction left them, so probabilities never move between lanes; image rows from `rows` on have no weight.
 // bf16: v_mfma_f32_32x32x16_bf16, the transposed operand comes from the transposing LDS read (ds_read_b64_tr_b16);
 // fp32: v_mfma_f32_32x32x2_f32 (exact products), where any lane can read its transposed element directly.
 #pragma once
@@ -108,11 +108,11 @@ struct AttTile<__bf16, DH> {
                 w.lo.f[m][e] = (__bf16)(x[8 * m + e] - (float)w.hi.f[m][e]);
             }
     }
-    __device__ static __forceinline__ void mma_cols(f32x16* out, const unsigned char* img, const lanes& l, const weights2& w) {
+    __device__ static __forceinline__ void mma_cols(f32x16* out, const unsigned char* img, const lanes& l, const weights2& w, int rows = 32) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) {
+            for (int dt = 0; dt < NDT && 16 * m < rows; ++dt) {
                 const bf16x4t lo = read_tr(img + m * 16 * ROWB + (l.col[0] ^ (dt << 6)));
                 const bf16x4t hi = read_tr(img + m * 16 * ROWB + (l.col[1] ^ (dt << 6)));
                 const bf16x8t a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -215,9 +215,10 @@ struct AttTile<float, DH> {
 #pragma unroll
         for (int r = 0; r < 16; ++r) w.f[r] = x[r];
     }
-    __device__ static __forceinline__ void mma_cols(f32x16* out, const unsigned char* img, const lanes& l, const weights& w) {
+    __device__ static __forceinline__ void mma_cols(f32x16* out, const unsigned char* img, const lanes& l, const weights& w, int rows = 32) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
+            if (8 * (r >> 2) >= rows) continue;
             const int kr = row_of(r, l.half);
             const unsigned char* row = img + kr * ROWB + (l.l31 & 3) * 4;
 #pragma unroll
@@ -237,6 +238,13 @@ struct AttTile<float, DH> {
             }
     }
 };
+
+// Orders a wave's LDS writes before other lanes' reads (and reads before the next writes) for the compiler; the hardware
+// executes one wave's LDS operations in order, so nothing is waited for.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
 // a value the compiler has to take as it is here: nothing made from it is kept from an earlier turn of a loop
 __device__ __forceinline__ void opaque(int& x) { asm volatile("" : "+v"(x)); }

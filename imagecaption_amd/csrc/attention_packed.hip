@@ -1131,6 +1131,11 @@ static bool short_rows(const int* tiles) { return 2 * (int64_t)tiles[2] < 3 * (i
 template <typename T>
 static bool tall_rows(const int* tiles, int heads) { return sizeof(T) == 2 && (int64_t)tiles[0] * heads >= 320; }
 
+// bf16: 32 rows and four waves for them, each taking every fourth run of keys, where 64 rows would leave CUs without a workgroup
+// (one text of 1655 tokens, 8 heads of 64: forward 21 -> 16 us, backward 44 -> 39; one of 1302, 8 heads of 128 over 4: 25 -> 24,
+// 67 -> 63; with 368 tiles of 64 rows, 4 texts of 734, 8 heads of 128 over 1, the other way: 18 / 30, 65 / 78)
+static bool low_rows(const int* tiles, int heads) { return (int64_t)tiles[1] * heads < 256; }
+
 // bytes of what dq leaves for dk / dv, whole 16-byte pieces
 template <typename T>
 static size_t stat_bytes(int Hq, size_t stat_rows) {
@@ -1159,7 +1164,9 @@ template <typename T, int DH>
 static void launch_fwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t st) {
     if (s->one_block) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 1, 1, true>), 2, p.Hq, 64);
     else if (short_rows(s->tiles)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
-    else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
+    else if (sizeof(T) == 2 && low_rows(s->tiles, p.Hq)) {
+        if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 1, 4, 1>), 2, p.Hq, 256);
+    } else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_fwd_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
     else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed16_fwd_kernel<DH>), 0, p.Hq, 256);
 }
 
@@ -1176,7 +1183,9 @@ static void launch_bwd(PackedParams& p, const capdec_packed_seqs* s, hipStream_t
     if (sizeof(T) == 2 && !one) p.stats = p.delta;
     if (s->tiles[0] > 0) {
         if (short_rows(s->tiles)) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 1, 1, 1>), 2, p.Hq, 64);
-        else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
+        else if (sizeof(T) == 2 && low_rows(s->tiles, p.Hq)) {
+            if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 1, 4, 1>), 2, p.Hq, 256);
+        } else if (!tall_rows<T>(s->tiles, p.Hq)) CAPDEC_PACKED((packed_bwd_dq_kernel<T, DH, 2, 2, 1>), 1, p.Hq, 256);
         else if constexpr (sizeof(T) == 2) CAPDEC_PACKED((packed16_bwd_dq_kernel<DH>), 0, p.Hq, 256);
     }
     if (s->tiles[3] > 0) {

@@ -107,6 +107,27 @@ def _inputs(lq, lk, Hq, Hkv, dh, dtype, seed, extra=0):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lq, lk, causal, Hq, Hkv, dh", [
+    ([70, 33, 128, 127] * 6, None, True, 8, 4, 64), ([70, 33, 128, 127] * 6, [40, 100, 0, 65] * 6, False, 8, 2, 128),  # 64 rows a workgroup
+    ([130, 257, 128, 40] * 7 + [1], None, True, 8, 4, 128), ([130, 257, 128, 40] * 7, [70, 300, 1, 0] * 7, True, 8, 8, 64),  # 128 rows
+    ([129, 200] * 12, [65, 31] * 12, False, 8, 1, 128)])
+def test_heights_of_workgroups_match_float64(lq, lk, causal, Hq, Hkv, dh):
+    """Batches with enough tiles for the taller workgroups of bf16 matrices."""
+    ops = _ops()
+    q, k, v, do = _inputs(lq, lk or lq, Hq, Hkv, dh, torch.bfloat16, 700 + dh)
+    scale = 1 / math.sqrt(dh)
+    ref = reference(q, k, v, do, lq, lk or lq, Hq, Hkv, causal, scale, E16)
+    seqs = ops.PackedSeqs(lq, lk, causal=causal, device=DEV)
+    assert seqs.c.tiles[1] * Hq >= 256 and (seqs.c.tiles[0] * Hq >= 320) == (max(lq) > 128)
+    o, lse = ops.attn_packed_fwd(q, k, v, Hq, Hkv, seqs)
+    within("lse", lse, ref)
+    grads = ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs)
+    for name, t in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        within(name, t, ref)
+    assert all(torch.equal(a, b) for a, b in zip(grads, ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lq, lk, causal, Hq, Hkv, dh", [([1500, 70], None, True, 8, 1, 64), ([900, 40, 1], [300, 7, 1000], False, 6, 2, 128),
                                                          ([1100] + [65] * 30, None, True, 4, 4, 128)])

@@ -1145,7 +1145,8 @@ static size_t stat_bytes(int Hq, size_t stat_rows) {
 // dk, dv of key tiles whose walk over the queries is longer than 5/4 of a workgroup's even share (512 run at once) are summed in
 // parts by several workgroups and joined in a second launch: such a walk would be running alone at the end (8 texts of 300 to
 // 4096 tokens, 16 heads of 128 over 4: 340 us in one piece, 242 and 13 for the join in parts; one text of 2000 over 2 heads,
-// the whole backward: 333 / 141).  With 3/4, 1/2, 1/4 of a share: 4, 8 and 23 % more for the first one's backward.  A part is at least 8 tiles.
+// the whole backward: 333 / 138).  With 3/4, 1/2, 1/4 of a share the first one's backward takes 4, 8 and 23 % more.  A part is
+// at least 8 tiles (4: 64 sequences of 64 to 128 tokens 33 -> 46 us, the join not being worth it).
 struct PackedParts {
     int parts, items, slots;  // of the longest tiles; tiles that are split, their parts together
 };

@@ -43,7 +43,8 @@ struct PagedItem {
 
 // Keys of a split: the batch's work -- keys times tiles of rows -- shared out over SPLIT_WANT workgroups, less what the sequences'
 // shorter last splits are expected to add: all of them run at once and take about as long (a prompt chunk over four sequences:
-// 105 us; without that allowance 116, with the longest chunk's tiles for every chunk 126).  At least SPLIT_MIN keys, at least
+// 105 us; without that allowance 113, with the longest chunk's tiles for every chunk 126; 8 contexts of 9 to 60 thousand tokens
+// with 384 / 512 / 640 workgroups to aim at: 47 / 45 / 59).  At least SPLIT_MIN keys, at least
 // what the longest possible sequence needs to have no more than `splits`, in whole runs of 128.
 // (In fp32: the share only has to be the same for all workgroups and, for the grid to hold all splits, no less than the work
 // of a SPLIT_WANT-th, which half a tile's allowance or 2^-18 makes sure of.)
@@ -71,11 +72,11 @@ __device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readla
 
 // Workgroup -> (sequence, split, tile of BLOCK rows), key / value head.  With splits, only as many workgroups are launched as
 // there can be in all, and which one a workgroup is follows from the lengths, by a scan over them that every wave makes for
-// itself.  (One workgroup for every
-// split that the longest possible sequence could have, most of them without work: 49 us instead of 46 for 8 contexts of 9 to 60
-// thousand tokens, 29 instead of 21 for chunks of 5 drafted tokens over 48 contexts.)  The row tiles of one
-// (sequence, head, split) go round the XCDs (blockIdx % 8): kept on one XCD they would share its L2, but a few such groups of up
-// to 16 tiles do not divide by eight (a prompt chunk over four sequences: 134 us against 123).
+// itself.  (One workgroup for every split that the longest possible sequence could have, most of them without work: 49 us
+// instead of 46 for 8 contexts of 9 to 60 thousand tokens, 29 instead of 21 for chunks of 5 drafted tokens over 48 contexts; the
+// scan by the whole workgroup, through LDS: 1.4 us more.)  The row tiles of one (sequence, head, split) go round the XCDs
+// (blockIdx % 8): kept on one XCD they would share its L2, but a few such groups of up to 16 tiles do not divide by eight (a
+// prompt chunk over four sequences: 134 us against 123).
 template <int BLOCK>
 __device__ __forceinline__ PagedItem paged_place(const PagedParams& p) {
     const int tid = threadIdx.x, lane = tid & 63, cap = p.cols << p.page_log2;

@@ -517,6 +517,40 @@ def test_prompt_cache_drafts_and_verification_together(dtype):
 
 # ---- refusals -------------------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    """Calls with scratch of their own (split keys, walks in parts), overlapping on two streams."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(3)
+    works = []
+    for i in range(2):
+        total = [3000 + 500 * i, 700, 90]
+        cache, table, _, _ = _filled([2, 1, 3], total, 2, 16, 128, (BF16, E4M3)[i], 900 + i)
+        q = torch.randn(6, 8 * 128, generator=g).to(BF16).to(DEV)
+        lens, cu = torch.tensor(total, dtype=torch.int32, device=DEV), torch.tensor([0, 2, 3, 6], dtype=torch.int32, device=DEV)
+        lengths = [1200 + 100 * i, 33]
+        wide = torch.randn(sum(lengths), 4 * 256, generator=g).to(BF16).to(DEV)
+        seqs = ops.PackedSeqs(lengths, device=DEV)
+
+        def work(cache=cache, table=table, q=q, lens=lens, cu=cu, wide=wide, seqs=seqs):
+            o, lse = ops.attn_packed_fwd(wide[:, :256], wide[:, 256:320], wide[:, 320:384], 4, 1, seqs)
+            grads = ops.attn_packed_bwd(wide[:, :256], wide[:, 256:320], wide[:, 320:384], o, wide[:, 512:768], lse, 4, 1, seqs)
+            return [o, *grads, ops.attn_paged(q, cache, table, lens, 8, cu_q=cu, max_q=3)]
+
+        works.append(work)
+    want = [w() for w in works]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in works]
+    got = []
+    for turn in range(6):
+        for w, s in zip(works, streams):
+            with torch.cuda.stream(s):
+                got.append(w())
+    torch.cuda.synchronize()
+    for i, res in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(res, want[i % 2])), i
+
+
+@pytest.mark.gpu
 def test_direct_and_general_calls_agree(monkeypatch):
     """The direct calls (csrc/calls.cpp) take the plain forms and do what the general way through ctypes does."""
     from imagecaption_amd import _capi

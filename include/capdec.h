@@ -358,8 +358,9 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
  *   bwd: dq, dk, dv from do; dk / dv sum over the query heads of their group.  No atomics: bitwise reproducible.
  *   scale between 2^-60 and 2^60.  Results must not overlap the matrices that are read; fewer than 2^31 - 1024 rows a side.
  * dtype CAPDEC_F32: every matrix fp32, exact fp32 products; CAPDEC_BF16S: every matrix bf16, fp32 accumulation, softmax and
- * statistics, probabilities and score gradients rounded to bf16 for the products that take them (to 16 bits, two bf16 terms,
- * where most sequences fit 32 rows), the only roundings besides the results'.  dh in {64, 128}; 16-byte aligned matrices, row strides multiples of 16 bytes, at most 2^25 bytes.  Non-finite values:
+ * statistics; probabilities and score gradients are rounded to bf16 for the products that take them -- to 16 bits, two bf16
+ * terms, where most sequences (backward: all) fit 32 rows --, the only roundings besides the results'.  dh in {64, 128};
+ * 16-byte aligned matrices, row strides multiples of 16 bytes, at most 2^25 bytes.  Non-finite values:
  * the products are plain ones (0 x inf = NaN), so an infinity or NaN in v reaches the rows of ITS sequence that share a
  * tile with it even where they are masked; it never reaches another sequence.
  * The plan: capdec_packed_plan checks the lengths (host arrays; lens_k = NULL: the same as lens_q), writes the tile table to

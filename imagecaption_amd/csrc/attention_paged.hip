@@ -182,9 +182,11 @@ __device__ __forceinline__ int window_end(const PagedParams& p, int k0, int kend
 }
 
 // the pages of the keys k0 .. kend - 1 (one window) into LDS, as byte offsets of this head's first row there; pages outside the
-// cache become -1 and are counted; *bad tells that there are some.  The caller waits for the workgroup before it uses them.
-__device__ __forceinline__ void load_pages(int64_t* pages, int* bad, const PagedParams& p, const PagedItem& w, int k0, int kend, int row_bytes, int tid,
-                                           int nt) {
+// cache become -1 and are counted where `last` is set, for the chunk's last tile of rows: it sees all keys, the first one of a long
+// chunk may see none of a split's or a window's.  *bad tells that there are some.  The caller waits for the workgroup before it
+// uses them.
+__device__ __forceinline__ void load_pages(int64_t* pages, int* bad, const PagedParams& p, const PagedItem& w, bool last, int k0, int kend, int row_bytes,
+                                           int tid, int nt) {
     __syncthreads();  // the window before is no longer read
     if (tid == 0) *bad = 0;
     __syncthreads();
@@ -196,7 +198,7 @@ __device__ __forceinline__ void load_pages(int64_t* pages, int* bad, const Paged
         if (id >= 0 && id < p.pages) at = (((int64_t)id * p.Hkv + w.hk) << p.page_log2) * row_bytes;
         else {
             *bad = 1;
-            if (w.hk == 0 && w.tile == 0) atomicAdd(&g_bad_pages, 1u);
+            if (w.hk == 0 && last) atomicAdd(&g_bad_pages, 1u);
         }
         pages[i] = at;
     }
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2
         }
         for (int win = w.kbegin, wend; win < w.kend; win = wend) {
             wend = window_end(p, win, w.kend);
-            load_pages(pages, &s_bad, p, w, win, wend, E4M3 ? DH : 2 * DH, tid, 256);
+            load_pages(pages, &s_bad, p, w, (tile + 1) * 32 * R >= nrows, win, wend, E4M3 ? DH : 2 * DH, tid, 256);
             __syncthreads();  // pages, rows
             const bool good = s_bad == 0;
             const int first_page = win >> p.page_log2;
@@ -543,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
         landed(qf);
         for (int win = w.kbegin, wend; win < end; win = wend) {
             wend = window_end(p, win, w.kend);
-            load_pages(pages, &s_bad, p, w, win, wend, E4M3 ? DH : 2 * DH, tid, 256);  // (the images are free from here on, too)
+            load_pages(pages, &s_bad, p, w, (tile + 1) * 128 >= nrows, win, wend, E4M3 ? DH : 2 * DH, tid, 256);  // (the images are free from here on, too)
             __syncthreads();
             const bool good = s_bad == 0;
             const int first_page = win >> p.page_log2, nt = (min(end, wend) - win + BN - 1) / BN;

@@ -272,6 +272,26 @@ def test_bad_pages_slots_and_lengths_are_skipped_and_counted(new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,heads,page,entry", [(1000, 1, 16, 50), (4200, 64, 8, 520)], ids=["split", "window"])
+def test_bad_pages_that_only_later_rows_see_are_counted(tokens, heads, page, entry):
+    """A whole prompt at once: its first tile of rows neither sees the later splits of the keys nor the later windows of pages."""
+    ops = _ops()
+    ops.check_pages()
+    dh = 64
+    cache, table, _, _ = _filled([tokens], [tokens], heads, page, dh, BF16, 12)
+    q = torch.randn(tokens, heads * dh, generator=torch.Generator().manual_seed(3)).to(BF16).to(DEV)
+    lens, cu = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([tokens], [0, tokens]))
+    whole = ops.attn_paged(q, cache, table, lens, heads, cu_q=cu, max_q=tokens)
+    ops.check_pages()
+    table[0, entry] = -1
+    got = ops.attn_paged(q, cache, table, lens, heads, cu_q=cu, max_q=tokens)
+    with pytest.raises(IndexError):
+        ops.check_pages()
+    first = entry * page
+    assert torch.equal(got[:first], whole[:first]) and not torch.equal(got[first:], whole[first:]) and bool(got.isfinite().all())
+
+
+@pytest.mark.gpu
 def test_slots_of_positions_and_pages_that_do_not_exist():
     ops = _ops()
     ops.check_pages()

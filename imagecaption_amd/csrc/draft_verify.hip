@@ -141,7 +141,9 @@ __global__ __launch_bounds__(VWAVES * 64) void draft_verify_kernel(VerifyParams 
                 const double x = shfl_up_d(upto, o);
                 if (lane >= o) upto += x;
             }
-            const unsigned long long hit = __ballot(run + upto > t);
+            // (the scan sums each lane's part in an order of its own: a lane without weight may be the first to pass t, by a last
+            // bit -- it holds no token to take)
+            const unsigned long long hit = __ballot(mine > 0.0 && run + upto > t);
             if (hit) {
                 found = true;
                 const int first = __ffsll(hit) - 1;

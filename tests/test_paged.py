@@ -486,6 +486,54 @@ def test_verification_edges():
     assert out.tolist() == [[5, 5], [9, 0], [0, 0], [4, 0]]
 
 
+def _scan(x):
+    """Running sums over 64 lanes in the order of a scan by doubling distances."""
+    x, o = x.copy(), 1
+    while o < 64:
+        x[o:] = x[o:] + x[:-o].copy()
+        o *= 2
+    return x
+
+
+def _an_inversion():
+    """256 weights with four zeros in one lane at which the scan's sum is one last bit above the lane before, that lane, and
+    weights to go behind them whose total makes half of everything equal to the sum before the zeros."""
+    rng = np.random.default_rng(0)
+    for _ in range(20000):
+        w = (rng.random(256) * 2.0 ** rng.integers(-30, 0, 256)).astype(np.float32)
+        lane = int(rng.integers(2, 60))
+        w[4 * lane:4 * lane + 4] = 0
+        d = w.astype(np.float64).reshape(64, 4)
+        mine = ((d[:, 0] + d[:, 1]) + d[:, 2]) + d[:, 3]
+        upto, total = _scan(mine), mine.copy()
+        for o in (32, 16, 8, 4, 2, 1):
+            total = total + total[np.arange(64) ^ o]
+        border = upto[lane - 1]
+        rest, left = [], 2 * border - total[0]
+        for _ in range(3):  # 53 bits as three numbers of 24
+            rest.append(np.float32(left))
+            left -= float(rest[-1])
+        behind = float(rest[0]) + float(rest[1]) + float(rest[2])
+        if int(np.argmax(upto > border)) == lane and left == 0 and min(rest) > 0 and total[0] + behind == 2 * border:
+            return w, lane, rest
+    raise AssertionError("no such weights")
+
+
+@pytest.mark.gpu
+def test_a_draw_on_the_border_of_tokens_without_weight():
+    """The draw falls on the border to four tokens of weight zero, where a sum of another order is one last bit higher: it takes
+    a neighbour of the border, not whatever token comes last."""
+    ops = _ops()
+    w, lane, rest = _an_inversion()
+    target = torch.zeros(1, 1, 4096)
+    target[0, 0, :256] = torch.from_numpy(w)
+    target[0, 0, 300:303] = torch.from_numpy(np.array(rest))
+    none = torch.zeros(1, 0, device=DEV)
+    out, acc = ops.draft_verify(target.to(DEV), None, none.long(), none, torch.tensor([0.5], device=DEV))
+    below, above = np.flatnonzero(w[:4 * lane])[-1], 4 * lane + 4 + np.flatnonzero(w[4 * lane + 4:])[0]
+    assert acc.tolist() == [0] and out.item() in (below, above), (out.item(), below, above)
+
+
 # ---- a program that uses them together ---------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [E4M3, BF16], ids=["e4m3", "bf16"])

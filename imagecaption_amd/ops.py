@@ -1180,7 +1180,8 @@ def kv_cache_write(cache, k, v, slots):
 
 def kv_cache_read(cache, slots, k=None, v=None, dtype=torch.bfloat16):
     """(k, v): the rows of ``slots`` (int32 [rows]; negative: zeros) as [rows, heads * dh] matrices of ``dtype`` (or into given
-    ones, both of one type)."""
+    ones, both of one type).  Rows of a given matrix behind the slots stay as they are; a new ``v`` beside a given ``k`` is as
+    high as it, with zeros there."""
     fast = _capi.fast
     if fast is not None and k is None and v is None and dtype in _ES:
         cur = _capi._cur_device()
@@ -1191,8 +1192,11 @@ def kv_cache_read(cache, slots, k=None, v=None, dtype=torch.bfloat16):
     if k is None:
         shape = (slots.numel(), cache.heads * cache.dh)
         k = cache.k.new_empty(shape, dtype=dtype if v is None else v.dtype)
-    v = torch.empty_like(k, memory_format=torch.contiguous_format) if v is None else v
+    new = v is None
+    v = torch.empty_like(k, memory_format=torch.contiguous_format) if new else v
     rows, dt, pk, lk, pv, lv, ps = _cache_rows("kv_cache_read", cache, k, v, slots)
+    if new and v.shape[0] > rows:
+        v[rows:].zero_()
     check(lib().capdec_kv_read(cache.cref, ps, rows, pk, lk, pv, lv, dt, stream()), "capdec_kv_read")
     return k, v
 

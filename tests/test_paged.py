@@ -101,6 +101,22 @@ def test_rows_of_zeros_tiny_values_and_non_finite_values():
     assert bool((k[4] / 3.3e38 - 1).abs().max() < 2.0 ** -4) and k[5, 0] == 1.0 and bool((k[5, 1:] == 0).all())
 
 
+@pytest.mark.gpu
+def test_rows_behind_the_slots_of_a_new_matrix_are_zeros():
+    """Keys read into a given matrix with more rows than slots: its rows behind them stay, the new matrix of values has zeros."""
+    ops = _ops()
+    rows, slots = torch.ones(3, 2 * 64, dtype=BF16, device=DEV), torch.arange(3, dtype=torch.int32, device=DEV)
+    cache = ops.PagedKVCache.new(2, 2, 16, 64, BF16, DEV)
+    ops.kv_cache_write(cache, rows, rows, slots)
+    for given in "kv":
+        block = torch.full((50, 2 * 64), 7.0, dtype=BF16, device=DEV)
+        torch.full((50, 2 * 64), 9.0, dtype=BF16, device=DEV)  # memory that held something else
+        k, v = ops.kv_cache_read(cache, slots, **{given: block})
+        new = v if given == "k" else k
+        assert (k if given == "k" else v) is block and bool((block[3:] == 7).all())
+        assert bool((k[:3] == 1).all()) and bool((v[:3] == 1).all()) and bool((new[3:] == 0).all())
+
+
 # ---- attention over the cache ---------------------------------------------------------------------------------------------
 def _filled(new, total, heads, page, dh, dtype, seed, cols=0, extra_pages=2):
     """A cache whose unused places hold NaN, filled through its own write; (cache, table, dense k, v [sum total, heads * dh])."""

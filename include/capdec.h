@@ -416,7 +416,8 @@ int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ld
  *   that may overlap in time.  Fixed summation orders: bitwise reproducible for given arguments.
  * Slots and pages outside the cache, and lengths past the page table, are never followed: a bad slot is skipped / reads as
  * zeros, a position on a bad page counts as unseen, a length is cut to the table.  capdec_kv_bad_pages counts them (wave-wise,
- * at least one for every bad entry met) on the current device since the last reset; it synchronises the device.
+ * at least one for every bad entry met) on the current device since the last reset; it synchronises the device, so
+ * no stream may be under capture then (the capture would be lost).
  * The dense counterpart is capdec_decode_attn; the reference re-runs the whole prefix instead (ref train.py:312-332). */
 typedef struct capdec_kv_cache {
     void *k, *v;

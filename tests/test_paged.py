@@ -790,3 +790,22 @@ def test_tensors_that_do_not_fit_are_refused():
             ops.draft_verify(*args)
     with pytest.raises(CapdecError):
         ops.draft_verify(p, p[:, :2], tok, u, us, num_draft=torch.zeros(3, dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.gpu
+def test_pages_are_not_checked_under_capture():
+    """The check reads counters on the host: refused while a graph is captured, and the capture goes on."""
+    from imagecaption_amd._capi import CapdecError
+    ops = _ops()
+    ops.check_pages()
+    x = torch.zeros(4, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(CapdecError, match="captured"):
+            ops.check_pages()
+        x += 1
+    for turn in range(1, 4):
+        graph.replay()
+        assert x.tolist() == [2.0 * turn] * 4
+    ops.check_pages()

@@ -92,7 +92,7 @@ at::Tensor new_like(const Matrix& m, int64_t width, const at::Tensor& like) { re
 
 PyObject* none() { Py_RETURN_NONE; }
 
-// something was thrown (an unusual tensor, no memory): the general way meets and reports the same
+// something was thrown (an unusual tensor, no memory) or raised: the general way meets and reports the same
 PyObject* refused() {
     PyErr_Clear();
     return none();
@@ -149,7 +149,8 @@ PyObject* attn_packed_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) try {
     const float scale = x.scale(7, p.dh);
     void* stream = x.address(9);
     const int save = PyObject_IsTrue(a[6]);
-    if (!x.ok || save < 0) return none();
+    if (save < 0) return refused();
+    if (!x.ok) return none();
     const at::Tensor& q = THPVariable_Unpack(a[1]);
     at::Tensor o = new_like(p.q, p.Hq * p.dh, q), lse;
     if (save) lse = at::empty({p.Hq, p.q.rows}, q.options().dtype(at::kFloat));

@@ -519,3 +519,14 @@ def test_tensors_that_do_not_fit_are_refused():
             ops.attn_packed_fwd(wide.as_strided((2, Hq * dh), (far, 1)), k, v, Hq, Hkv, two)
     with pytest.raises(CapdecError):
         ops.attn_packed_bwd(q, k, v, o, do, lse, Hq, Hkv, seqs, dk=torch.zeros(14, 64, dtype=torch.bfloat16, device=DEV))
+
+
+@pytest.mark.gpu
+def test_an_argument_without_a_truth_value_is_its_own_error():
+    import numpy as np
+    ops = _ops()
+    q, k, v, _ = (t.contiguous() for t in _inputs([5, 9], [5, 9], 4, 2, 64, torch.bfloat16, 51))
+    seqs = ops.PackedSeqs([5, 9], device=DEV)
+    ops.attn_packed_fwd(q, k, v, 4, 2, seqs)
+    with pytest.raises(ValueError, match="truth value"):
+        ops.attn_packed_fwd(q, k, v, 4, 2, seqs, save_lse=np.array([1, 0]))

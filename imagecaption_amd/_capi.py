@@ -179,10 +179,11 @@ def lib():
             fn = getattr(l, name)  # AttributeError if the .so does not export a declared symbol
             fn.restype, fn.argtypes = res, args
         _lib = l
-        if _raw_stream is not None:
+        from .build import calls_fit
+        if _raw_stream is not None and calls_fit():  # not built, or for another torch: the same calls through ctypes, at more host time
             try:
                 from . import _calls
-            except ImportError:  # not built, or built for another torch: the same calls through ctypes, at more host time
+            except ImportError:
                 pass
             else:
                 _calls.bind(*(C.cast(getattr(l, "capdec_" + n), C.c_void_p).value for n in _DIRECT))

@@ -91,16 +91,31 @@ def build(force=False, verbose=True):
     return LIB
 
 
+def calls_stamp():
+    """What a build of csrc/calls.cpp was made for: it reads torch's objects by their layout, and no loader checks that."""
+    import torch
+    return f"capdec calls for torch {torch.__version__} {torch.version.git_version} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} {sys.implementation.cache_tag};"
+
+
+def calls_fit():
+    """Whether _calls.so is there and was built for the running torch and Python (its stamp is read, nothing of it is run)."""
+    if not os.path.exists(CALLS):
+        return False
+    with open(CALLS, "rb") as f:
+        return calls_stamp().encode() in f.read()
+
+
 def build_calls(force=False, verbose=True):
     """csrc/calls.cpp -> _calls.so: host code only, built against the installed torch."""
     import sysconfig
     import torch
     src = os.path.join(CSRC, "calls.cpp")
-    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), _deps_mtime()):
+    if not force and calls_fit() and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), _deps_mtime()):
         return
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DCAPDEC_CALLS_STAMP="{calls_stamp()}"']
     cmd += ["-isystem" + i for i in inc] + [src, "-o", CALLS, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

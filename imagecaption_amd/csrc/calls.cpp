@@ -14,6 +14,9 @@
 
 #include "../../include/capdec.h"
 
+// the torch and the Python this was built for; build.py looks for it in the file before anything is loaded
+extern "C" __attribute__((used, visibility("default"))) const char capdec_calls_stamp[] = CAPDEC_CALLS_STAMP;
+
 namespace {
 
 struct Entry {

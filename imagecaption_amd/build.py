@@ -6,8 +6,10 @@ Each ``csrc/*.hip`` is compiled to an object under ``csrc/_build/`` (skipped whe
 linked into ``imagecaption_amd/libcapdec.so``.  hipcc cross-compiles for gfx950 without a GPU.
 """
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -105,13 +107,34 @@ def calls_fit():
         return calls_stamp().encode() in f.read()
 
 
+def _calls_need():
+    """What a build of csrc/calls.cpp needs and this machine lacks; None: nothing."""
+    try:
+        import torch
+    except ImportError:
+        return "torch"
+    if shutil.which("g++") is None:
+        return "g++"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python.h"
+    if not os.path.exists(os.path.join(os.path.dirname(torch.__file__), "include", "torch", "csrc", "autograd", "python_variable.h")):
+        return "torch's headers"
+    return None
+
+
 def build_calls(force=False, verbose=True):
-    """csrc/calls.cpp -> _calls.so: host code only, built against the installed torch."""
-    import sysconfig
-    import torch
-    src = os.path.join(CSRC, "calls.cpp")
-    if not force and calls_fit() and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), _deps_mtime()):
+    """csrc/calls.cpp -> _calls.so: host code only, built against the installed torch.  It saves host time; without it the
+    same calls go through ctypes, so a machine that has hipcc alone gets the library without it."""
+    src, missing = os.path.join(CSRC, "calls.cpp"), _calls_need()
+    if missing != "torch" and not force and calls_fit() and os.path.getmtime(CALLS) >= max(os.path.getmtime(src), _deps_mtime()):
         return
+    if missing is not None:
+        if os.path.exists(CALLS):  # made for another torch, or from older sources than the library
+            os.remove(CALLS)
+        if verbose:
+            print(f"[capdec build] no {missing}: the direct calls ({os.path.basename(CALLS)}) are not built")
+        return
+    import torch
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",

@@ -312,9 +312,10 @@ struct DmaTile : AttTile<__bf16, DH> {
         }
     };
 };
-// every transfer of this wave has landed, and every wave of the workgroup has come this far
+// every transfer of this wave has landed, and every wave of the workgroup has come this far and has its reads of the images:
+// the compiler places its own waits where a value is used, which may be behind a barrier that it does not see as one of memory
 __device__ __forceinline__ void dma_sync() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }

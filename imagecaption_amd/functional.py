@@ -190,8 +190,8 @@ class AttnPackedFn(torch.autograd.Function):
 
 
 def attn_packed(q, k, v, Hq, Hkv, seqs, scale=None):
-    """Differentiable ops.attn_packed_fwd: q [rows, Hq * dh], k / v [rows, Hkv * dh], ``seqs`` an ops.PackedSeqs -> o.  First
-    derivatives only.  Where a backward pass is captured into a graph, no eager graph over the same leaves may be alive."""
+    """Differentiable ops.attn_packed_fwd: q [rows, Hq * dh], k / v [rows, Hkv * dh], ``seqs`` an ops.PackedSeqs -> o.  No
+    dropout of the probabilities.  First derivatives only.  Where a backward pass is captured into a graph, no eager graph over the same leaves may be alive."""
     return AttnPackedFn.apply(q, k, v, Hq, Hkv, seqs, scale)
 
 

@@ -931,8 +931,9 @@ class PackedSeqs:
     """Lengths of the sequences that lie back to back in the rows of packed matrices, and the tile table that the packed
     attention kernels walk on the device: made once for a set of lengths, used by every layer and both directions.
     ``lengths_k`` None: keys / values have the queries' lengths.  ``causal``: row i of nq sees the rows j <= i + nk - nq
-    of its sequence.  Makes a blocking copy to ``device`` (not under graph capture).  A graph that captured calls with it reads
-    its table at every replay: keep it as long as the graph."""
+    of its sequence.  Waits for the current stream and makes a blocking copy to ``device`` (not under graph capture), so a loop
+    whose lengths change every step drains its stream there once a step; make the plans of known lengths ahead.  A graph that
+    captured calls with it reads its table at every replay: keep it as long as the graph."""
 
     def __init__(self, lengths_q, lengths_k=None, causal=True, device="cuda"):
         lq = [int(v) for v in lengths_q]
@@ -1032,7 +1033,7 @@ def _packed_args(name, q, k, v, Hq, Hkv, seqs, scale):
 
 def attn_packed_fwd(q, k, v, Hq, Hkv, seqs, out=None, save_lse=True, scale=None):
     """Attention over packed sequences: q [>= rows_q, Hq * dh], k / v [>= rows_k, Hkv * dh] (row-strided views, all fp32 or
-    all bf16, dh 64 or 128), ``seqs`` a PackedSeqs.  Returns (o, lse [Hq, rows of q] or None).  Rows behind the last sequence
+    all bf16, dh 64 or 128), ``seqs`` a PackedSeqs; scaled scores within +-2^24.  Returns (o, lse [Hq, rows of q] or None).  Rows behind the last sequence
     stay as they are in a given ``out`` (which must not overlap q, k or v) and are zeros in a new one."""
     fast = _capi.fast
     if fast is not None and out is None:

@@ -356,11 +356,16 @@ int capdec_attn_bwd_bf16(const void* q16, int ldq, const void* k16, int ldk, con
  *   fwd.  scratch: capdec_attn_packed_scratch_bytes bytes (NULL if that is 0), 16-byte aligned, needs no clearing, not to be
  *   shared by calls that may overlap in time.
  *   bwd: dq, dk, dv from do; dk / dv sum over the query heads of their group.  No atomics: bitwise reproducible.
- *   scale between 2^-60 and 2^60.  Results must not overlap the matrices that are read; fewer than 2^31 - 1024 rows a side.
+ *   scale between 2^-60 and 2^60.  Scores and statistics are fp32: a weight is off by about 2^-23 of its row's largest scaled
+ *   score, relative to itself, so scaled scores have to stay within +-2^24 -- there they no longer tell a factor of e from another,
+ *   and from 2^28 on a row may come out as NaN or as one that sees nothing.
+ *   No dropout of the probabilities: what trains with it (capdec_attn_fwd's drop_p) stays on the padded form.
+ *   Results must not overlap the matrices that are read; fewer than 2^31 - 1024 rows a side.
  * dtype CAPDEC_F32: every matrix fp32, exact fp32 products; CAPDEC_BF16S: every matrix bf16, fp32 accumulation, softmax and
  * statistics; probabilities and score gradients are rounded to bf16 for the products that take them -- to 16 bits, two bf16
- * terms, where most sequences (backward: all) fit 32 rows --, the only roundings besides the results'.  dh in {64, 128};
- * 16-byte aligned matrices, row strides multiples of 16 bytes, at most 2^25 bytes.  Non-finite values:
+ * terms, where most sequences of the plan (backward: all) fit 32 rows --, the only roundings besides the results'.  So the other
+ * sequences of its batch may decide how a sequence's weights are rounded: its result is within the same bounds, not the same bits.
+ * dh in {64, 128}; 16-byte aligned matrices, row strides multiples of 16 bytes, at most 2^25 bytes.  Non-finite values:
  * the products are plain ones (0 x inf = NaN), so an infinity or NaN in v reaches the rows of ITS sequence that share a
  * tile with it even where they are masked; it never reaches another sequence.
  * The plan: capdec_packed_plan checks the lengths (host arrays; lens_k = NULL: the same as lens_q), writes the tile table to
@@ -408,7 +413,8 @@ int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ld
  *   to bf16 for the context product (after the value's scale is multiplied in; to 16 bits, two bf16 terms, up to 64 rows a key /
  *   value head), the result once.  A token that sees nothing
  *   gets o = 0, lse = -inf; lse (fp32 [Hq, rows]) may be NULL.  Rows of no sequence stay as they are in lse,
- *   and in o too unless `clear` is set: then they get zeros.  scale between 2^-60 and 2^60.  Positions past kv_lens are never read, whatever their slots hold; an infinity or NaN among the values of
+ *   and in o too unless `clear` is set: then they get zeros.  scale between 2^-60 and 2^60, scaled scores within +-2^24 as in
+ *   capdec_attn_packed_fwd.  Positions past kv_lens are never read, whatever their slots hold; an infinity or NaN among the values of
  *   a seen position reaches the new tokens of ITS sequence that do not see it yet as well (0 x inf), no other sequence.
  *   Everything that varies from step to step (cu_q, kv_lens, page_table) is read on the device, so a captured call can be
  *   replayed with new contents.  The keys are split over workgroups and joined in a second launch when there are few rows;

@@ -530,3 +530,19 @@ def test_an_argument_without_a_truth_value_is_its_own_error():
     ops.attn_packed_fwd(q, k, v, 4, 2, seqs)
     with pytest.raises(ValueError, match="truth value"):
         ops.attn_packed_fwd(q, k, v, 4, 2, seqs, save_lse=np.array([1, 0]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lq", [[20, 9, 32], [300, 70]], ids=["short", "long"])
+def test_scores_up_to_the_documented_size_stay_finite(lq, dtype):
+    """Scaled scores of up to 2^24: weights say little there, but no row becomes NaN or one that sees nothing."""
+    ops = _ops()
+    q, k, v, do = _inputs(lq, lq, 4, 2, 64, dtype, 95)
+    top = max(float((a.float() @ b.float().T).abs().max()) for a in q.split(64, 1) for b in k.split(64, 1))
+    scale = 2.0 ** 24 / top
+    seqs = ops.PackedSeqs(lq, device=DEV)
+    o, lse = ops.attn_packed_fwd(q, k, v, 4, 2, seqs, scale=scale)
+    assert float(lse.abs().max()) > 2.0 ** 20  # the test means something
+    for t in (o, lse, *ops.attn_packed_bwd(q, k, v, o, do, lse, 4, 2, seqs, scale=scale)):
+        assert bool(t.isfinite().all())

@@ -809,3 +809,17 @@ def test_pages_are_not_checked_under_capture():
         graph.replay()
         assert x.tolist() == [2.0 * turn] * 4
     ops.check_pages()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [E4M3, BF16], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("new", [[1, 2, 1], [40, 70, 20]], ids=["few", "many"])
+def test_scores_up_to_the_documented_size_stay_finite(new, dtype):
+    ops = _ops()
+    total, Hq, Hkv = [700, 70, 1200], 4, 2
+    cache, table, k, _ = _filled(new, total, Hkv, 16, 64, dtype, 14)
+    q = torch.randn(sum(new), Hq * 64, generator=torch.Generator().manual_seed(4)).to(BF16).to(DEV)
+    top = max(float((a.float() @ b.float().T).abs().max()) for a in q.split(64, 1) for b in k.split(64, 1))
+    lens, cu = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in (total, [0] + np.cumsum(new).tolist()))
+    o, lse = ops.attn_paged(q, cache, table, lens, Hq, cu_q=cu, max_q=max(new), scale=2.0 ** 24 / top, return_lse=True)
+    assert bool(o.isfinite().all()) and bool(lse.isfinite().all()) and float(lse.abs().max()) > 2.0 ** 20

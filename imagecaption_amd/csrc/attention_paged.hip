@@ -2,12 +2,13 @@
 //
 // The rows of a (sequence, key / value head) are its new tokens times the query heads of the group: they all read the same
 // keys, so they share a tile.  Two kernels, both over (sequence, key / value head, split of the keys, tile of rows):
-//   paged_keys_kernel  few rows (decode steps, drafted tokens): bound by the cache's bytes.  A tile of 32 or 64 rows; each of
-//                      the four waves streams every fourth run of 32 keys through an LDS image of its own (global ->
-//                      registers one run ahead -> LDS, no barrier in the loop) and the waves join at the end.
-//   paged_rows_kernel  many rows (chunks of a prompt): bound by the matrix products.  A tile of 128 rows, 32 a wave; 64
-//                      keys at a time are shared by the waves through LDS.
-// e4m3 codes become bf16 (exactly) on their way into LDS; a key's scale multiplies its scores, a value's scale its weights.
+//   paged_keys_kernel  few rows (decode steps, drafted tokens): bound by the cache's bytes.  A tile of 32 or 64 rows, kept in
+//                      LDS; each of the four waves streams every fourth run of 32 keys: the keys go from registers straight to
+//                      the matrix instructions, the values through an LDS image of the wave's own, no barrier in the loop; the
+//                      waves join at the end.
+//   paged_rows_kernel  many rows (chunks of a prompt): bound by the matrix products.  A tile of 128 rows, 32 a wave, in
+//                      registers; 64 keys and values at a time are shared by the waves through LDS.
+// e4m3 codes become bf16 (exactly) in registers; a key's scale multiplies its scores, a value's scale its weights.
 // Splits leave (maximum, sum, unnormalised context) in fp32 and a second launch joins them; a sequence short enough for one
 // split writes its result at once.
 #include <algorithm>
@@ -314,10 +315,13 @@ __device__ __forceinline__ void hide(f32x16& s, const PagedParams& p, const int6
 
 // (Weights keep 16 bits: bound by the cache's bytes, the kernel has room for the products of their second terms.  8 contexts of 9
 // to 60 thousand tokens: 46 us either way; 48 of 100 to 8000, five tokens each: 21 -> 22.7.)
-// R blocks of 32 rows; every wave walks its own runs of 32 keys, one run ahead in registers.  The rows are the same for all
-// waves and stay in LDS; values pass through an LDS image (their operand is transposed), keys go to the matrix
+// R blocks of 32 rows; every wave walks its own runs of 32 keys, the next run asked for before this one's products.  The rows are
+// the same for all waves and stay in LDS; values pass through an LDS image (their operand is transposed), keys go to the matrix
 // instructions as they come: less LDS for a workgroup and a shorter way through each run, which is what bounds the kernel (a
 // run's steps depend on each other, so the rate is the number of waves a CU holds).
+// An e4m3 run stays in registers until its turn.  The values of a bf16 run do not: PageStage's array of uint4 is copied whole, and
+// this compiler keeps it in private memory (160 bytes a lane at 128 dims, 96 at 64), so the wave waits for the next run's values,
+// and for its keys before them, as soon as it has asked for them, and the values move three times.
 template <bool E4M3, int DH, int R>
 __global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2)) void paged_keys_kernel(PagedParams p) {
     using L = AttTile<__bf16, DH>;
@@ -513,7 +517,8 @@ __global__ __launch_bounds__(256, DH == 128 ? (R == 1 ? 2 : 1) : (R == 1 ? 3 : 2
 }
 
 // 128 rows, 32 a wave; 64 keys at a time shared by the waves.  bf16 pages travel by DMA one tile ahead; e4m3 pages pass
-// through registers, where they become bf16.
+// through registers, where they become bf16.  (At 128 dims a wave is at its 256 registers: two are spilled for bf16 pages, four
+// for e4m3; they are stored before the walk over the keys and taken back behind it.)
 template <bool E4M3, int DH>
 __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedParams p) {
     using L = AttTile<__bf16, DH>;

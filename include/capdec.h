@@ -400,8 +400,8 @@ int capdec_attn_packed_bwd(const capdec_packed_seqs* seqs, const void* q, int ld
  * table[j / page] * page + j % page.  page is a power of two from 8 to 256, dh 64 or 128, pages * page < 2^31.
  *   CAPDEC_BF16S  bf16 rows;
  *   CAPDEC_E4M3   rounded as they are written: scale = max(amax |x|, 2^-100) / 448 (fp32, one for every row of a head, in
- *                 k_scale / v_scale [pages, heads, page]), code = e4m3(x / scale), value code * scale.  A row that holds an
- *                 infinity or a NaN reads back as NaN throughout.
+ *                 k_scale / v_scale [pages, heads, page]), code = e4m3(x / scale), value code * scale; a negative zero is
+ *                 kept as zero.  A row that holds an infinity or a NaN reads back as NaN throughout.
  * capdec_kv_write: row r of k / v ([rows, heads * dh], fp32 or bf16 by `dtype`) goes to slots[r]; a negative slot is skipped.
  *   The slots of one call must differ: of two rows sent to one slot, which one each element comes from is not defined.
  * capdec_kv_read: the rows back as fp32 or bf16 (rounded once); a negative slot reads as zeros.

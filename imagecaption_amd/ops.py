@@ -1206,7 +1206,7 @@ def check_pages():
     """Raise IndexError if kernels on the current device have met slots or pages outside their cache, or lengths past their
     page table, since the last check: such entries are never followed, only counted.  Synchronises, so it is refused while the
     current stream is captured, and must not be called while another one is."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
         raise _capi.CapdecError("check_pages: the counters are read on the host and cannot be captured; check between the replays")
     n = C.c_uint(0)
     check(lib().capdec_kv_bad_pages(C.byref(n), 1), "capdec_kv_bad_pages")

@@ -823,3 +823,11 @@ def test_scores_up_to_the_documented_size_stay_finite(new, dtype):
     lens, cu = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in (total, [0] + np.cumsum(new).tolist()))
     o, lse = ops.attn_paged(q, cache, table, lens, Hq, cu_q=cu, max_q=max(new), scale=2.0 ** 24 / top, return_lse=True)
     assert bool(o.isfinite().all()) and bool(lse.isfinite().all()) and float(lse.abs().max()) > 2.0 ** 20
+
+
+def test_pages_are_checked_where_there_is_a_gpu():
+    from imagecaption_amd._capi import CapdecError
+    if torch.cuda.is_available():
+        pytest.skip("there is a GPU")
+    with pytest.raises(CapdecError):
+        _ops().check_pages()
